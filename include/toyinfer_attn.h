@@ -365,6 +365,109 @@ int toyinfer_sample_topk_topp_f32(const float* logits, uint32_t vocab, float tem
                                   uint32_t* out_token, void* workspace, size_t workspace_bytes,
                                   void* stream);
 
+/* ------------------------------------------------ many requests: paged cache
+ * Extension: the reference serves one sequence at a time from one contiguous
+ * cache per layer (src/transformer.cpp:320-681).  Here a layer's K and V cache
+ * are pages of page_size rows, row r of page p and KV head h at
+ * p*page_stride + (r*Hkv + h)*D elements (page_stride >= page_size*Hkv*D and a
+ * multiple of 8, so the two caches may share one array, a page of K beside one
+ * of V).  block_tables [batch][max_blocks] names each request's pages in order;
+ * "slot" s is row s % page_size of page s / page_size.  page_size is a power of
+ * two in 8..65536; D in {64, 128}; bf16 tensors 16-byte aligned, uint32 arrays
+ * 4-byte aligned.  Lengths, tables, positions and slots are read on the device
+ * when the kernels run, so a captured step replays with other requests.  Each
+ * new token is one row of q, k, v and o, the requests' rows back to back from
+ * row 0 in request order.
+ * Limits: batch <= TOYINFER_PAGED_MAX_BATCH; num_tokens * Hq/Hkv < 2^31;
+ * max_blocks * page_size < 2^31; num_pages * page_size < 2^32
+ * (TOYINFER_ERR_UNSUPPORTED beyond). */
+#define TOYINFER_PAGED_MAX_BATCH 4096u
+
+/* Block tables, positions and slots of one step from the requests' lengths:
+ * request b has context_lens[b] tokens in the cache, the pages of which its
+ * row of block_tables names, and new_lens[b] new ones (0 allowed).  The pages
+ * that they need are taken from the top of a stack, free_pages[*num_free - 1]
+ * downwards, in request order, and appended to the row (other entries are left
+ * as they are).
+ *   query_start [batch+1]   first token row of each request, then their number
+ *   seq_lens [batch]        context_lens + new_lens
+ *   positions [num_tokens]  of each token row in its sequence
+ *   slot_mapping [num_tokens]
+ *   status [2]              pages left on the stack; requests refused
+ * A request is refused whose pages the stack does not hold after the requests
+ * before it (refused ones counted), whose row would pass max_blocks or whose
+ * token rows would pass num_tokens: it takes no page, seq_lens[b] =
+ * context_lens[b], and its token rows get slot 0xFFFFFFFF.  Token rows past the
+ * last request's get position 0 and slot 0xFFFFFFFF.  *num_free counts at most
+ * free_capacity pages.  No output may overlap an input or another output. */
+int toyinfer_paged_tables_u32(const uint32_t* context_lens, const uint32_t* new_lens,
+                              uint32_t batch, const uint32_t* free_pages, uint32_t free_capacity,
+                              const uint32_t* num_free, uint32_t page_size,
+                              uint32_t* block_tables, uint32_t max_blocks, uint32_t num_tokens,
+                              uint32_t* query_start, uint32_t* seq_lens, uint32_t* positions,
+                              uint32_t* slot_mapping, uint32_t* status, void* stream);
+
+/* toyinfer_decode_qkv_prologue_bf16 for num_tokens tokens at positions and
+ * cache slots of their own: per-head RMSNorm and RoPE of q [num_tokens][Hq][D]
+ * into q_out (which may be q) and of k [num_tokens][Hkv][D] into k_cache, v
+ * copied into v_cache.  Norm and rotation are computed in fp32 and rounded
+ * once (the unfused calls round the norm's result too).  Angles from
+ * rope_cos_sin [num_positions][D/2][2] (toyinfer_rope_cos_sin_f32, 16-byte
+ * aligned); a position >= num_positions uses the last row.  A token whose slot
+ * is not below num_pages * page_size writes q_out only.  Slots of one call are
+ * distinct (of tokens that share one, either's bytes may stay).  The caches
+ * overlap neither each other's rows nor q, k, v and q_out. */
+int toyinfer_paged_qkv_prologue_bf16(const void* q, const void* k, const void* v,
+                                     const void* q_norm_weight, const void* k_norm_weight,
+                                     const float* rope_cos_sin, uint32_t num_positions,
+                                     const uint32_t* positions, const uint32_t* slot_mapping,
+                                     uint32_t num_tokens, float rms_norm_eps, void* q_out,
+                                     void* k_cache, void* v_cache, uint32_t num_pages,
+                                     uint32_t page_size, uint64_t page_stride,
+                                     uint32_t num_q_heads, uint32_t num_kv_heads,
+                                     uint32_t head_dim, void* stream);
+
+/* Attention of the new tokens over the paged cache, which already holds their
+ * own K and V: a whole prompt, a chunk of one, a decoded token (a chunk of
+ * one) and several drafted ones, mixed in one batch.  Token row i of request b
+ * (rows query_start[b] .. query_start[b+1]) stands at position p = seq_lens[b]
+ * - (query_start[b+1] - query_start[b]) + i and sees the keys j <= p with
+ * window == 0, or p - j < window, or j < sinks: a sliding window with the first
+ * `sinks` tokens kept in sight.  o = softmax(q.k / sqrt(D)) v over those; a row
+ * that sees none (p < 0) gives 0, and what a row does not see, infinities and
+ * NaN included, does not reach it.  Rows past query_start[batch] are left as
+ * they are.  o overlaps neither q nor the caches.
+ *
+ * The plan is the step's work list.  toyinfer_paged_attention_plan builds it on
+ * the device from the lengths (one launch, shared by the layers' calls, in
+ * stream order); an attention call whose sizes are not those of its plan fills
+ * o with NaN.  Both take lengths of any content: query_start is read up to
+ * num_tokens, seq_lens up to max_blocks * page_size, and a page number >=
+ * num_pages as the last page.
+ * plan: toyinfer_paged_attention_plan_bytes() bytes; workspace:
+ * toyinfer_paged_attention_workspace_bytes() bytes (independent of the
+ * lengths); both 256-byte aligned, without initialisation.  Calls that share a
+ * workspace must be ordered on one stream. */
+size_t toyinfer_paged_attention_plan_bytes(uint32_t batch, uint32_t num_tokens,
+                                           uint32_t num_q_heads, uint32_t num_kv_heads,
+                                           uint32_t heads_dim);
+size_t toyinfer_paged_attention_workspace_bytes(uint32_t num_q_heads, uint32_t num_kv_heads,
+                                                uint32_t heads_dim);
+int toyinfer_paged_attention_plan(const uint32_t* query_start, const uint32_t* seq_lens,
+                                  uint32_t batch, uint32_t num_tokens, uint32_t page_size,
+                                  uint32_t max_blocks, uint32_t window, uint32_t sinks,
+                                  uint32_t num_q_heads, uint32_t num_kv_heads,
+                                  uint32_t heads_dim, void* plan, size_t plan_bytes,
+                                  void* stream);
+int toyinfer_paged_attention_bf16(const void* q, const void* k_cache, const void* v_cache, void* o,
+                                  const uint32_t* block_tables, const void* plan,
+                                  size_t plan_bytes, uint32_t batch, uint32_t num_tokens,
+                                  uint32_t num_pages, uint32_t page_size, uint64_t page_stride,
+                                  uint32_t max_blocks, uint32_t window, uint32_t sinks,
+                                  uint32_t num_q_heads, uint32_t num_kv_heads,
+                                  uint32_t heads_dim, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -77,6 +77,18 @@ SIGNATURES = {
     "toyinfer_sample_workspace_bytes": (_sz, []),
     "toyinfer_sample_topk_topp_f32": (_i32, [_vp, _u32, _f32, _u32, _f32, _vp, _vp, _vp, _sz,
                                              _vp]),
+    "toyinfer_paged_tables_u32": (_i32, [_vp, _vp, _u32, _vp, _u32, _vp, _u32, _vp, _u32, _u32, _vp,
+                                         _vp, _vp, _vp, _vp, _vp]),
+    "toyinfer_paged_qkv_prologue_bf16": (
+        _i32, [_vp, _vp, _vp, _vp, _vp, _vp, _u32, _vp, _vp, _u32, _f32, _vp, _vp, _vp, _u32, _u32,
+               _u64, _u32, _u32, _u32, _vp]),
+    "toyinfer_paged_attention_plan_bytes": (_sz, [_u32, _u32, _u32, _u32, _u32]),
+    "toyinfer_paged_attention_workspace_bytes": (_sz, [_u32, _u32, _u32]),
+    "toyinfer_paged_attention_plan": (_i32, [_vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _u32,
+                                             _u32, _u32, _vp, _sz, _vp]),
+    "toyinfer_paged_attention_bf16": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _u32, _u32, _u32,
+                                             _u32, _u64, _u32, _u32, _u32, _u32, _u32, _u32, _vp,
+                                             _sz, _vp]),
     "toyinfer_decode_qkv_prologue_bf16": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _f32,
                                                  _vp, _vp, _vp, _u32, _u32, _u32, _vp]),
 }
@@ -475,3 +487,129 @@ def sample_topk_topp_f32(logits, vocab: int, temperature: float, top_k: int, top
                                              workspace.numel() * workspace.element_size(),
                                              _stream(stream)))
 
+
+# ------------------------------------------------------------- paged cache
+
+def _need(fn: str, dtype: str, *pairs) -> None:
+    """Each (tensor, elements): on the current device, dense, of the dtype
+    ("bf16", "u32" as int32 or uint32, "f32", "any") and holding at least that
+    many elements.  The C ABI sees addresses only."""
+    import torch
+
+    types = {"bf16": (torch.bfloat16,), "u32": (torch.int32, torch.uint32),
+             "f32": (torch.float32,)}.get(dtype)
+    device = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for t, n in pairs:
+        if (not t.is_contiguous() or t.numel() < n or t.get_device() != device or device < 0
+                or (types and t.dtype not in types)):
+            raise ToyInferError(fn, ERR_INVALID_ARGUMENT)
+
+
+def _need_cache(fn: str, num_pages: int, page_size: int, page_stride: int, num_kv_heads: int,
+                head_dim: int, *caches) -> None:
+    """Caches may be views with pages further apart than a page is long; what
+    they span from their first element has to lie in their storage."""
+    import torch
+
+    span = (num_pages - 1) * page_stride + page_size * num_kv_heads * head_dim
+    for t in caches:
+        room = t.untyped_storage().nbytes() // 2 - t.storage_offset()
+        if t.dtype is not torch.bfloat16 or room < span or not t.is_cuda:
+            raise ToyInferError(fn, ERR_INVALID_ARGUMENT)
+
+
+def paged_tables_u32(context_lens, new_lens, batch: int, free_pages, free_capacity: int, num_free,
+                     page_size: int, block_tables, max_blocks: int, num_tokens: int, query_start,
+                     seq_lens, positions, slot_mapping, status, stream=None) -> None:
+    """One step's block tables, positions and slots from the requests' lengths,
+    new pages from the top of the stack free_pages[:num_free]; status = (pages
+    left, requests refused)."""
+    fn = "paged_tables_u32"
+    _need(fn, "u32", (context_lens, batch), (new_lens, batch), (free_pages, free_capacity),
+          (num_free, 1), (block_tables, batch * max_blocks), (query_start, batch + 1),
+          (seq_lens, batch), (positions, num_tokens), (slot_mapping, num_tokens), (status, 2))
+    _check(fn, LIB.toyinfer_paged_tables_u32(
+        _ptr(context_lens), _ptr(new_lens), batch, _ptr(free_pages), free_capacity, _ptr(num_free),
+        page_size, _ptr(block_tables), max_blocks, num_tokens, _ptr(query_start), _ptr(seq_lens),
+        _ptr(positions), _ptr(slot_mapping), _ptr(status), _stream(stream)))
+
+
+def paged_qkv_prologue_bf16(q, k, v, q_norm_weight, k_norm_weight, rope_cos_sin,
+                            num_positions: int, positions, slot_mapping, num_tokens: int,
+                            rms_norm_eps: float, q_out, k_cache, v_cache, num_pages: int,
+                            page_size: int, page_stride: int, num_q_heads: int,
+                            num_kv_heads: int, head_dim: int, stream=None) -> None:
+    """q_norm + RoPE of q into q_out, k_norm + RoPE of k and v into their cache
+    slots, for num_tokens tokens (one launch)."""
+    fn = "paged_qkv_prologue_bf16"
+    row = num_tokens * head_dim
+    _need(fn, "bf16", (q, row * num_q_heads), (k, row * num_kv_heads), (v, row * num_kv_heads),
+          (q_norm_weight, head_dim), (k_norm_weight, head_dim), (q_out, row * num_q_heads))
+    _need(fn, "f32", (rope_cos_sin, num_positions * head_dim))
+    _need(fn, "u32", (positions, num_tokens), (slot_mapping, num_tokens))
+    _need_cache(fn, num_pages, page_size, page_stride, num_kv_heads, head_dim, k_cache, v_cache)
+    _check(fn, LIB.toyinfer_paged_qkv_prologue_bf16(
+        _ptr(q), _ptr(k), _ptr(v), _ptr(q_norm_weight), _ptr(k_norm_weight), _ptr(rope_cos_sin),
+        num_positions, _ptr(positions), _ptr(slot_mapping), num_tokens, rms_norm_eps, _ptr(q_out),
+        _ptr(k_cache), _ptr(v_cache), num_pages, page_size, page_stride, num_q_heads, num_kv_heads,
+        head_dim, _stream(stream)))
+
+
+def paged_attention_plan_bytes(batch: int, num_tokens: int, num_q_heads: int, num_kv_heads: int,
+                               heads_dim: int) -> int:
+    return int(LIB.toyinfer_paged_attention_plan_bytes(batch, num_tokens, num_q_heads,
+                                                       num_kv_heads, heads_dim))
+
+
+def paged_attention_plan_buffer(batch: int, num_tokens: int, num_q_heads: int, num_kv_heads: int,
+                                heads_dim: int, device):
+    """An uninitialised uint8 tensor for the plan of steps of these sizes."""
+    import torch
+
+    return torch.empty(paged_attention_plan_bytes(batch, num_tokens, num_q_heads, num_kv_heads,
+                                                  heads_dim), dtype=torch.uint8, device=device)
+
+
+def paged_attention_workspace_bytes(num_q_heads: int, num_kv_heads: int, heads_dim: int) -> int:
+    return int(LIB.toyinfer_paged_attention_workspace_bytes(num_q_heads, num_kv_heads, heads_dim))
+
+
+def paged_attention_workspace(num_q_heads: int, num_kv_heads: int, heads_dim: int, device):
+    """An uninitialised uint8 workspace tensor for these heads, whatever the lengths."""
+    import torch
+
+    return torch.empty(paged_attention_workspace_bytes(num_q_heads, num_kv_heads, heads_dim),
+                       dtype=torch.uint8, device=device)
+
+
+def paged_attention_plan(query_start, seq_lens, batch: int, num_tokens: int, page_size: int,
+                         max_blocks: int, window: int, sinks: int, num_q_heads: int,
+                         num_kv_heads: int, heads_dim: int, plan, stream=None) -> None:
+    """The work list of one step's paged attention, shared by its layers."""
+    fn = "paged_attention_plan"
+    _need(fn, "u32", (query_start, batch + 1), (seq_lens, batch))
+    _need(fn, "any", (plan, 1))
+    _check(fn, LIB.toyinfer_paged_attention_plan(
+        _ptr(query_start), _ptr(seq_lens), batch, num_tokens, page_size, max_blocks, window, sinks,
+        num_q_heads, num_kv_heads, heads_dim, _ptr(plan), plan.numel() * plan.element_size(),
+        _stream(stream)))
+
+
+def paged_attention_bf16(q, k_cache, v_cache, o, block_tables, plan, batch: int, num_tokens: int,
+                         num_pages: int, page_size: int, page_stride: int, max_blocks: int,
+                         window: int, sinks: int, num_q_heads: int, num_kv_heads: int,
+                         heads_dim: int, workspace, stream=None) -> None:
+    """Attention of the requests' new tokens over the paged cache, causal or in
+    a sliding window with `sinks` first tokens in sight; plan from
+    paged_attention_plan with the same sizes."""
+    fn = "paged_attention_bf16"
+    rows = num_tokens * num_q_heads * heads_dim
+    _need(fn, "bf16", (q, rows), (o, rows))
+    _need(fn, "u32", (block_tables, batch * max_blocks))
+    _need(fn, "any", (plan, 1), (workspace, 1))
+    _need_cache(fn, num_pages, page_size, page_stride, num_kv_heads, heads_dim, k_cache, v_cache)
+    _check(fn, LIB.toyinfer_paged_attention_bf16(
+        _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(o), _ptr(block_tables), _ptr(plan),
+        plan.numel() * plan.element_size(), batch, num_tokens, num_pages, page_size, page_stride,
+        max_blocks, window, sinks, num_q_heads, num_kv_heads, heads_dim, _ptr(workspace),
+        workspace.numel() * workspace.element_size(), _stream(stream)))

@@ -10,6 +10,7 @@
 
 #include "../../include/toyinfer_attn.h"
 #include "kernels.hpp"
+#include "paged.hpp"
 
 using namespace tiattn;
 
@@ -762,6 +763,226 @@ int toyinfer_sample_topk_topp_f32(const float* logits, uint32_t vocab, float tem
     a.out = out_token;
     a.workspace = workspace;
     return from_hip(launch_sample(a, as_stream(stream)));
+}
+
+// -------------------------------------------------------------- paged cache
+
+static bool distinct(const void* const* p, const uint64_t* bytes, int first, int n) {
+    // Ranges `first` .. n-1 (outputs) overlap none of the others.
+    for (int i = first; i < n; ++i)
+        for (int j = 0; j < i; ++j)
+            if (overlap(p[i], bytes[i], p[j], bytes[j])) return false;
+    return true;
+}
+
+static int check_paging(uint32_t page_size, uint32_t max_blocks) {
+    if (page_size < 8 || page_size > 65536 || (page_size & (page_size - 1)) || max_blocks == 0)
+        return TOYINFER_ERR_INVALID_ARGUMENT;
+    return (uint64_t)max_blocks * page_size < (1ull << 31) ? TOYINFER_OK : TOYINFER_ERR_UNSUPPORTED;
+}
+
+// The caches' arguments; *bytes receives what each spans.
+static int check_caches(const void* k_cache, const void* v_cache, uint32_t num_pages, uint32_t page_size,
+                        uint64_t page_stride, uint32_t hkv, uint32_t d, uint64_t* bytes) {
+    if (int st = check_paging(page_size, 1)) return st;
+    if (!k_cache || !v_cache || num_pages == 0) return TOYINFER_ERR_INVALID_ARGUMENT;
+    if (!aligned(k_cache, 16) || !aligned(v_cache, 16)) return TOYINFER_ERR_INVALID_ARGUMENT;
+    const uint64_t page = (uint64_t)page_size * hkv * d;
+    if (page_stride < page || page_stride % 8 != 0) return TOYINFER_ERR_INVALID_ARGUMENT;
+    if ((uint64_t)num_pages * page_size >= (1ull << 32) || page_stride >= (1ull << 40))
+        return TOYINFER_ERR_UNSUPPORTED;
+    *bytes = 2 * ((num_pages - 1) * page_stride + page);
+    // Pages of one cache may lie between pages of the other, not on them.
+    const uintptr_t a = (uintptr_t)k_cache, b = (uintptr_t)v_cache;
+    const uint64_t apart = (a < b ? b - a : a - b) % (2 * page_stride);
+    if (overlap(k_cache, *bytes, v_cache, *bytes) && (apart < 2 * page || 2 * page_stride - apart < 2 * page))
+        return TOYINFER_ERR_INVALID_ARGUMENT;
+    return TOYINFER_OK;
+}
+
+int toyinfer_paged_tables_u32(const uint32_t* context_lens, const uint32_t* new_lens,
+                              uint32_t batch, const uint32_t* free_pages, uint32_t free_capacity,
+                              const uint32_t* num_free, uint32_t page_size,
+                              uint32_t* block_tables, uint32_t max_blocks, uint32_t num_tokens,
+                              uint32_t* query_start, uint32_t* seq_lens, uint32_t* positions,
+                              uint32_t* slot_mapping, uint32_t* status, void* stream) {
+    if (batch == 0 || num_tokens == 0) return TOYINFER_ERR_INVALID_ARGUMENT;
+    if (int st = check_paging(page_size, max_blocks)) return st;
+    const void* const p[] = {context_lens, new_lens, free_pages, num_free, block_tables, query_start, seq_lens,
+                             positions, slot_mapping, status};
+    const uint64_t bytes[] = {4ull * batch, 4ull * batch, 4ull * free_capacity, 4, 4ull * batch * max_blocks,
+                              4ull * (batch + 1ull), 4ull * batch, 4ull * num_tokens, 4ull * num_tokens, 8};
+    for (int i = 0; i < 10; ++i)
+        if ((!p[i] && !(i == 2 && free_capacity == 0)) || !aligned(p[i], 4)) return TOYINFER_ERR_INVALID_ARGUMENT;
+    if (!distinct(p, bytes, 4, 10)) return TOYINFER_ERR_INVALID_ARGUMENT;
+    if (batch > kPagedMaxBatch || num_tokens >= (1u << 31)) return TOYINFER_ERR_UNSUPPORTED;
+    PagedTablesArgs a;
+    a.context_lens = context_lens;
+    a.new_lens = new_lens;
+    a.batch = batch;
+    a.free_pages = free_pages;
+    a.free_capacity = free_capacity;
+    a.num_free = num_free;
+    a.page_shift = 31 - __builtin_clz(page_size);
+    a.block_tables = block_tables;
+    a.max_blocks = max_blocks;
+    a.num_tokens = num_tokens;
+    a.query_start = query_start;
+    a.seq_lens = seq_lens;
+    a.positions = positions;
+    a.slots = slot_mapping;
+    a.status = status;
+    return from_hip(launch_paged_tables(a, as_stream(stream)));
+}
+
+int toyinfer_paged_qkv_prologue_bf16(const void* q, const void* k, const void* v,
+                                     const void* q_norm_weight, const void* k_norm_weight,
+                                     const float* rope_cos_sin, uint32_t num_positions,
+                                     const uint32_t* positions, const uint32_t* slot_mapping,
+                                     uint32_t num_tokens, float rms_norm_eps, void* q_out,
+                                     void* k_cache, void* v_cache, uint32_t num_pages,
+                                     uint32_t page_size, uint64_t page_stride,
+                                     uint32_t num_q_heads, uint32_t num_kv_heads,
+                                     uint32_t head_dim, void* stream) {
+    if (int st = check_heads(num_q_heads, num_kv_heads, head_dim)) return st;
+    if (num_tokens == 0 || num_positions == 0) return TOYINFER_ERR_INVALID_ARGUMENT;
+    uint64_t cache = 0;
+    if (int st = check_caches(k_cache, v_cache, num_pages, page_size, page_stride, num_kv_heads, head_dim, &cache))
+        return st;
+    const uint64_t row = 2ull * num_tokens * head_dim;
+    const void* const p[] = {q, k, v, q_norm_weight, k_norm_weight, rope_cos_sin, positions, slot_mapping, q_out,
+                             k_cache, v_cache};
+    const uint64_t bytes[] = {row * num_q_heads, row * num_kv_heads, row * num_kv_heads, 2ull * head_dim,
+                              2ull * head_dim, 4ull * num_positions * head_dim, 4ull * num_tokens,
+                              4ull * num_tokens, row * num_q_heads, cache, cache};
+    for (int i = 0; i < 9; ++i)
+        if (!p[i] || !aligned(p[i], i == 6 || i == 7 ? 4 : 16)) return TOYINFER_ERR_INVALID_ARGUMENT;
+    for (int i = 8; i < 11; ++i)
+        for (int j = 0; j < (i == 8 ? 8 : 9); ++j)  // (the caches against each other: check_caches)
+            if (!(i == 8 && j == 0 && q_out == q) && overlap(p[i], bytes[i], p[j], bytes[j]))
+                return TOYINFER_ERR_INVALID_ARGUMENT;
+    if ((uint64_t)num_tokens * (num_q_heads + 2ull * num_kv_heads) >= (1ull << 31)) return TOYINFER_ERR_UNSUPPORTED;
+    PagedPrologueArgs a;
+    a.q = static_cast<const uint16_t*>(q);
+    a.k = static_cast<const uint16_t*>(k);
+    a.v = static_cast<const uint16_t*>(v);
+    a.q_weight = static_cast<const uint16_t*>(q_norm_weight);
+    a.k_weight = static_cast<const uint16_t*>(k_norm_weight);
+    a.rope = rope_cos_sin;
+    a.num_positions = num_positions;
+    a.positions = positions;
+    a.slots = slot_mapping;
+    a.num_tokens = num_tokens;
+    a.eps = rms_norm_eps;
+    a.q_out = static_cast<uint16_t*>(q_out);
+    a.k_cache = static_cast<uint16_t*>(k_cache);
+    a.v_cache = static_cast<uint16_t*>(v_cache);
+    a.num_slots = num_pages * page_size;
+    a.page_shift = 31 - __builtin_clz(page_size);
+    a.page_stride = page_stride;
+    a.hq = num_q_heads;
+    a.hkv = num_kv_heads;
+    return from_hip(launch_paged_prologue(a, head_dim, as_stream(stream)));
+}
+
+static int check_paged_step(uint32_t batch, uint32_t num_tokens, uint32_t hq, uint32_t hkv, uint32_t d) {
+    if (int st = check_heads(hq, hkv, d)) return st;
+    if (batch == 0 || num_tokens == 0) return TOYINFER_ERR_INVALID_ARGUMENT;
+    if (batch > kPagedMaxBatch || (uint64_t)num_tokens * (hq / hkv) >= (1ull << 31)) return TOYINFER_ERR_UNSUPPORTED;
+    return TOYINFER_OK;
+}
+
+static PagedPlanHeader plan_header(uint32_t batch, uint32_t num_tokens, uint32_t page_size, uint32_t max_blocks,
+                                   uint32_t window, uint32_t sinks, uint32_t hq, uint32_t hkv, uint32_t d) {
+    PagedPlanHeader h{};
+    h.batch = batch;
+    h.num_tokens = num_tokens;
+    h.page_size = page_size;
+    h.max_blocks = max_blocks;
+    h.window = window;
+    h.sinks = sinks;
+    h.hq = hq;
+    h.hkv = hkv;
+    h.d = d;
+    return h;
+}
+
+// The workspace holds the partial outputs, then their statistics.
+static size_t paged_part_o_bytes(uint32_t hkv, uint32_t d) {
+    return (size_t)hkv * paged_partial_blocks(hkv) * kPagedBlockRows * d * sizeof(float);
+}
+
+size_t toyinfer_paged_attention_plan_bytes(uint32_t batch, uint32_t num_tokens, uint32_t num_q_heads,
+                                           uint32_t num_kv_heads, uint32_t heads_dim) {
+    if (check_paged_step(batch, num_tokens, num_q_heads, num_kv_heads, heads_dim)) return 0;
+    return paged_plan_layout(batch, num_tokens, num_q_heads, num_kv_heads).bytes;
+}
+
+size_t toyinfer_paged_attention_workspace_bytes(uint32_t num_q_heads, uint32_t num_kv_heads, uint32_t heads_dim) {
+    if (check_heads(num_q_heads, num_kv_heads, heads_dim)) return 0;
+    return paged_part_o_bytes(num_kv_heads, heads_dim) +
+           (size_t)num_kv_heads * paged_partial_blocks(num_kv_heads) * kPagedBlockRows * sizeof(float2);
+}
+
+int toyinfer_paged_attention_plan(const uint32_t* query_start, const uint32_t* seq_lens,
+                                  uint32_t batch, uint32_t num_tokens, uint32_t page_size,
+                                  uint32_t max_blocks, uint32_t window, uint32_t sinks,
+                                  uint32_t num_q_heads, uint32_t num_kv_heads,
+                                  uint32_t heads_dim, void* plan, size_t plan_bytes,
+                                  void* stream) {
+    if (int st = check_paged_step(batch, num_tokens, num_q_heads, num_kv_heads, heads_dim)) return st;
+    if (int st = check_paging(page_size, max_blocks)) return st;
+    if (!query_start || !seq_lens || !plan) return TOYINFER_ERR_INVALID_ARGUMENT;
+    if (!aligned(query_start, 4) || !aligned(seq_lens, 4) || !aligned(plan, 256)) return TOYINFER_ERR_INVALID_ARGUMENT;
+    const size_t need = paged_plan_layout(batch, num_tokens, num_q_heads, num_kv_heads).bytes;
+    if (plan_bytes < need) return TOYINFER_ERR_WORKSPACE;
+    if (overlap(plan, need, query_start, 4 * (batch + 1ull)) || overlap(plan, need, seq_lens, 4ull * batch))
+        return TOYINFER_ERR_INVALID_ARGUMENT;
+    PagedPlanArgs a;
+    a.query_start = query_start;
+    a.seq_lens = seq_lens;
+    a.head = plan_header(batch, num_tokens, page_size, max_blocks, window, sinks, num_q_heads, num_kv_heads, heads_dim);
+    a.plan = plan;
+    return from_hip(launch_paged_plan(a, as_stream(stream)));
+}
+
+int toyinfer_paged_attention_bf16(const void* q, const void* k_cache, const void* v_cache, void* o,
+                                  const uint32_t* block_tables, const void* plan,
+                                  size_t plan_bytes, uint32_t batch, uint32_t num_tokens,
+                                  uint32_t num_pages, uint32_t page_size, uint64_t page_stride,
+                                  uint32_t max_blocks, uint32_t window, uint32_t sinks,
+                                  uint32_t num_q_heads, uint32_t num_kv_heads,
+                                  uint32_t heads_dim, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+    if (int st = check_paged_step(batch, num_tokens, num_q_heads, num_kv_heads, heads_dim)) return st;
+    if (int st = check_paging(page_size, max_blocks)) return st;
+    uint64_t cache = 0;
+    if (int st = check_caches(k_cache, v_cache, num_pages, page_size, page_stride, num_kv_heads, heads_dim, &cache))
+        return st;
+    if (!q || !o || !block_tables || !plan || !workspace) return TOYINFER_ERR_INVALID_ARGUMENT;
+    if (!aligned(q, 16) || !aligned(o, 16) || !aligned(block_tables, 4) || !aligned(plan, 256) ||
+        !aligned(workspace, 256))
+        return TOYINFER_ERR_INVALID_ARGUMENT;
+    const size_t plan_need = paged_plan_layout(batch, num_tokens, num_q_heads, num_kv_heads).bytes;
+    const size_t ws_need = toyinfer_paged_attention_workspace_bytes(num_q_heads, num_kv_heads, heads_dim);
+    if (plan_bytes < plan_need || workspace_bytes < ws_need) return TOYINFER_ERR_WORKSPACE;
+    const uint64_t rows = 2ull * num_tokens * num_q_heads * heads_dim;
+    const void* const p[] = {q, k_cache, v_cache, block_tables, plan, o, workspace};
+    const uint64_t bytes[] = {rows, cache, cache, 4ull * batch * max_blocks, plan_need, rows, ws_need};
+    if (!distinct(p, bytes, 5, 7)) return TOYINFER_ERR_INVALID_ARGUMENT;
+    PagedAttnArgs a;
+    a.q = static_cast<const uint16_t*>(q);
+    a.k_cache = static_cast<const uint16_t*>(k_cache);
+    a.v_cache = static_cast<const uint16_t*>(v_cache);
+    a.o = static_cast<uint16_t*>(o);
+    a.block_tables = block_tables;
+    a.plan = plan;
+    a.head = plan_header(batch, num_tokens, page_size, max_blocks, window, sinks, num_q_heads, num_kv_heads, heads_dim);
+    a.num_pages = num_pages;
+    a.page_stride = page_stride;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + paged_part_o_bytes(num_kv_heads, heads_dim));
+    return from_hip(launch_paged_attention(a, as_stream(stream)));
 }
 
 }  // extern "C"
