@@ -254,14 +254,23 @@ def check_plan(st):
     workspace, before a kernel relies on it."""
     raw = st.plan.cpu().numpy()
     head = raw[:256].view(np.uint32)
-    n = int(head[11])
-    lanes = max(1, 512 // st.hkv)
-    items = raw[256:256 + 48 * n].view(np.uint32).reshape(n, 12)
+    n, ranges = int(head[10]), int(head[12])
+    lanes = max(1, 256 // st.hkv)
+    assert lanes <= ranges
+    every = raw[256:256 + 48 * (ranges + n)].view(np.uint32).reshape(-1, 12)
+    items = []
+    for i in every[:ranges]:
+        while i[3]:
+            items.append(i)
+            if i[11] == 0xFFFFFFFF:
+                break
+            i = every[i[11]]
+    assert len(items) == n
     group = st.hq // st.hkv
     units, blocks = {}, []
     for it in items:
         req, token0, row0, rows = (int(x) for x in it[:4])
-        assert req < st.batch and 1 <= rows <= 128 and token0 == st.start[req]
+        assert req < st.batch and 1 <= rows <= 256 and token0 == st.start[req]
         key_end, low, sink = int(it[5]), int(it[6]), int(it[7])
         assert key_end <= st.requests[req][0] and sink <= low
         units.setdefault((req, row0, rows, key_end, low, sink), []).append(it)
@@ -279,7 +288,7 @@ def check_plan(st):
         else:
             assert its[0][10] == 0xFFFFFFFF
         seen.setdefault(req, []).append((row0, row0 + rows))
-    assert len(blocks) == len(set(blocks)) and max(blocks, default=0) < 8 * lanes
+    assert len(blocks) == len(set(blocks)) and max(blocks, default=0) < 16 * lanes
     for b, (_, new) in enumerate(st.requests):
         spans = sorted(seen.get(b, []))
         assert [s for s, _ in spans] == [0, *[e for _, e in spans[:-1]]][:len(spans)]

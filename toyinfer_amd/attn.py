@@ -575,10 +575,10 @@ def paged_attention_workspace_bytes(num_q_heads: int, num_kv_heads: int, heads_d
 
 
 def paged_attention_workspace(num_q_heads: int, num_kv_heads: int, heads_dim: int, device):
-    """An uninitialised uint8 workspace tensor for these heads, whatever the lengths."""
+    """A zeroed uint8 workspace tensor for these heads, whatever the lengths."""
     import torch
 
-    return torch.empty(paged_attention_workspace_bytes(num_q_heads, num_kv_heads, heads_dim),
+    return torch.zeros(paged_attention_workspace_bytes(num_q_heads, num_kv_heads, heads_dim),
                        dtype=torch.uint8, device=device)
 
 

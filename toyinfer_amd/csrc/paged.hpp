@@ -57,48 +57,53 @@ hipError_t launch_paged_prologue(const PagedPrologueArgs& a, uint32_t d, hipStre
 // --------------------------------------------------------------- attention
 //
 // The rows of a request, for one KV head, are (new token, query head of the
-// group) pairs: row r is token r / group, head r % group.  A unit is up to 128
+// group) pairs: row r is token r / group, head r % group.  A unit is up to 256
 // consecutive rows of a request, an item a range of a unit's key tiles; the
 // same units and items serve every KV head.
-constexpr uint32_t kPagedTile = 64;         // keys per tile
-constexpr uint32_t kPagedSlots = 512;       // workgroups: two per compute unit
-constexpr uint32_t kPagedMaxRows = 128;     // rows of a unit
-constexpr uint32_t kPagedBlockRows = 32;    // rows of a wave
+constexpr uint32_t kPagedTile = 64;       // keys per tile
+constexpr uint32_t kPagedSlots = 256;     // workgroups: one per compute unit
+constexpr uint32_t kPagedMaxRows = 256;   // rows of a unit
+constexpr uint32_t kPagedBlockRows = 32;  // rows of a wave
 
-// Lanes per KV head: each runs one workgroup's list of items.
+// Lanes per KV head: workgroups that start on it.
 inline __host__ __device__ uint32_t paged_lanes(uint32_t hkv) {
     return hkv >= kPagedSlots ? 1 : kPagedSlots / hkv;
 }
-// 32-row blocks of partial results that the workspace holds per KV head: an
-// item of a split unit costs at least half of a lane's share (paged_plan.hip),
-// so there are fewer than two per lane, of at most four blocks each.
+// A plan of cut units has up to kPagedLevels ranges per lane, one with units of
+// 256 rows, two with 128.  A cut leaves two pieces of its unit, so per KV head
+// the workspace holds this many 32-row blocks of partial results, and the plan
+// half as many blocks that are in pieces.
+constexpr uint32_t kPagedLevels = 4;
 inline __host__ __device__ uint32_t paged_partial_blocks(uint32_t hkv) {
-    return 2 * paged_lanes(hkv) * (kPagedMaxRows / kPagedBlockRows);
+    return 2 * (kPagedMaxRows / kPagedBlockRows) * paged_lanes(hkv);
 }
 
 struct PagedPlanHeader {
     // The arguments that the plan was made for; the attention compares them.
     uint32_t batch, num_tokens, page_size, max_blocks, window, sinks, hq, hkv, d, magic;
-    uint32_t units, items;
+    uint32_t items;
     uint32_t split_blocks;  // 32-row blocks whose partials are to be merged, per KV head
-    uint32_t pad[51];
+    uint32_t ranges;        // lists of items: lane l runs list l, then draws further ones
+    uint32_t units;         // in the plan's array of them; a split one's `partial` is not kPagedWhole
+    uint32_t pad[50];
 };
 static_assert(sizeof(PagedPlanHeader) == 256, "the items follow at a cache line");
 constexpr uint32_t kPagedMagic = 0x70616765u;
 
-constexpr uint32_t kPagedWhole = 0xffffffffu;
+constexpr uint32_t kPagedWhole = 0xffffffffu, kPagedNone = 0xffffffffu;
+// Item r < ranges is the first of list r (rows 0: the list is empty).
 struct PagedItem {
     uint32_t req;      // row of the block table
     uint32_t token0;   // row of q and o that holds the request's first new token
     uint32_t row0;     // first row of the unit
-    uint32_t rows;     // 1..128
+    uint32_t rows;     // 1..256
     int32_t pos0;      // position of the request's first new token (< 0: it sees nothing)
     uint32_t key_end;  // keys at or past it are seen by no row of the unit
     uint32_t low_tile; // tiles [0, sink_tiles) and from low_tile on are seen
     uint32_t sink_tiles;
     uint32_t tile_begin, tile_end;  // of the unit's tiles, counted through that gap
     uint32_t partial;  // first 32-row block of its partial results, or kPagedWhole
-    uint32_t pad;
+    uint32_t next;     // the list's next item, or kPagedNone
 };
 static_assert(sizeof(PagedItem) == 48, "read by 16-byte loads");
 
@@ -107,7 +112,8 @@ static_assert(sizeof(PagedItem) == 48, "read by 16-byte loads");
 struct PagedSplitBlock {
     uint32_t token0, row0, rows;  // as in PagedItem, of this block (rows 1..32)
     uint32_t first, stride, pieces;
-    uint32_t pad[2];
+    uint32_t req;
+    int32_t pos0;  // as in PagedItem
 };
 static_assert(sizeof(PagedSplitBlock) == 32, "read by 16-byte loads");
 
@@ -116,18 +122,18 @@ inline __host__ __device__ uint32_t paged_max_units(uint32_t batch, uint32_t num
     return batch + (uint32_t)(((uint64_t)num_tokens * group) / kPagedBlockRows);
 }
 struct PagedPlanLayout {
-    size_t items, units, costs, split_blocks, bytes;
+    size_t items, split_blocks, units, costs, bytes;
 };
 inline __host__ __device__ PagedPlanLayout paged_plan_layout(uint32_t batch, uint32_t num_tokens,
                                                              uint32_t hq, uint32_t hkv) {
-    const size_t units = paged_max_units(batch, num_tokens, hq / hkv);
-    const size_t split = 2 * (size_t)paged_lanes(hkv);
+    const size_t units = paged_max_units(batch, num_tokens, hq / hkv), cuts = kPagedLevels * paged_lanes(hkv);
     PagedPlanLayout l;
     l.items = sizeof(PagedPlanHeader);
-    l.split_blocks = l.items + (units + split) * sizeof(PagedItem);
-    l.units = l.split_blocks + split * (kPagedMaxRows / kPagedBlockRows) * sizeof(PagedSplitBlock);
+    // The ranges' first items, then at most one per unit and cut.
+    l.split_blocks = l.items + (units + 2 * cuts) * sizeof(PagedItem);
+    l.units = l.split_blocks + paged_partial_blocks(hkv) / 2 * sizeof(PagedSplitBlock);
     l.costs = l.units + units * sizeof(PagedItem);
-    l.bytes = (l.costs + 2 * (units + 1) * sizeof(uint32_t) + 255) / 256 * 256;
+    l.bytes = (l.costs + (units + 1) * sizeof(uint64_t) + 255) / 256 * 256;
     return l;
 }
 
@@ -149,6 +155,8 @@ struct PagedAttnArgs {
     PagedPlanHeader head;  // what the plan has to have been made for
     uint32_t num_pages;
     uint64_t page_stride;  // elements
+    uint32_t* tickets;     // [KV head], zero between calls
+    uint32_t* flags;       // [2], zero between calls: a hidden infinity or NaN was met; workgroups done
     float* part_o;         // [KV head][block][D / 4][64 lanes][4]
     float2* part_ml;       // [KV head][block][32 rows]: reference (log2), sum
 };

@@ -1,23 +1,29 @@
 // Attention of new tokens over a paged KV cache, for gfx950.
 //
-// A persistent grid of two workgroups per compute unit runs the items of a
-// plan (paged_plan.hip): up to 128 (token, head) rows of one request and KV
-// head against a range of its 64-key tiles.  Packing the query heads of a group
-// into the rows lets one K/V tile serve them all, for a decoded token (rows =
-// group) as for a chunk.  Three forms by the unit's rows, all of 32 rows per
-// wave on v_mfma_f32_32x32x16_bf16, with the operand layouts of the prefill
+// A persistent grid of one workgroup of eight waves per compute unit runs the
+// items of a plan (paged_plan.hip): up to 256 (token, head) rows of one request
+// and KV head against a range of its 64-key tiles.  Packing the query heads of
+// a group into the rows lets one K/V tile serve them all, for a decoded token
+// (rows = group) as for a chunk.  Four forms by the unit's rows, all of 32 rows
+// per wave on v_mfma_f32_32x32x16_bf16, with the operand layouts of the prefill
 // kernel (S^T = K Q^T, O^T += V^T P^T, a lane owns one row):
-//   > 64 rows: four waves of 32 rows share each tile;
-//   33..64:    two waves of 32 rows, each over one 32-key half of a tile, twice;
-//   <= 32:     every wave streams 32-key halves of its own, without barriers:
-//              K's operands go from LDS to registers, the next K is requested
-//              into the place they leave, likewise V, so a wave's loads are in
-//              flight while it computes.
+//   > 128 rows: eight waves of 32 rows share each tile;
+//   65..128:    four waves of 32 rows share a tile, two tiles at a time;
+//   33..64:     two waves of 32 rows share a 32-key half, four halves at a time;
+//   <= 32:      kStreams waves stream 32-key halves of their own, without
+//               barriers: K's operands go from LDS to registers, the next K is
+//               requested into the place they leave, likewise V, so a wave's
+//               loads are in flight while it computes.
 // K and V reach LDS by buffer loads that write it.  Each instruction fills 1 KiB,
-// 4 (head_dim 128) or 8 (64) rows, which one page holds: its buffer resource is
-// built from the page's number by scalar instructions, in 64 bits, and ends
-// behind the last key that the unit sees, so that rows past it read as zeros.
-// The page numbers of an item wait in LDS.
+// 4 (head_dim 128) or 8 (64) rows, which lie in one page: its address is a scalar
+// 64-bit base and a lane's constant.  The bases of an item's tiles, one per
+// min(page size, 64) keys, wait in LDS.  Rows past the last key that the unit
+// sees are some row of its last page and masked like any hidden key; V's are
+// zeroed in LDS, since 0 * NaN is NaN.  Where a tile has a key that some row
+// does not see and its V holds infinities or NaN, 0 times them turns that row
+// to NaN: the workgroup says so in a flag, and the second kernel then computes
+// the rows that hold NaN again, key by key.  (Done here instead, in registers
+// that the compiler took from the loops, it cost the streaming form 15 %.)
 #include <math.h>
 
 #include "common.hpp"
@@ -28,8 +34,10 @@ namespace {
 
 typedef short v4i16_t __attribute__((ext_vector_type(4)));
 
-constexpr int kPaThreads = 256;
-constexpr uint32_t kTabEntries = 2048;        // page numbers in LDS at a time
+constexpr int kPaThreads = 512;
+constexpr int kPaWaves = kPaThreads / 64;
+constexpr int kStreams = 4;
+constexpr uint32_t kTabEntries = 1024;        // bases in LDS at a time
 constexpr float kPaRescale = 8.0f;            // a running reference moves up by more than 2^8 only
 constexpr float kPaMassMax = 0x1p64f, kPaMassMin = 0x1p-64f;
 
@@ -52,7 +60,8 @@ struct PaShape {
     static constexpr int RI = 64 / CPR;          // rows per load instruction
     static constexpr int HALF_LOADS = 32 / RI;   // instructions per 32 rows
     static constexpr int NF = D / 8;             // float4 per lane of a 32-row block's output
-    static constexpr int BUF = 2 * 64 * D;       // elements: K and V of one tile
+    static constexpr int TILE = 2 * 64 * D;      // elements: K and V of one tile
+    static constexpr int BUF = 2 * TILE;         // of one step
 };
 
 // Where an item's keys lie (all uniform).
@@ -67,35 +76,42 @@ struct KeySource {
     }
 };
 
-// RI rows from key `key` of the page that lane `entry` of `pages` names.
-template <int D>
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_rsrc(const KeySource& s, const char* base, uint32_t pages,
-                                                           uint32_t entry, uint32_t key) {
-    const uint32_t page = __builtin_amdgcn_readlane(pages, entry);
-    const uint32_t in_page = key & ((1u << s.page_shift) - 1);
-    const uint32_t rows = key < s.key_end ? min(s.key_end - key, (uint32_t)PaShape<D>::RI) : 0;
-    const uint32_t bytes = rows ? (rows - 1) * s.row_bytes + D * 2 : 0;
-    return make_rsrc(base + (uint64_t)page * s.page_bytes + (uint64_t)in_page * s.row_bytes, bytes);
+// Lane `entry` of `bases` (byte offsets of an entry's rows in the caches).
+__device__ __forceinline__ uint64_t base_of(uint2 bases, uint32_t entry) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(bases.y, entry) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane(bases.x, entry);
 }
 
-__device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, uint16_t* lds, uint32_t voff) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, voff, 0, 0, 0);
+// (Buffer loads: the compiler counts a global load that writes LDS as an LDS
+// access too and then waits for all of them before every operand.)
+template <int AUX>
+__device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint16_t* lds) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, voff, 0, 0, AUX);
 }
+// A resource that starts at `base`: a lane adds at most eight rows.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const char* base) { return make_rsrc(base, 0x7fffffffu); }
 
-// Rows of a wave: this lane's position and the wave's first and last.
+// Rows of a wave: this lane's position; the wave's first and last, and the
+// first keys inside their windows (uniform).
 struct RowView {
-    int32_t pos, first, last;
+    int32_t pos, first, last, first_low, last_low;
     uint32_t window, sinks;  // window 2^31: none
+    __device__ __forceinline__ void span(int32_t f, int32_t l) {
+        first = f;
+        last = l;
+        first_low = max(0, (int32_t)((uint32_t)f + 1 - window));
+        last_low = max(0, (int32_t)((uint32_t)l + 1 - window));
+    }
     __device__ __forceinline__ bool sees(uint32_t key) const {
-        return (uint32_t)(pos - (int32_t)key) < window || ((int32_t)key <= pos && key < sinks);
+        return ((uint32_t)(pos - (int32_t)key) < window) | (((int32_t)key <= pos) & (key < sinks));
     }
     // No row of the wave sees a key of [k0, k1].
-    __device__ __forceinline__ bool none(uint32_t k0, uint32_t k1) const {
-        return (int32_t)k0 > last || (k0 >= sinks && (int64_t)k1 + window <= (int64_t)first);
+    __device__ __forceinline__ bool none(int32_t k0, int32_t k1) const {
+        return k0 > last || (k1 < first_low && (uint32_t)k0 >= sinks);
     }
     // Some row does not see some key of [k0, k1].
-    __device__ __forceinline__ bool some_hidden(uint32_t k0, uint32_t k1) const {
-        return (int32_t)k1 > first || ((int64_t)k0 + window <= (int64_t)last && k1 >= sinks);
+    __device__ __forceinline__ bool some_hidden(int32_t k0, int32_t k1) const {
+        return k1 > first || (k0 < last_low && (uint32_t)k1 >= sinks);
     }
 };
 
@@ -169,6 +185,8 @@ __device__ __forceinline__ void probabilities(f32x16_t (&st)[NB], RowState<D>& s
 
 template <int D, int NB>
 __device__ __forceinline__ void hide(f32x16_t (&st)[NB], const RowView& rv, uint32_t k0, int kg) {
+    // Keeps the branch around this: as selects it would run for every tile.
+    asm volatile("; hidden keys");
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -191,58 +209,16 @@ __device__ __forceinline__ uint32_t nonfinite_halves(uint32_t w) {
     return ((e & 0xffffu) == 0x7f80u ? 1u : 0u) | ((e >> 16) == 0x7f80u ? 0x10000u : 0u);
 }
 
+// Whether the 32 NB rows from vb on hold infinities or NaN.
 template <int D, int NB>
-__device__ __forceinline__ bool any_nonfinite(const uint16_t* vb, const int (&v_off)[D / 32]) {
+__device__ __forceinline__ bool any_nonfinite(const uint16_t* vb, int lane) {
     uint32_t bad = 0;
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-        for (int tt = 0; tt < 2 * NB; ++tt) {
-            if (tt == 0) __builtin_amdgcn_sched_barrier(0);
-            const uint4 v = v_operand<D>(vb, v_off[db], tt);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) bad |= nonfinite_halves(word_of(v, e));
-        }
-    return __any(bad != 0);
-}
-
-// A word of two bf16 with those that are not finite replaced by 0.
-__device__ __forceinline__ uint32_t finite_part(uint32_t w) {
-    const uint32_t bad = nonfinite_halves(w);
-    return w & ~(((bad & 1u) ? 0xffffu : 0u) | ((bad >> 16) ? 0xffff0000u : 0u));
-}
-
-// O^T += V^T P^T for a tile where some row does not see some key and V holds
-// infinities or NaN: 0 * NaN would carry them into rows that do not see
-// them.  The finite part of V multiplies P; what is not finite is added, key by
-// key, to the rows that see the key.
-template <int D, int NB>
-__device__ __forceinline__ void values_isolated(RowState<D>& s, const uint16_t* vb, const int (&v_off)[D / 32],
-                                                const bf16x8_t (&pf)[2 * NB], const RowView& rv, uint32_t k0, int kg) {
-#pragma unroll
-    for (int tt = 0; tt < 2 * NB; ++tt)
-#pragma unroll
-        for (int db = 0; db < D / 32; ++db) {
-            __builtin_amdgcn_sched_barrier(0);  // one operand at a time: few registers
-            uint4 v = v_operand<D>(vb, v_off[db], tt);
-            v = make_uint4(finite_part(v.x), finite_part(v.y), finite_part(v.z), finite_part(v.w));
-            s.o[db] = mfma32x32x16(as_bf16x8(v), pf[tt], s.o[db]);
-        }
 #pragma unroll 1
-    for (int key = 0; key < 32 * NB; ++key) {
-        const bool seen = rv.sees(k0 + key);
-#pragma unroll
-        for (int f = 0; f < D / 8; ++f) {
-            __builtin_amdgcn_sched_barrier(0);
-            const uint2 w = *reinterpret_cast<const uint2*>(vb + key * D + 8 * (f ^ pv_swz<D>(key)) + 4 * kg);
-            const uint32_t x[2] = {w.x & ~finite_part(w.x), w.y & ~finite_part(w.y)};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float y = e & 1 ? bf16_hi(x[e / 2]) : bf16_lo(x[e / 2]);
-                s.o[f / 4][4 * (f % 4) + e] += seen ? y : 0.0f;
-            }
-        }
+    for (int i = 0; i < 32 * NB * D / 512; ++i) {
+        const uint4 v = *reinterpret_cast<const uint4*>(vb + 512 * i + 8 * lane);
+        bad |= nonfinite_halves(v.x) | nonfinite_halves(v.y) | nonfinite_halves(v.z) | nonfinite_halves(v.w);
     }
+    return __any(bad != 0);
 }
 
 template <int D, int NB>
@@ -276,7 +252,8 @@ template <int D, int NB>
 __device__ __forceinline__ void tile(RowState<D>& s, const uint16_t* kb, const uint16_t* vb,
                                      const int (&k_off)[D / 16], const int (&v_off)[D / 32],
                                      const bf16x8_t (&qf)[D / 16], const RowView& rv, uint32_t k0, uint32_t key_end,
-                                     float scale_log2, int kg) {
+                                     float scale_log2, int lane, uint32_t* flag) {
+    const int kg = lane >> 5;
     constexpr int KSTEPS = D / 16;
     f32x16_t st[NB];
 #pragma unroll
@@ -308,10 +285,8 @@ __device__ __forceinline__ void tile(RowState<D>& s, const uint16_t* kb, const u
     if (hidden) hide<D, NB>(st, rv, k0, kg);
     bf16x8_t pf[2 * NB];
     probabilities<D, NB>(st, s, pf, scale_log2);
-    if (hidden && rv.some_hidden(k0, min(k1, key_end - 1)) && any_nonfinite<D, NB>(vb, v_off))
-        values_isolated<D, NB>(s, vb, v_off, pf, rv, k0, kg);
-    else
-        values<D, NB>(s, vb, v_off, pf);
+    if (hidden && rv.some_hidden(k0, min(k1, key_end - 1)) && any_nonfinite<D, NB>(vb, lane)) *flag = 1;
+    values<D, NB>(s, vb, v_off, pf);
 }
 
 // What every form needs of an item.
@@ -319,17 +294,31 @@ struct ItemView {
     PagedItem it;
     KeySource src;
     uint32_t kvh, group;
-    const uint32_t* table;   // the request's row
-    uint32_t num_pages;
 };
 
-// The page numbers of tiles [c0, c1), one per min(page size, 64) keys; keys
-// that no row sees get page 0 (their rows are never loaded).
-__device__ __forceinline__ void fill_table(const ItemView& v, uint32_t* s_tab, uint32_t c0, uint32_t c1) {
+__device__ __forceinline__ void point_at(ItemView& v, const PagedAttnArgs& a, const PagedItem& it, uint32_t kvh) {
+    v.it = it;
+    v.kvh = kvh;
+    v.src.key_end = it.key_end;
+    v.src.low_tile = it.low_tile;
+    v.src.sink_tiles = it.sink_tiles;
+    v.src.k = reinterpret_cast<const char*>(a.k_cache + (uint64_t)kvh * a.head.d);
+    v.src.v = reinterpret_cast<const char*>(a.v_cache + (uint64_t)kvh * a.head.d);
+}
+
+// The bases of tiles [c0, c1), by `threads` threads: entry i of a tile is for
+// its keys from i << entry_shift on.  Past the last key seen: its entry.
+__device__ __forceinline__ void fill_table(const PagedAttnArgs& a, const ItemView& v, uint2* tab, uint32_t c0,
+                                           uint32_t c1, uint32_t tid, uint32_t threads) {
     const uint32_t per_shift = 6 - v.src.entry_shift, n = (c1 - c0) << per_shift;
-    for (uint32_t i = threadIdx.x; i < n; i += kPaThreads) {
+    const uint32_t in_page = (1u << v.src.page_shift) - 1, in_entry = (1u << v.src.entry_shift) - 1;
+    const uint32_t* const row = a.block_tables + (uint64_t)v.it.req * a.head.max_blocks;
+    for (uint32_t i = tid; i < n; i += threads) {
         const uint32_t key = v.src.key0(c0 + (i >> per_shift)) + ((i & ((1u << per_shift) - 1)) << v.src.entry_shift);
-        s_tab[i] = key < v.src.key_end ? min(v.table[key >> v.src.page_shift], v.num_pages - 1) : 0;
+        const uint32_t k = min(key, (v.src.key_end - 1) & ~in_entry);
+        const uint32_t page = min(row[k >> v.src.page_shift], a.num_pages - 1);
+        const uint64_t base = page * v.src.page_bytes + (uint64_t)(k & in_page) * v.src.row_bytes;
+        tab[i] = make_uint2((uint32_t)base, (uint32_t)(base >> 32));
     }
 }
 
@@ -368,13 +357,13 @@ __device__ __forceinline__ void put_ml(const PagedAttnArgs& a, const ItemView& v
 }
 
 // Merge of the KS waves (streams) that hold the same 32 rows, through s_a and
-// s_b (free: a barrier has passed), and the output; wave = stream * (4 / KS) +
-// row block.
-template <int D, int KS>
+// s_b, and the output.  Wave = stream * RB + row
+// block; the 8 / RB waves of a row block share its output.
+template <int D, int RB, int KS = kPaWaves / RB>
 __device__ __forceinline__ void finish(const PagedAttnArgs& a, const ItemView& v, RowState<D>& s, uint16_t* s_a,
                                        uint16_t* s_b, float2 (*s_ml)[32], int wave, int lane) {
-    constexpr int NF = PaShape<D>::NF, RB = 4 / KS;
-    const int rb = wave % RB, stream = wave / RB;
+    constexpr int NF = PaShape<D>::NF, PARTS = kPaWaves / RB;
+    const int rb = wave % RB, part = wave / RB;
     const float l = xor32_sum(s.l);
     if constexpr (KS == 1) {
 #pragma unroll
@@ -387,14 +376,17 @@ __device__ __forceinline__ void finish(const PagedAttnArgs& a, const ItemView& v
         return;
     } else {
         auto area = [&](int w) __attribute__((always_inline)) {
-            return reinterpret_cast<float4*>(w < 2 ? s_a : s_b) + (w & 1) * NF * 64;
+            return reinterpret_cast<float4*>(w < 4 ? s_a : s_b) + (w & 3) * NF * 64;
         };
-        float4* const mine = area(wave);
+        __syncthreads();  // (an item without tiles comes here straight from the last one's merge)
+        if (part < KS) {
+            float4* const mine = area(wave);
 #pragma unroll
-        for (int f = 0; f < NF; ++f)
-            mine[f * 64 + lane] = make_float4(s.o[f / 4][4 * (f % 4)], s.o[f / 4][4 * (f % 4) + 1],
-                                              s.o[f / 4][4 * (f % 4) + 2], s.o[f / 4][4 * (f % 4) + 3]);
-        if (lane < 32) s_ml[wave][lane] = make_float2(s.m, l);
+            for (int f = 0; f < NF; ++f)
+                mine[f * 64 + lane] = make_float4(s.o[f / 4][4 * (f % 4)], s.o[f / 4][4 * (f % 4) + 1],
+                                                  s.o[f / 4][4 * (f % 4) + 2], s.o[f / 4][4 * (f % 4) + 3]);
+            if (lane < 32) s_ml[wave][lane] = make_float2(s.m, l);
+        }
         __syncthreads();
         float m = -INFINITY, w[KS], den = 0.0f;
 #pragma unroll
@@ -410,8 +402,8 @@ __device__ __forceinline__ void finish(const PagedAttnArgs& a, const ItemView& v
             den = fmaf(w[k], lk, den);
         }
 #pragma unroll
-        for (int i = 0; i < NF / KS; ++i) {
-            const int f = stream * (NF / KS) + i;
+        for (int i = 0; i < NF / PARTS; ++i) {
+            const int f = part * (NF / PARTS) + i;
             float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
@@ -423,26 +415,34 @@ __device__ __forceinline__ void finish(const PagedAttnArgs& a, const ItemView& v
             }
             put<D>(a, v, rb, lane, f, x, den);
         }
-        if (stream == 0) put_ml(a, v, rb, lane, m == -INFINITY ? 0.0f : m, den);
+        if (part == 0) put_ml(a, v, rb, lane, m == -INFINITY ? 0.0f : m, den);
     }
 }
 
-// More than 32 rows: RB = 4 or 2 row blocks, the four waves fill each 64-key
-// tile together and its 4 / RB streams take 64 / (4 / RB) of its keys.
+// More than 32 rows: RB = 8, 4 or 2 row blocks.  A step is one tile (RB = 8) or
+// two, filled by all waves; stream s of the 8 / RB takes its own 64 (RB >= 4) or
+// 32 keys of it.
 template <int D, int RB>
 __device__ __forceinline__ void run_shared(const PagedAttnArgs& a, const ItemView& v, uint16_t* s_a, uint16_t* s_b,
-                                           uint32_t* s_tab, float2 (*s_ml)[32], float scale_log2, RowView rv) {
+                                           uint2* s_tab, float2 (*s_ml)[32], float scale_log2, RowView rv) {
     using P = PaShape<D>;
-    constexpr int KS = 4 / RB, NB = 2 / KS, LOADS = 2 * P::HALF_LOADS / 4;  // per wave, tile and tensor
+    constexpr int KS = kPaWaves / RB, TILES = RB == 8 ? 1 : 2, NB = 2 * TILES / KS;
+    constexpr int ROWS = 64 * TILES / kPaWaves, LOADS = ROWS / P::RI;  // per wave, step and tensor
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ql = lane & 31, kg = lane >> 5, rb = wave % RB, stream = wave / RB;
     const uint32_t per_shift = 6 - v.src.entry_shift, chunk = kTabEntries >> per_shift;
 
-    // This lane's bytes of a load instruction's rows, blocks wave + 4j.
+    // A wave loads ROWS consecutive rows of the step, RI per instruction; this
+    // lane's bytes of an instruction's rows.
     const int lr = lane / P::CPR, phys = lane % P::CPR;
-    const uint32_t koff = lr * v.src.row_bytes + 16 * (phys ^ pk_swz<D>(P::RI * wave + lr));
-    const uint32_t voff = lr * v.src.row_bytes + 16 * (phys ^ pv_swz<D>(lr));
-    static_assert((4 * P::RI) % (D / 8) == 0, "a wave's blocks share one swizzle");
+    const int fill_tile = ROWS * wave / 64, fill_row = ROWS * wave % 64;
+    uint32_t koff[LOADS];
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j)
+        koff[j] = ((P::RI * j & 7) + lr) * v.src.row_bytes + 16 * (phys ^ pk_swz<D>(fill_row + P::RI * j + lr));
+    uint32_t voff[8 / P::RI];
+#pragma unroll
+    for (int j = 0; j < 8 / P::RI; ++j) voff[j] = (P::RI * j + lr) * v.src.row_bytes + 16 * (phys ^ pv_swz<D>(lr));
     int k_off[P::KSTEPS], v_off[P::DBLK];
 #pragma unroll
     for (int ks = 0; ks < P::KSTEPS; ++ks) k_off[ks] = ql * D + 8 * ((2 * ks + kg) ^ pk_swz<D>(ql));
@@ -455,8 +455,7 @@ __device__ __forceinline__ void run_shared(const PagedAttnArgs& a, const ItemVie
     const uint32_t last_row = v.it.rows - 1, row = min((uint32_t)(rb * 32 + ql), last_row);
     const uint32_t w_first = min((uint32_t)rb * 32, last_row), w_last = min((uint32_t)rb * 32 + 31, last_row);
     rv.pos = v.it.pos0 + (int32_t)((v.it.row0 + row) / v.group);
-    rv.first = v.it.pos0 + (int32_t)((v.it.row0 + w_first) / v.group);
-    rv.last = v.it.pos0 + (int32_t)((v.it.row0 + w_last) / v.group);
+    rv.span(v.it.pos0 + (int32_t)((v.it.row0 + w_first) / v.group), v.it.pos0 + (int32_t)((v.it.row0 + w_last) / v.group));
     const bool live = rb * 32 < (int)v.it.rows;
     bf16x8_t qf[P::KSTEPS];
     load_rows<D>(qf, a, v, row, kg);
@@ -466,133 +465,502 @@ __device__ __forceinline__ void run_shared(const PagedAttnArgs& a, const ItemVie
     for (uint32_t c0 = v.it.tile_begin; c0 < v.it.tile_end; c0 += chunk) {
         const uint32_t c1 = min(v.it.tile_end, c0 + chunk);
         __syncthreads();  // the last chunk's page numbers and tiles are done with
-        fill_table(v, s_tab, c0, c1);
+        fill_table(a, v, s_tab, c0, c1, threadIdx.x, kPaThreads);
         __syncthreads();
-        auto pages_of = [&](uint32_t t) __attribute__((always_inline)) {
-            return s_tab[((t - c0) << per_shift) + (lane & ((1u << per_shift) - 1))];
+        // This wave's part of the step from tile t on (its tile may lie past the
+        // last).
+        auto bases_of = [&](uint32_t t) __attribute__((always_inline)) {
+            return s_tab[((min(t + fill_tile, c1 - 1) - c0) << per_shift) + (lane & ((1u << per_shift) - 1))];
         };
-        auto fill = [&](uint32_t t, uint32_t pages, uint16_t* buf) __attribute__((always_inline)) {
-            const uint32_t k0 = v.src.key0(t);
+        auto fill = [&](uint32_t t, uint2 bases, uint16_t* buf) __attribute__((always_inline)) {
+            if (TILES > 1 && t + fill_tile >= c1) return;
+            uint16_t* const to = buf + P::TILE * fill_tile;
 #pragma unroll
-            for (int j = 0; j < LOADS; ++j) {
-                const int blk = wave + 4 * j, r = P::RI * blk;
-                load_lds16(row_rsrc<D>(v.src, v.src.k, pages, r >> v.src.entry_shift, k0 + r), buf + 512 * blk, koff);
-                load_lds16(row_rsrc<D>(v.src, v.src.v, pages, r >> v.src.entry_shift, k0 + r), buf + 64 * D + 512 * blk,
-                           voff);
+            for (int g = 0; g < ROWS / 8; ++g) {  // eight rows: one page
+                const uint32_t r = fill_row + 8 * g;
+                const uint64_t off = base_of(bases, r >> v.src.entry_shift) +
+                                     (r & ((1u << v.src.entry_shift) - 1)) * v.src.row_bytes;
+                const __amdgpu_buffer_rsrc_t rk = rows_at(v.src.k + off), rv = rows_at(v.src.v + off);
+#pragma unroll
+                for (int i = 0; i < 8 / P::RI; ++i) {
+                    load_lds16<0>(rk, koff[g * (8 / P::RI) + i], to + D * (r + P::RI * i));
+                    load_lds16<0>(rv, voff[i], to + D * (64 + r + P::RI * i));
+                }
             }
         };
-        uint32_t pages = pages_of(c0);
-        fill(c0, pages, s_a);
-        pages = pages_of(min(c0 + 1, c1 - 1));
-        __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
-        __syncthreads();
-        // Tile t from `cur` while tile t + 1 streams into `nxt`, whose last
-        // readers passed the previous barrier.  The wait for the loads is
-        // explicit: the compiler's tracking of loads that write LDS is not
-        // relied on.
-        auto step = [&](uint32_t t, const uint16_t* cur, uint16_t* nxt) __attribute__((always_inline)) {
-            if (t + 1 < c1) {
-                fill(t + 1, pages, nxt);
-                pages = pages_of(min(t + 2, c1 - 1));
-            }
-            const uint32_t k0 = v.src.key0(t) + 32 * NB * stream;
-            if (live && !rv.none(k0, k0 + 32 * NB - 1))
-                tile<D, NB>(s, cur + 32 * NB * stream * D, cur + (64 + 32 * NB * stream) * D, k_off, v_off, qf, rv, k0,
-                            v.src.key_end, scale_log2, kg);
+        // This wave's loads of the step from tile t into buf, and zeros over its
+        // rows of V past the last key seen.  The wait is explicit: the compiler's
+        // tracking of loads that write LDS is not relied on.
+        auto land = [&](uint32_t t, uint16_t* buf) __attribute__((always_inline)) {
             __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+            const uint32_t k0 = v.src.key0(t + fill_tile) + fill_row;
+            if (t + fill_tile < c1 && k0 + ROWS > v.src.key_end) {
+#pragma unroll
+                for (int j = 0; j < LOADS; ++j)
+                    if (k0 + P::RI * j + lr >= v.src.key_end)
+                        *reinterpret_cast<uint4*>(buf + P::TILE * fill_tile + D * (64 + fill_row + P::RI * j) + 8 * lane) =
+                            make_uint4(0, 0, 0, 0);
+            }
             __syncthreads();
         };
-        for (uint32_t t = c0; t < c1; t += 2) {
+        fill(c0, bases_of(c0), s_a);
+        uint2 bases = bases_of(c0 + TILES);
+        land(c0, s_a);
+        // The step from tile t out of `cur` while the next streams into `nxt`,
+        // whose last readers passed the previous barrier.
+        constexpr int KEYS = 32 * NB;
+        const int my_tile = KEYS * stream / 64, my_row = KEYS * stream % 64;
+        auto step = [&](uint32_t t, const uint16_t* cur, uint16_t* nxt) __attribute__((always_inline)) {
+            if (t + TILES < c1) {
+                fill(t + TILES, bases, nxt);
+                bases = bases_of(t + 2 * TILES);
+            }
+            const uint32_t k0 = v.src.key0(t + my_tile) + my_row;
+            const uint16_t* const kb = cur + P::TILE * my_tile + D * my_row;
+            if (live && (TILES == 1 || t + my_tile < c1) && !rv.none(k0, k0 + KEYS - 1))
+                tile<D, NB>(s, kb, kb + 64 * D, k_off, v_off, qf, rv, k0, v.src.key_end, scale_log2, lane, a.flags);
+            land(t + TILES, nxt);
+        };
+        for (uint32_t t = c0; t < c1; t += 2 * TILES) {
             step(t, s_a, s_b);
-            if (t + 1 < c1) step(t + 1, s_b, s_a);
+            if (t + TILES < c1) step(t + TILES, s_b, s_a);
         }
     }
-    finish<D, KS>(a, v, s, s_a, s_b, s_ml, wave, lane);
+    finish<D, RB, KS>(a, v, s, s_a, s_b, s_ml, wave, lane);
 }
 
-// Up to 32 rows: wave w streams the 32-key halves w, w + 4, ... of the tiles.
+// Operand reads of the streaming form, in asm: to the compiler they are no LDS
+// accesses, which it would make wait for every load in flight that writes LDS.
+// Each block waits for its own reads.  The swizzles make a k-step's (K) or a
+// d-block's (V) address the first one's with a bit or two flipped.
+template <int KSTEPS>
+__device__ __forceinline__ void read_k(uint4 (&k)[KSTEPS], uint2& bases, uint32_t at, uint32_t bases_at) {
+    typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+    typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+    u4_t r[KSTEPS];
+    u2_t e;
+    if constexpr (KSTEPS == 8)
+        asm volatile(
+            "ds_read_b64 %8, %17\n\t"
+            "ds_read_b128 %0, %9\n\t"
+            "ds_read_b128 %1, %10\n\t"
+            "ds_read_b128 %2, %11\n\t"
+            "ds_read_b128 %3, %12\n\t"
+            "ds_read_b128 %4, %13\n\t"
+            "ds_read_b128 %5, %14\n\t"
+            "ds_read_b128 %6, %15\n\t"
+            "ds_read_b128 %7, %16\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]),
+              "=&v"(e)
+            : "v"(at), "v"(at ^ 32), "v"(at ^ 64), "v"(at ^ 96), "v"(at ^ 128), "v"(at ^ 160), "v"(at ^ 192),
+              "v"(at ^ 224), "v"(bases_at)
+            : "memory");
+    else
+        asm volatile(
+            "ds_read_b64 %4, %9\n\t"
+            "ds_read_b128 %0, %5\n\t"
+            "ds_read_b128 %1, %6\n\t"
+            "ds_read_b128 %2, %7\n\t"
+            "ds_read_b128 %3, %8\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(e)
+            : "v"(at), "v"(at ^ 32), "v"(at ^ 64), "v"(at ^ 96), "v"(bases_at)
+            : "memory");
+#pragma unroll
+    for (int i = 0; i < KSTEPS; ++i) k[i] = make_uint4(r[i].x, r[i].y, r[i].z, r[i].w);
+    bases = make_uint2(e.x, e.y);
+}
+
+// V^T operands of 32 keys: v[tt][db].
+__device__ __forceinline__ void read_v(uint4 (&v)[2][4], uint32_t at) {
+    typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+    u2_t r[16];  // d-block 0: keys 0, 8, 16, 24 on; d-block 1: ...
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %16\n\t"
+        "ds_read_b64_tr_b16 %1, %16 offset:2048\n\t"
+        "ds_read_b64_tr_b16 %2, %16 offset:4096\n\t"
+        "ds_read_b64_tr_b16 %3, %16 offset:6144\n\t"
+        "ds_read_b64_tr_b16 %4, %17\n\t"
+        "ds_read_b64_tr_b16 %5, %17 offset:2048\n\t"
+        "ds_read_b64_tr_b16 %6, %17 offset:4096\n\t"
+        "ds_read_b64_tr_b16 %7, %17 offset:6144\n\t"
+        "ds_read_b64_tr_b16 %8, %18\n\t"
+        "ds_read_b64_tr_b16 %9, %18 offset:2048\n\t"
+        "ds_read_b64_tr_b16 %10, %18 offset:4096\n\t"
+        "ds_read_b64_tr_b16 %11, %18 offset:6144\n\t"
+        "ds_read_b64_tr_b16 %12, %19\n\t"
+        "ds_read_b64_tr_b16 %13, %19 offset:2048\n\t"
+        "ds_read_b64_tr_b16 %14, %19 offset:4096\n\t"
+        "ds_read_b64_tr_b16 %15, %19 offset:6144\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]),
+          "=&v"(r[8]), "=&v"(r[9]), "=&v"(r[10]), "=&v"(r[11]), "=&v"(r[12]), "=&v"(r[13]), "=&v"(r[14]), "=&v"(r[15])
+        : "v"(at), "v"(at ^ 64), "v"(at ^ 128), "v"(at ^ 192)
+        : "memory");
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+            v[tt][db] = make_uint4(r[4 * db + 2 * tt].x, r[4 * db + 2 * tt].y, r[4 * db + 2 * tt + 1].x,
+                                   r[4 * db + 2 * tt + 1].y);
+}
+__device__ __forceinline__ void read_v(uint4 (&v)[2][2], uint32_t at) {
+    typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+    u2_t r[8];
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8\n\t"
+        "ds_read_b64_tr_b16 %1, %8 offset:1024\n\t"
+        "ds_read_b64_tr_b16 %2, %8 offset:2048\n\t"
+        "ds_read_b64_tr_b16 %3, %8 offset:3072\n\t"
+        "ds_read_b64_tr_b16 %4, %9\n\t"
+        "ds_read_b64_tr_b16 %5, %9 offset:1024\n\t"
+        "ds_read_b64_tr_b16 %6, %9 offset:2048\n\t"
+        "ds_read_b64_tr_b16 %7, %9 offset:3072\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+        : "v"(at), "v"(at ^ 64)
+        : "memory");
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int db = 0; db < 2; ++db)
+            v[tt][db] = make_uint4(r[4 * db + 2 * tt].x, r[4 * db + 2 * tt].y, r[4 * db + 2 * tt + 1].x,
+                                   r[4 * db + 2 * tt + 1].y);
+}
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return (uint32_t)(size_t)(const __attribute__((address_space(3))) void*)p;
+}
+
+// A plan entry that no launch in flight writes, by scalar loads.
+template <typename T>
+__device__ __forceinline__ T plan_load(const void* plan, uint64_t byte) {
+    static_assert(sizeof(T) % 16 == 0, "whole loads");
+    typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+    u4_t w[sizeof(T) / 16];
+#pragma unroll
+    for (size_t i = 0; i < sizeof(T) / 16; ++i)
+        w[i] = reinterpret_cast<const u4_t __attribute__((address_space(4)))*>(
+            (uint64_t)plan + byte)[i];
+    return __builtin_bit_cast(T, w);
+}
+
+// The part of the header that the kernels read.  A plan that was made for
+// other arguments does not fit: the attention then fills o with NaN.
+struct PlanHead {
+    uint32_t batch, num_tokens, page_size, max_blocks, window, sinks, hq, hkv, d, magic, items, split_blocks, ranges, units;
+    uint32_t pad[2];
+    __device__ __forceinline__ bool fits(const PagedPlanHeader& w) const {
+        return ((batch ^ w.batch) | (num_tokens ^ w.num_tokens) | (page_size ^ w.page_size) |
+                (max_blocks ^ w.max_blocks) | (window ^ w.window) | (sinks ^ w.sinks) | (hq ^ w.hq) | (hkv ^ w.hkv) |
+                (d ^ w.d) | (magic ^ kPagedMagic)) == 0;
+    }
+};
+
+// What the workgroup runs next, in LDS: an item or, of a streamed one, as many
+// of its tiles as a table holds.
+constexpr uint32_t kSegEntries = kTabEntries / 2;
+struct Segment {
+    PagedItem it;      // tile_end is the segment's; the item's is below
+    uint32_t kvh, kind, item_end, opens;
+};
+enum : uint32_t { kSegNone = 0, kSegStream = 1, kSegShared = 2 };
+
+// By one wave: `it` of KV head `kvh` from tile `from` on as a segment, with the
+// table and the query rows of a streamed one.
 template <int D>
-__device__ __forceinline__ void run_streams(const PagedAttnArgs& a, const ItemView& v, uint16_t* s_a, uint16_t* s_b,
-                                            uint32_t* s_tab, float2 (*s_ml)[32], float scale_log2, RowView rv) {
+__device__ __forceinline__ void stage(const PagedAttnArgs& a, ItemView& v, PagedItem it, uint32_t kvh, uint32_t from,
+                                      Segment* seg, uint2* tab, uint16_t* q) {
+    const uint32_t lane = threadIdx.x & 63;
+    const bool opens = from == it.tile_begin;
+    const uint32_t item_end = it.tile_end;
+    point_at(v, a, it, kvh);
+    uint32_t kind = kSegShared;
+    if (it.rows <= 32) {
+        kind = kSegStream;
+        const uint32_t per_shift = 6 - v.src.entry_shift;
+        it.tile_begin = from;
+        it.tile_end = min(item_end, from + (kSegEntries >> per_shift));
+        if (opens) {
+            constexpr uint32_t CPR = D / 8;
+            for (uint32_t i = lane; i < it.rows * CPR; i += 64) {
+                const uint32_t row = i / CPR, c = i % CPR, r = it.row0 + row;
+                const uint32_t token = it.token0 + r / v.group, head = kvh * v.group + r % v.group;
+                *reinterpret_cast<uint4*>(q + row * D + 8 * (c ^ pk_swz<D>(row))) =
+                    ldg16(a.q + ((uint64_t)token * a.head.hq + head) * D + 8 * c);
+            }
+        }
+        fill_table(a, v, tab, it.tile_begin, it.tile_end, lane, 64);
+    }
+    if (lane == 0) {
+        Segment s;
+        s.it = it;
+        s.kvh = kvh;
+        s.kind = kind;
+        s.item_end = item_end;
+        s.opens = opens;
+        *seg = s;
+    }
+}
+
+// By one wave: what follows item `it` of KV head `kvh` in its list, or the
+// list of a ticket (`drawn`: lane 0 holds one), staged.
+template <int D>
+__device__ __forceinline__ void advance(const PagedAttnArgs& a, ItemView& v, const PlanHead& head, PagedItem it,
+                                        uint32_t kvh, bool drawn, uint32_t ticket, Segment* seg, uint2* tab,
+                                        uint16_t* q) {
+    const uint32_t lane = threadIdx.x & 63, hkv = a.head.hkv, lanes = paged_lanes(hkv);
+    uint32_t idx = it.next;
+    while (true) {
+        if (idx == kPagedNone) {
+            if (head.ranges <= lanes) break;
+            if (!drawn && lane == 0) ticket = atomicAdd(a.tickets + kvh, 1u);
+            drawn = false;
+            idx = lanes + __builtin_amdgcn_readfirstlane(ticket);
+            // This head's lists are gone: the head with the most left.  The
+            // counters only grow, so this ends.
+            while (idx >= head.ranges) {
+                const uint32_t mine = (kvh + lane) % hkv;
+                const uint32_t gone = __hip_atomic_load(a.tickets + mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                uint32_t least = gone;
+#pragma unroll
+                for (int m = 32; m >= 1; m >>= 1) least = min(least, (uint32_t)__shfl_xor(least, m));
+                if (lanes + least >= head.ranges) break;
+                kvh = __builtin_amdgcn_readlane(mine, __builtin_ctzll(__ballot(gone == least)));
+                if (lane == 0) ticket = atomicAdd(a.tickets + kvh, 1u);
+                idx = lanes + __builtin_amdgcn_readfirstlane(ticket);
+            }
+            if (idx >= head.ranges) break;
+        }
+        it = plan_load<PagedItem>(a.plan, sizeof(PagedPlanHeader) + (uint64_t)idx * sizeof(PagedItem));
+        if (it.rows) {
+            stage<D>(a, v, it, kvh, it.tile_begin, seg, tab, q);
+            return;
+        }
+        idx = kPagedNone;  // an empty list
+    }
+    if (lane == 0) seg->kind = kSegNone;
+}
+
+// Workgroup barrier that waits for this wave's LDS operations only and leaves
+// its loads in flight.
+__device__ __forceinline__ void lds_ops_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Up to 32 rows: wave w < kStreams streams the 32-key halves w, w + kStreams,
+// ... of a segment's tiles, and on into the next segment, which wave kStreams
+// stages meanwhile: a wave's first loads of it go out behind its last ones of
+// this, and are in flight while the streams merge.  (Staged by all waves after
+// the merge, a new item cost 20 us of its workgroup under load: its ticket, the
+// item, the table and the first keys are fetched one after the other.)
+// Runs segments from `slot` on; returns the slot of one that is not streamed.
+template <int D>
+__device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView v, const PlanHead& head,
+                                                uint32_t slot, Segment* s_seg, uint16_t* s_a, uint16_t* s_b,
+                                                uint2* s_tab, uint16_t* s_q, float2 (*s_ml)[32], float scale_log2,
+                                                RowView rv) {
     using P = PaShape<D>;
-    constexpr int NL = P::HALF_LOADS;
+    constexpr int NL = P::HALF_LOADS, NF = P::NF, NT = 2;  // non-temporal: the keys are read once
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ql = lane & 31, kg = lane >> 5;
-    const uint32_t per_shift = 6 - v.src.entry_shift, chunk = kTabEntries >> per_shift;
-    uint16_t* const sk = s_a + wave * 32 * D;
-    uint16_t* const sv = s_b + wave * 32 * D;
+    const uint32_t per_shift = 6 - v.src.entry_shift, half = wave & 1;
+    uint16_t* const sk = s_a + (wave % kStreams) * 32 * D;
+    uint16_t* const sv = s_b + (wave % kStreams) * 32 * D;
+    // The merge lies behind the streams' tiles: stream k's 32 rows in fragment
+    // order at merge_at(k).
+    const uint32_t merge_a = lds_address(s_a + P::BUF / 2), merge_b = lds_address(s_b + P::BUF / 2);
+    static_assert(kStreams * 32 * D <= P::BUF / 2 && kStreams == 4, "tiles in the first half, two streams' rows in each second");
+    auto merge_at = [&](int k) __attribute__((always_inline)) {
+        return (k < 2 ? merge_a : merge_b) + (k & 1) * NF * 1024 + 16 * lane;
+    };
 
     const int lr = lane / P::CPR, phys = lane % P::CPR;
     constexpr int SWZ = D / 8 / P::RI;  // instructions after which K's swizzle repeats
     uint32_t koff[SWZ];
 #pragma unroll
-    for (int j = 0; j < SWZ; ++j) koff[j] = lr * v.src.row_bytes + 16 * (phys ^ pk_swz<D>(P::RI * j + lr));
-    const uint32_t voff = lr * v.src.row_bytes + 16 * (phys ^ pv_swz<D>(lr));
-    int k_off[P::KSTEPS], v_off[P::DBLK];
+    for (int j = 0; j < SWZ; ++j)
+        koff[j] = ((P::RI * j & 7) + lr) * v.src.row_bytes + 16 * (phys ^ pk_swz<D>(P::RI * j + lr));
+    uint32_t voff[8 / P::RI];
 #pragma unroll
-    for (int ks = 0; ks < P::KSTEPS; ++ks) k_off[ks] = ql * D + 8 * ((2 * ks + kg) ^ pk_swz<D>(ql));
+    for (int j = 0; j < 8 / P::RI; ++j) voff[j] = (P::RI * j + lr) * v.src.row_bytes + 16 * (phys ^ pv_swz<D>(lr));
+    int v_off[P::DBLK];
     {
         const int s16 = lane & 15, g16 = lane >> 4, vrow = 4 * kg + (s16 >> 2);
 #pragma unroll
         for (int db = 0; db < P::DBLK; ++db)
             v_off[db] = vrow * D + 8 * ((4 * db + 2 * (g16 & 1) + ((s16 & 3) >> 1)) ^ pv_swz<D>(vrow)) + 4 * (s16 & 1);
     }
-    const uint32_t last_row = v.it.rows - 1, row = min((uint32_t)ql, last_row);
-    rv.pos = v.it.pos0 + (int32_t)((v.it.row0 + row) / v.group);
-    rv.first = v.it.pos0 + (int32_t)(v.it.row0 / v.group);
-    rv.last = v.it.pos0 + (int32_t)((v.it.row0 + last_row) / v.group);
-    bf16x8_t qf[P::KSTEPS];
-    load_rows<D>(qf, a, v, row, kg);
-    RowState<D> s;
-    clear(s);
-
-    for (uint32_t c0 = v.it.tile_begin; c0 < v.it.tile_end; c0 += chunk) {
-        const uint32_t c1 = min(v.it.tile_end, c0 + chunk);
-        __syncthreads();
-        fill_table(v, s_tab, c0, c1);
-        __syncthreads();
-        auto pages_of = [&](uint32_t h) __attribute__((always_inline)) {
-            return s_tab[(((h >> 1) - c0) << per_shift) + (lane & ((1u << per_shift) - 1))];
-        };
-        auto key_of = [&](uint32_t h) __attribute__((always_inline)) { return v.src.key0(h >> 1) + 32 * (h & 1); };
-        auto fill_k = [&](uint32_t h, uint32_t pages) __attribute__((always_inline)) {
-            const uint32_t k0 = key_of(h), r0 = 32 * (h & 1);
+    const uint32_t k_at = lds_address(sk + ql * D + 8 * (kg ^ pk_swz<D>(ql))), v_at = lds_address(sv + v_off[0]);
+    // This wave's halves lie in one half of their tiles.
+    auto fill_k = [&](const char* from, uint2 bases) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < NL; ++j)
-                load_lds16(row_rsrc<D>(v.src, v.src.k, pages, (r0 + P::RI * j) >> v.src.entry_shift, k0 + P::RI * j),
-                           sk + 512 * j, koff[j % SWZ]);
-        };
-        auto fill_v = [&](uint32_t h, uint32_t pages) __attribute__((always_inline)) {
-            const uint32_t k0 = key_of(h), r0 = 32 * (h & 1);
+        for (int g = 0; g < 4; ++g) {  // eight rows: one page
+            const uint32_t r = 32 * half + 8 * g;
+            const __amdgpu_buffer_rsrc_t rows = rows_at(from + base_of(bases, r >> v.src.entry_shift) +
+                                                        (r & ((1u << v.src.entry_shift) - 1)) * v.src.row_bytes);
 #pragma unroll
-            for (int j = 0; j < NL; ++j)
-                load_lds16(row_rsrc<D>(v.src, v.src.v, pages, (r0 + P::RI * j) >> v.src.entry_shift, k0 + P::RI * j),
-                           sv + 512 * j, voff);
-        };
-        const uint32_t end = 2 * c1;
-        uint32_t h = 2 * c0 + wave;
-        if (h < end) {
-            const uint32_t pages = pages_of(h);
-            fill_k(h, pages);
-            fill_v(h, pages);
+            for (int i = 0; i < 8 / P::RI; ++i)
+                load_lds16<NT>(rows, koff[(g * (8 / P::RI) + i) % SWZ], sk + D * (8 * g + P::RI * i));
         }
-        for (; h < end; h += 4) {
-            const uint32_t next = h + 4, k0 = key_of(h);
-            const bool more = next < end;
-            const uint32_t pages = more ? pages_of(next) : 0;
+    };
+    auto fill_v = [&](const char* from, uint2 bases) __attribute__((always_inline)) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const uint32_t r = 32 * half + 8 * g;
+            const __amdgpu_buffer_rsrc_t rows = rows_at(from + base_of(bases, r >> v.src.entry_shift) +
+                                                        (r & ((1u << v.src.entry_shift) - 1)) * v.src.row_bytes);
+#pragma unroll
+            for (int i = 0; i < 8 / P::RI; ++i) load_lds16<NT>(rows, voff[i], sv + D * (8 * g + P::RI * i));
+        }
+    };
+    // Entry of half h of a segment that begins at tile c0.
+    auto entry_of = [&](uint32_t at, uint32_t h, uint32_t c0) __attribute__((always_inline)) {
+        return s_tab + at * kSegEntries + (((h >> 1) - c0) << per_shift) + (lane & ((1u << per_shift) - 1));
+    };
+    // Of a segment: the halves that hold a key which is seen end here.
+    auto end_of = [&](const PagedItem& it) __attribute__((always_inline)) {
+        if (it.tile_end <= it.tile_begin) return 2 * it.tile_begin;
+        KeySource k = v.src;
+        k.low_tile = it.low_tile;
+        k.sink_tiles = it.sink_tiles;
+        return k.key0(it.tile_end - 1) + 32 < it.key_end ? 2 * it.tile_end : 2 * it.tile_end - 1;
+    };
+    auto segment = [&](uint32_t at) __attribute__((always_inline)) {
+        Segment s;
+        uint32_t w[sizeof(Segment) / 4];
+#pragma unroll
+        for (size_t i = 0; i < sizeof(Segment) / 4; ++i)
+            w[i] = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t*>(s_seg + at)[i]);
+        __builtin_memcpy(&s, w, sizeof(s));
+        return s;
+    };
+
+    // All waves, after the streams' results are in LDS.
+    auto merge = [&]() __attribute__((always_inline)) {
+        float m = -INFINITY, w[kStreams], den = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kStreams; ++k) {
+            const float2 ml = s_ml[k][lane & 31];
+            w[k] = ml.x;
+            if (ml.y != 0.0f) m = fmaxf(m, ml.x);
+        }
+#pragma unroll
+        for (int k = 0; k < kStreams; ++k) {
+            const float lk = s_ml[k][lane & 31].y;
+            w[k] = lk != 0.0f ? __builtin_amdgcn_exp2f(w[k] - m) : 0.0f;
+            den = fmaf(w[k], lk, den);
+        }
+#pragma unroll
+        for (int i = 0; i < NF / kPaWaves; ++i) {
+            const int f = wave * (NF / kPaWaves) + i;
+            f32x4_t y[kStreams];
+            asm volatile(
+                "ds_read_b128 %0, %4\n\t"
+                "ds_read_b128 %1, %5\n\t"
+                "ds_read_b128 %2, %6\n\t"
+                "ds_read_b128 %3, %7\n\t"
+                "s_waitcnt lgkmcnt(0)"
+                : "=&v"(y[0]), "=&v"(y[1]), "=&v"(y[2]), "=&v"(y[3])
+                : "v"(merge_at(0) + f * 1024), "v"(merge_at(1) + f * 1024), "v"(merge_at(2) + f * 1024),
+                  "v"(merge_at(3) + f * 1024)
+                : "memory");
+            f32x4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < kStreams; ++k) x += w[k] * y[k];
+            put<D>(a, v, 0, lane, f, make_float4(x.x, x.y, x.z, x.w), den);
+        }
+        if (wave == 0) put_ml(a, v, 0, lane, m == -INFINITY ? 0.0f : m, den);
+    };
+
+    if (wave >= kStreams) {
+        while (true) {
+            const Segment seg = segment(slot);
+            if (seg.kind != kSegStream) return slot;
+            point_at(v, a, seg.it, seg.kvh);
+            const bool closes = seg.it.tile_end == seg.item_end;
+            if (wave == kStreams) {
+                const uint32_t to = slot ^ 1;
+                PagedItem it = seg.it;
+                it.tile_end = seg.item_end;
+                ItemView w = v;
+                if (closes)
+                    advance<D>(a, w, head, it, seg.kvh, false, 0, s_seg + to, s_tab + to * kSegEntries, s_q + to * 32 * D);
+                else
+                    stage<D>(a, w, it, seg.kvh, seg.it.tile_end, s_seg + to, s_tab + to * kSegEntries, s_q + to * 32 * D);
+            }
+            lds_ops_barrier();  // the next segment is staged
+            lds_ops_barrier();  // this one's results are in LDS, its table and rows done with
+            if (closes) merge();
+            slot ^= 1;
+        }
+    }
+    RowState<D> s;
+    bf16x8_t qf[P::KSTEPS];
+    bool armed = false;  // this wave's first loads of the segment are out
+    while (true) {
+        const Segment seg = segment(slot);
+        if (seg.kind != kSegStream) return slot;
+        point_at(v, a, seg.it, seg.kvh);
+        const bool closes = seg.it.tile_end == seg.item_end;
+        bool next_has = false;
+        const uint32_t last_row = seg.it.rows - 1, row = min((uint32_t)ql, last_row);
+        rv.pos = seg.it.pos0 + (int32_t)((seg.it.row0 + row) / v.group);
+        rv.span(seg.it.pos0 + (int32_t)(seg.it.row0 / v.group), seg.it.pos0 + (int32_t)((seg.it.row0 + last_row) / v.group));
+        const uint32_t c0 = seg.it.tile_begin, end = end_of(seg.it);
+        uint32_t h = 2 * c0 + wave;
+        const uint32_t n = h < end ? (end - h + kStreams - 1) / kStreams : 0;
+        if (!armed && n) {
+            const uint2 bases = *entry_of(slot, h, c0);
+            fill_k(v.src.k, bases);
+            fill_v(v.src.v, bases);
+        }
+        if (seg.opens) {
+            const uint16_t* const q = s_q + slot * 32 * D + row * D;
+#pragma unroll
+            for (int ks = 0; ks < P::KSTEPS; ++ks)
+                qf[ks] = as_bf16x8(*reinterpret_cast<const uint4*>(q + 8 * ((2 * ks + kg) ^ pk_swz<D>(row))));
+            clear(s);
+        }
+        // The next segment is known from this iteration on.
+        const uint32_t meet = n > 2 ? 2 : n ? n - 1 : 0;
+        const char *next_k = nullptr, *next_v = nullptr;
+        uint32_t next_c0 = 0;
+        auto look_ahead = [&]() __attribute__((always_inline)) {
+            lds_ops_barrier();
+            const Segment nx = segment(slot ^ 1);
+            if (nx.kind != kSegStream) return;
+            next_c0 = nx.it.tile_begin;
+            next_has = 2 * next_c0 + wave < end_of(nx.it);
+            next_k = reinterpret_cast<const char*>(a.k_cache + (uint64_t)nx.kvh * D);
+            next_v = reinterpret_cast<const char*>(a.v_cache + (uint64_t)nx.kvh * D);
+        };
+        if (n == 0) {
+            look_ahead();
+            if (next_has) {
+                const uint2 bases = *entry_of(slot ^ 1, 2 * next_c0 + wave, next_c0);
+                fill_k(next_k, bases);
+                fill_v(next_v, bases);
+            }
+        }
+        for (uint32_t i = 0; i < n; ++i, h += kStreams) {
+            if (i == meet) look_ahead();
+            const uint32_t k0 = v.src.key0(h >> 1) + 32 * half;
+            const bool inside = i + 1 < n, more = inside || next_has;
+            const char* const from_k = inside ? v.src.k : next_k;
+            const char* const from_v = inside ? v.src.v : next_v;
+            const uint2* const entry = inside     ? entry_of(slot, h + kStreams, c0)
+                                       : next_has ? entry_of(slot ^ 1, 2 * next_c0 + wave, next_c0)
+                                                  : entry_of(slot, h, c0);
             // K has landed (V, requested after it, may not have): its operands
             // to registers, then the next K into its place.
             __builtin_amdgcn_s_waitcnt(wait_vmcnt(NL));
-            __builtin_amdgcn_sched_barrier(0);
             uint4 ka[P::KSTEPS];
-#pragma unroll
-            for (int ks = 0; ks < P::KSTEPS; ++ks) ka[ks] = *reinterpret_cast<const uint4*>(sk + k_off[ks]);
-            __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
-            __builtin_amdgcn_sched_barrier(0);
-            if (more) fill_k(next, pages);
+            uint2 bases;
+            read_k(ka, bases, k_at, lds_address(entry));
+            if (more) fill_k(from_k, bases);
             f32x16_t st[1];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) st[0][i] = 0.0f;
+            for (int j = 0; j < 16; ++j) st[0][j] = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < P::KSTEPS; ++ks) st[0] = mfma32x32x16(as_bf16x8(ka[ks]), qf[ks], st[0]);
             const uint32_t k1 = k0 + 31;
@@ -605,100 +973,170 @@ __device__ __forceinline__ void run_streams(const PagedAttnArgs& a, const ItemVi
                 __builtin_amdgcn_s_waitcnt(wait_vmcnt(NL));
             else
                 __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
-            __builtin_amdgcn_sched_barrier(0);
-            if (hidden && k0 < v.src.key_end && rv.some_hidden(k0, min(k1, v.src.key_end - 1)) &&
-                any_nonfinite<D, 1>(sv, v_off)) {
-                values_isolated<D, 1>(s, sv, v_off, pf, rv, k0, kg);
+            if (hidden) {
+                asm volatile("" ::: "memory");
+#pragma unroll
+                for (int j = 0; j < NL; ++j)
+                    if (k0 + P::RI * j + lr >= v.src.key_end)
+                        *reinterpret_cast<uint4*>(sv + 512 * j + 8 * lane) = make_uint4(0, 0, 0, 0);
                 __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
-                __builtin_amdgcn_sched_barrier(0);
-                if (more) fill_v(next, pages);
-            } else {
-                uint4 va[2][P::DBLK];
-#pragma unroll
-                for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                    for (int db = 0; db < P::DBLK; ++db) va[tt][db] = v_operand<D>(sv, v_off[db], tt);
-                __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
-                __builtin_amdgcn_sched_barrier(0);
-                if (more) fill_v(next, pages);
-#pragma unroll
-                for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                    for (int db = 0; db < P::DBLK; ++db)
-                        s.o[db] = mfma32x32x16(as_bf16x8(va[tt][db]), pf[tt], s.o[db]);
+                if (rv.some_hidden(k0, min(k1, v.src.key_end - 1)) && any_nonfinite<D, 1>(sv, lane)) *a.flags = 1;
             }
+            uint4 va[2][P::DBLK];
+            read_v(va, v_at);
+            if (more) fill_v(from_v, bases);
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int db = 0; db < P::DBLK; ++db)
+                    s.o[db] = mfma32x32x16(as_bf16x8(va[tt][db]), pf[tt], s.o[db]);
         }
+        if (closes) {
+            const float l = xor32_sum(s.l);
+            const uint32_t to = merge_at(wave);
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+                const f32x4_t x = {s.o[f / 4][4 * (f % 4)], s.o[f / 4][4 * (f % 4) + 1], s.o[f / 4][4 * (f % 4) + 2],
+                                   s.o[f / 4][4 * (f % 4) + 3]};
+                asm volatile("ds_write_b128 %0, %1 offset:%2" ::"v"(to), "v"(x), "n"(f * 1024) : "memory");
+            }
+            if (lane < 32) s_ml[wave][lane] = make_float2(s.m, l);
+        }
+        lds_ops_barrier();
+        if (closes) merge();
+        armed = next_has;
+        slot ^= 1;
     }
-    __syncthreads();  // every wave is done with its tiles
-    finish<D, 4>(a, v, s, s_a, s_b, s_ml, wave, lane);
-}
-
-// Whether the plan was made for these arguments; a launch with another plan
-// fills o with NaN.
-__device__ __forceinline__ bool plan_fits(const PagedPlanHeader& want, const void* plan) {
-    const uint32_t* h = static_cast<const uint32_t*>(plan);
-    return scalar_load(h) == want.batch && scalar_load(h + 1) == want.num_tokens &&
-           scalar_load(h + 2) == want.page_size && scalar_load(h + 3) == want.max_blocks &&
-           scalar_load(h + 4) == want.window && scalar_load(h + 5) == want.sinks && scalar_load(h + 6) == want.hq &&
-           scalar_load(h + 7) == want.hkv && scalar_load(h + 8) == want.d && scalar_load(h + 9) == kPagedMagic;
 }
 
 template <int D>
-__global__ __launch_bounds__(kPaThreads, 2) void paged_attn_kernel(PagedAttnArgs a, float scale_log2) {
+__global__ __launch_bounds__(kPaThreads, 1) void paged_attn_kernel(PagedAttnArgs a, float scale_log2) {
     __shared__ __align__(1024) uint16_t s_a[PaShape<D>::BUF];
     __shared__ __align__(1024) uint16_t s_b[PaShape<D>::BUF];
-    __shared__ uint32_t s_tab[kTabEntries];
-    __shared__ float2 s_ml[4][32];
+    __shared__ uint2 s_tab[kTabEntries];
+    __shared__ __align__(16) uint16_t s_q[2 * 32 * D];
+    __shared__ float2 s_ml[kPaWaves][32];
+    __shared__ Segment s_seg[2];
     const uint32_t hkv = a.head.hkv, lanes = paged_lanes(hkv);
     const uint32_t kvh = blockIdx.x % hkv, l = blockIdx.x / hkv;
-    if (!plan_fits(a.head, a.plan)) {
+    const PlanHead head = plan_load<PlanHead>(a.plan, 0);
+    const PagedItem first = plan_load<PagedItem>(a.plan, sizeof(PagedPlanHeader) + (uint64_t)l * sizeof(PagedItem));
+    if (!head.fits(a.head)) {
         const uint64_t n = (uint64_t)a.head.num_tokens * a.head.hq * (D / 8);
         for (uint64_t i = (uint64_t)blockIdx.x * kPaThreads + threadIdx.x; i < n; i += (uint64_t)gridDim.x * kPaThreads)
             reinterpret_cast<uint4*>(a.o)[i] = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
         return;
     }
-    const uint32_t* plan = static_cast<const uint32_t*>(a.plan);
-    const uint32_t n_items = scalar_load(plan + 11);
-    const uint32_t* items = plan + sizeof(PagedPlanHeader) / 4;
     RowView rv{};
     rv.window = a.head.window && a.head.window < 0x80000000u ? a.head.window : 0x80000000u;
     rv.sinks = a.head.window ? a.head.sinks : 0;
-    ItemView v;
-    v.kvh = kvh;
+    ItemView v{};
     v.group = a.head.hq / hkv;
-    v.num_pages = a.num_pages;
     v.src.page_shift = 31 - __builtin_clz(a.head.page_size);
     v.src.entry_shift = min(v.src.page_shift, 6u);
     v.src.row_bytes = hkv * D * 2;
     v.src.page_bytes = 2 * a.page_stride;
-    v.src.k = reinterpret_cast<const char*>(a.k_cache + (uint64_t)kvh * D);
-    v.src.v = reinterpret_cast<const char*>(a.v_cache + (uint64_t)kvh * D);
-    for (uint32_t round = 0;; ++round) {
-        const uint32_t idx = round * lanes + (round & 1 ? lanes - 1 - l : l);
-        if (idx >= n_items) {
-            // An odd round's unused places are its first lanes': nothing follows.
-            break;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint32_t slot = 0;
+    if (wave == 0) {
+        ItemView w = v;
+        if (first.rows)
+            stage<D>(a, w, first, kvh, first.tile_begin, s_seg, s_tab, s_q);
+        else  // (an empty list: further ones may not be)
+            advance<D>(a, w, head, PagedItem{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, kPagedNone}, kvh, false, 0, s_seg, s_tab, s_q);
+    }
+    __syncthreads();
+    while (s_seg[slot].kind != kSegNone) {
+        if (s_seg[slot].kind == kSegStream) {
+            slot = run_streams<D>(a, v, head, slot, s_seg, s_a, s_b, s_tab, s_q, s_ml, scale_log2, rv);
+            continue;
         }
-        const uint32_t* w = items + (uint64_t)idx * (sizeof(PagedItem) / 4);
-        v.it.req = scalar_load(w);
-        v.it.token0 = scalar_load(w + 1);
-        v.it.row0 = scalar_load(w + 2);
-        v.it.rows = scalar_load(w + 3);
-        v.it.pos0 = (int32_t)scalar_load(w + 4);
-        v.src.key_end = scalar_load(w + 5);
-        v.src.low_tile = scalar_load(w + 6);
-        v.src.sink_tiles = scalar_load(w + 7);
-        v.it.tile_begin = scalar_load(w + 8);
-        v.it.tile_end = scalar_load(w + 9);
-        v.it.partial = scalar_load(w + 10);
-        v.table = a.block_tables + (uint64_t)v.it.req * a.head.max_blocks;
-        if (v.it.rows > 64)
+        Segment seg;
+        {
+            uint32_t w[sizeof(Segment) / 4];
+#pragma unroll
+            for (size_t i = 0; i < sizeof(Segment) / 4; ++i)
+                w[i] = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t*>(s_seg + slot)[i]);
+            __builtin_memcpy(&seg, w, sizeof(seg));
+        }
+        point_at(v, a, seg.it, seg.kvh);
+        // A ticket for the list after this one, drawn now and looked at below.
+        const bool draws = head.ranges > lanes && seg.it.next == kPagedNone;
+        uint32_t ticket = 0;
+        if (draws && threadIdx.x == 0) ticket = atomicAdd(a.tickets + seg.kvh, 1u);
+        if (v.it.rows > 128)
+            run_shared<D, 8>(a, v, s_a, s_b, s_tab, s_ml, scale_log2, rv);
+        else if (v.it.rows > 64)
             run_shared<D, 4>(a, v, s_a, s_b, s_tab, s_ml, scale_log2, rv);
-        else if (v.it.rows > 32)
-            run_shared<D, 2>(a, v, s_a, s_b, s_tab, s_ml, scale_log2, rv);
         else
-            run_streams<D>(a, v, s_a, s_b, s_tab, s_ml, scale_log2, rv);
+            run_shared<D, 2>(a, v, s_a, s_b, s_tab, s_ml, scale_log2, rv);
+        __syncthreads();  // every wave is done with the tiles
+        if (wave == 0) {
+            ItemView w = v;
+            advance<D>(a, w, head, seg.it, seg.kvh, draws, ticket, s_seg, s_tab, s_q);
+        }
+        slot = 0;
         __syncthreads();
+    }
+}
+
+// One row's attention again, by a wave, key by key over those that it sees: a
+// lane takes D / 64 of the dims.  Slow, and only for rows that an infinity or
+// NaN which they do not see has turned to NaN.
+template <int D>
+__device__ __forceinline__ void exact_row(const PagedAttnArgs& a, float scale_log2, uint32_t req, int32_t pos,
+                                          uint32_t token, uint32_t kvh, uint32_t head, uint32_t dim0, uint32_t dims) {
+    constexpr int DPL = D / 64;
+    const uint32_t lane = threadIdx.x & 63, page_shift = 31 - __builtin_clz(a.head.page_size);
+    const uint32_t window = a.head.window, sinks = window ? a.head.sinks : 0;
+    const uint32_t low = window && pos >= 0 && (uint32_t)pos + 1 > window ? (uint32_t)pos + 1 - window : 0;
+    const uint32_t* const table = a.block_tables + (uint64_t)req * a.head.max_blocks;
+    const uint16_t* const q = a.q + ((uint64_t)token * a.head.hq + head) * D;
+    auto row_at = [&](const uint16_t* cache, uint32_t key) {
+        const uint32_t page = min(table[key >> page_shift], a.num_pages - 1);
+        return cache + page * a.page_stride + ((uint64_t)(key & (a.head.page_size - 1)) * a.head.hkv + kvh) * D;
+    };
+    float m = -INFINITY, l = 0.0f, acc[DPL];
+#pragma unroll
+    for (int e = 0; e < DPL; ++e) acc[e] = 0.0f;
+    for (int32_t k0 = 0; k0 <= pos; k0 += 64) {
+        const uint32_t key = k0 + lane;
+        const bool seen = (int32_t)key <= pos && (key >= low || key < sinks);
+        const uint64_t mask = __ballot(seen);
+        if (!mask) continue;
+        float sc = -INFINITY;
+        if (seen) {
+            const uint16_t* const k = row_at(a.k_cache, key);
+            float dot = 0.0f;
+#pragma unroll 1
+            for (int i = 0; i < D; ++i) dot = fmaf(bf16_to_f32(q[i]), bf16_to_f32(k[i]), dot);
+            sc = dot * scale_log2;
+        }
+        float mx = sc;
+#pragma unroll
+        for (int b = 32; b >= 1; b >>= 1) mx = fmaxf(mx, __shfl_xor(mx, b));
+        if (mx > m) {
+            const float alpha = __builtin_amdgcn_exp2f(m - mx);
+            l *= alpha;
+#pragma unroll
+            for (int e = 0; e < DPL; ++e) acc[e] *= alpha;
+            m = mx;
+        }
+        const float p = seen ? __builtin_amdgcn_exp2f(sc - (m == -INFINITY ? 0.0f : m)) : 0.0f;
+        for (uint64_t left = mask; left; left &= left - 1) {
+            const int j = __builtin_ctzll(left);
+            const float pj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), j));
+            const uint16_t* const v = row_at(a.v_cache, k0 + j);
+            l += pj;
+#pragma unroll
+            for (int e = 0; e < DPL; ++e) acc[e] = fmaf(pj, bf16_to_f32(v[DPL * lane + e]), acc[e]);
+        }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < DPL; ++e) {
+        const uint32_t d = DPL * lane + e;
+        if (d >= dim0 && d < dim0 + dims) a.o[((uint64_t)token * a.head.hq + head) * D + d] = f32_to_bf16(acc[e] * inv);
     }
 }
 
@@ -706,22 +1144,25 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_attn_kernel(PagedAttnArgs
 // of one row block, its waves every fourth piece, and the four partial merges
 // meet in LDS.
 constexpr uint32_t kMergeWgs = 512;
+constexpr int kMergeThreads = 256;
 
 template <int D>
-__global__ __launch_bounds__(kPaThreads) void paged_merge_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedAttnArgs a, float scale_log2) {
     constexpr int DBLK = D / 32, NF = PaShape<D>::NF, U = 4;
     __shared__ float4 s_o[4][4][64];
     __shared__ float2 s_ml[4][64];
-    if (!plan_fits(a.head, a.plan)) return;
-    const uint32_t* plan = static_cast<const uint32_t*>(a.plan);
-    const uint32_t hkv = a.head.hkv, group = a.head.hq / hkv, blocks = scalar_load(plan + 12);
+    const PlanHead head = plan_load<PlanHead>(a.plan, 0);
+    if (!head.fits(a.head)) return;
+    const uint32_t hkv = a.head.hkv, group = a.head.hq / hkv, blocks = head.split_blocks;
+    const bool again = scalar_load(a.flags) != 0;
+    // The tickets back to zero, for the next call.
+    for (uint32_t i = blockIdx.x * kMergeThreads + threadIdx.x; i < hkv; i += gridDim.x * kMergeThreads) a.tickets[i] = 0;
     const PagedPlanLayout lay = paged_plan_layout(a.head.batch, a.head.num_tokens, a.head.hq, hkv);
-    const PagedSplitBlock* split =
-        reinterpret_cast<const PagedSplitBlock*>(static_cast<const char*>(a.plan) + lay.split_blocks);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (uint32_t i = blockIdx.x; i < blocks * hkv * DBLK; i += gridDim.x) {
         const uint32_t db = i % DBLK, kvh = i / DBLK % hkv;
-        const PagedSplitBlock sb = split[i / (DBLK * hkv)];
+        const PagedSplitBlock sb =
+            plan_load<PagedSplitBlock>(a.plan, lay.split_blocks + (uint64_t)(i / (DBLK * hkv)) * sizeof(PagedSplitBlock));
         const uint64_t b0 = (uint64_t)kvh * paged_partial_blocks(hkv) + sb.first;
         const bool has = (uint32_t)(lane & 31) < sb.rows;
         float M = -INFINITY, den = 0.0f;
@@ -779,22 +1220,57 @@ __global__ __launch_bounds__(kPaThreads) void paged_merge_kernel(PagedAttnArgs a
             x.z = fmaf(w[k], y.z, x.z);
             x.w = fmaf(w[k], y.w, x.w);
         }
+        const float inv = tot == 0.0f ? 0.0f : 1.0f / tot;
         if (has) {
-            const uint32_t r = sb.row0 + (lane & 31), token = sb.token0 + r / group, head = kvh * group + r % group;
-            const float inv = tot == 0.0f ? 0.0f : 1.0f / tot;
-            uint16_t* o = a.o + ((uint64_t)token * a.head.hq + head) * D + 32 * db + 8 * wave + 4 * (lane >> 5);
+            const uint32_t r = sb.row0 + (lane & 31), token = sb.token0 + r / group, h = kvh * group + r % group;
+            uint16_t* o = a.o + ((uint64_t)token * a.head.hq + h) * D + 32 * db + 8 * wave + 4 * (lane >> 5);
             *reinterpret_cast<uint2*>(o) =
                 make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
         }
+        if (again) {
+            // This wave's eight dims of the rows that came out as NaN.
+            const float sum = (x.x + x.y + x.z + x.w) * inv;  // (NaN for opposite infinities too: no harm)
+            uint64_t rows = __ballot(has && sum != sum);
+            rows = (rows | rows >> 32) & 0xffffffffull;
+            for (; rows; rows &= rows - 1) {
+                const uint32_t r = sb.row0 + __builtin_ctzll(rows), token = sb.token0 + r / group;
+                exact_row<D>(a, scale_log2, sb.req, sb.pos0 + (int32_t)(r / group), token, kvh, kvh * group + r % group,
+                             32 * db + 8 * wave, 8);
+            }
+        }
+    }
+    if (!again) return;
+    // The rows of whole units that hold NaN.
+    const uint32_t waves = gridDim.x * (kMergeThreads / 64);
+    for (uint32_t i = blockIdx.x * (kMergeThreads / 64) + wave; i < head.units * hkv; i += waves) {
+        const PagedItem u = plan_load<PagedItem>(a.plan, lay.units + (uint64_t)(i / hkv) * sizeof(PagedItem));
+        const uint32_t kvh = i % hkv;
+        if (u.partial != kPagedWhole) continue;
+        for (uint32_t row = 0; row < u.rows; ++row) {
+            const uint32_t r = u.row0 + row, token = u.token0 + r / group, h = kvh * group + r % group;
+            const uint16_t* o = a.o + ((uint64_t)token * a.head.hq + h) * D + D / 64 * lane;
+            bool bad = false;
+#pragma unroll
+            for (int e = 0; e < D / 64; ++e) bad |= (o[e] & 0x7fffu) > 0x7f80u;
+            if (__any(bad))
+                exact_row<D>(a, scale_log2, u.req, u.pos0 + (int32_t)(r / group), token, kvh, h, 0, D);
+        }
+    }
+    // The flag back to zero, by the last workgroup to come here (flags[1] counts).
+    __syncthreads();
+    if (threadIdx.x == 0 && atomicAdd(a.flags + 1, 1u) == gridDim.x - 1) {
+        a.flags[0] = 0;
+        a.flags[1] = 0;
     }
 }
 
 template <int D>
 hipError_t launch_attn_t(const PagedAttnArgs& a, hipStream_t st) {
     const uint32_t wgs = a.head.hkv * paged_lanes(a.head.hkv);
-    hipLaunchKernelGGL((paged_attn_kernel<D>), dim3(wgs), dim3(kPaThreads), 0, st, a, kLog2e / sqrtf((float)D));
+    const float scale_log2 = kLog2e / sqrtf((float)D);
+    hipLaunchKernelGGL((paged_attn_kernel<D>), dim3(wgs), dim3(kPaThreads), 0, st, a, scale_log2);
     if (hipError_t e = hipGetLastError()) return e;
-    hipLaunchKernelGGL((paged_merge_kernel<D>), dim3(kMergeWgs), dim3(kPaThreads), 0, st, a);
+    hipLaunchKernelGGL((paged_merge_kernel<D>), dim3(kMergeWgs), dim3(kMergeThreads), 0, st, a, scale_log2);
     return hipGetLastError();
 }
 

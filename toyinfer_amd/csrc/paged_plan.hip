@@ -2,20 +2,26 @@
 // attention of every layer.
 //
 // One workgroup.  A request of n new tokens has n * group rows per KV head;
-// they are cut into units of up to 32, 64 or 128 rows that walk the request's
+// they are cut into units of up to 32, 64, 128 or 256 rows that walk the request's
 // key tiles together.  Larger units read each key tile for more rows, smaller
 // ones spread better: the size is the largest that gives every lane (a
 // workgroup of the attention kernel) two units, or, for fewer rows than that,
-// the largest whose tiles, split over all lanes, still make a walk of
-// kWalkTiles each.  A unit that costs more than `cap` is split over its key
-// tiles into items with partial results.  `cap` is the candidate with the
-// least estimated time: the rounds of items per lane times the longest, against
-// the even share plus the longest.  The items are ordered by cost, longest
-// first, and lane l takes items l, 2N-1-l, 2N+l, ... of N lanes.
+// the largest whose tiles, spread over all lanes, still make a walk of
+// kWalkTiles each.  The lanes draw lists of items as they come free, for their
+// speeds differ: of two workgroups of a compute unit the older is served first
+// (64 requests of 4096 keys, one equal share per lane: 130 and 160 us), and
+// the dies reach memory unequally.  Either
+// * a list is a whole unit, longest first, or
+// * the units' tiles laid end to end are cut into ranges, of half a lane's even
+//   share first, then a quarter, then an eighth.  A unit with a cut inside
+//   leaves partial results of each piece, merged by a second kernel.
+// The estimate of whichever is shorter decides: rounds of whole units times
+// their mean, or the longest of them, against the even share plus the pieces'
+// overhead.
 //
-// Costs are in quarters of the time in which one lane runs a 64-key tile of 32
-// rows out of the cache: the products of 32 rows take 4, and the tile's bytes
-// from HBM kHbmCost, shared by the units of the request that read them.
+// Costs are in units of about 0.12 us of a lane: a 64-key tile takes kRowCost
+// per 32 rows of products, or kHbmCost for its bytes from HBM, shared by the
+// units of the request that read them.
 #include "common.hpp"
 #include "paged.hpp"
 
@@ -24,41 +30,34 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
-constexpr uint32_t kHbmCost = 16;
-constexpr uint32_t kItemCost = 16;   // starting and merging an item
+constexpr uint32_t kRowCost = 2, kHbmCost = 11;
+constexpr uint32_t kItemCost = 24;  // starting and finishing an item
 constexpr uint32_t kWalkTiles = 8;
-constexpr int kCaps = 32;
-// Candidates for `cap` over the even share per lane, the last unbounded.  At
-// least half of it, which bounds the partial results (paged_partial_blocks).
-__device__ const float kCapOver[kCaps] = {1.0f,  1.02f, 1.04f, 1.06f, 1.08f, 1.1f,  1.13f, 1.16f,
-                                          1.2f,  1.25f, 1.3f,  1.35f, 1.4f,  1.5f,  1.6f,  1.75f,
-                                          1.9f,  2.0f,  2.2f,  2.5f,  2.75f, 3.0f,  3.5f,  4.0f,
-                                          5.0f,  6.0f,  8.0f,  10.0f, 12.0f, 16.0f, 32.0f, 3.0e38f};
+constexpr uint32_t kPieceTiles = 2;  // cuts lie on multiples of it, one 32-key half per wave
+constexpr uint32_t kLocalUnits = 2048;
+constexpr uint32_t kSizes = 4;         // 32, 64, 128 or 256 rows per unit
+constexpr uint32_t kLevelShare = 800;  // a lane's share from which its ranges shrink by level
 
 __device__ __forceinline__ uint64_t wave_sum64(uint64_t x) {
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) x += __shfl_xor(x, m);
     return x;
 }
-__device__ __forceinline__ uint32_t wave_max32(uint32_t x) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) x = max(x, (uint32_t)__shfl_xor(x, m));
-    return x;
-}
 
-// Exclusive sum over the workgroup's threads in thread order, total in *sum.
-__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* sum) {
-    __shared__ uint32_t s_tot[kPlanWaves];
+// Exclusive sums over the workgroup's threads in thread order, total in *sum.
+template <typename T>
+__device__ __forceinline__ T block_scan(T x, T* sum) {
+    __shared__ T s_tot[kPlanWaves];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t inc = x;
+    T inc = x;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
-        const uint32_t u = __shfl_up(inc, m);
+        const T u = __shfl_up(inc, m);
         if (lane >= m) inc += u;
     }
     if (lane == 63) s_tot[wave] = inc;
     __syncthreads();
-    uint32_t before = 0, all = 0;
+    T before = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < kPlanWaves; ++w) {
         before += w < wave ? s_tot[w] : 0;
@@ -69,37 +68,28 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* sum) {
     return before + inc - x;
 }
 
-__device__ __forceinline__ uint64_t block_sum64(uint64_t x) {
-    __shared__ uint64_t s_tot[kPlanWaves];
-    x = wave_sum64(x);
-    if ((threadIdx.x & 63) == 0) s_tot[threadIdx.x >> 6] = x;
-    __syncthreads();
-    uint64_t r = 0;
-#pragma unroll
-    for (int w = 0; w < kPlanWaves; ++w) r += s_tot[w];
-    __syncthreads();
-    return r;
+// Index of the last entry <= x of ascending a[0..n), a[0] <= x.
+template <typename T>
+__device__ __forceinline__ uint32_t last_at_most(const T* a, uint32_t n, T x) {
+    uint32_t lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (a[mid] <= x)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
 }
 
-__device__ __forceinline__ uint32_t unit_rows_for(uint32_t rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+__device__ __forceinline__ uint32_t unit_rows_for(uint32_t rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
 
 struct Request {
     uint32_t token0, n, len;
 };
-// Lengths as the kernels may use them whatever the arrays hold: tokens inside
-// q, keys inside the block table.
-__device__ __forceinline__ Request request(const PagedPlanArgs& a, uint32_t b) {
-    Request r;
-    const uint32_t s = min(a.query_start[b], a.head.num_tokens), e = min(a.query_start[b + 1], a.head.num_tokens);
-    const uint64_t room = (uint64_t)a.head.max_blocks * a.head.page_size;
-    r.token0 = s;
-    r.n = e > s ? e - s : 0;
-    r.len = (uint32_t)min((uint64_t)a.seq_lens[b], room);
-    return r;
-}
 
-// The key tiles that rows [row0, row0 + rows) see (tile_end = their number).
-__device__ __forceinline__ PagedItem unit_of(const PagedPlanArgs& a, uint32_t b, const Request& r, uint32_t group,
+// The key tiles that rows [row0, row0 + rows) of request b see.
+__device__ __forceinline__ PagedItem unit_of(const PagedPlanHeader& h, uint32_t b, const Request& r, uint32_t group,
                                              uint32_t row0, uint32_t rows) {
     PagedItem u;
     u.req = b;
@@ -110,231 +100,271 @@ __device__ __forceinline__ PagedItem unit_of(const PagedPlanArgs& a, uint32_t b,
     const int32_t first = u.pos0 + (int32_t)(row0 / group), last = u.pos0 + (int32_t)((row0 + rows - 1) / group);
     u.key_end = last < 0 ? 0 : (uint32_t)last + 1;
     uint32_t low = 0;
-    if (a.head.window && first >= 0 && (uint32_t)first + 1 > a.head.window) low = (uint32_t)first + 1 - a.head.window;
+    if (h.window && first >= 0 && (uint32_t)first + 1 > h.window) low = (uint32_t)first + 1 - h.window;
     u.low_tile = low / kPagedTile;
-    const uint32_t sink_tiles = (uint32_t)(((uint64_t)a.head.sinks + kPagedTile - 1) / kPagedTile);
-    u.sink_tiles = a.head.window ? min(sink_tiles, u.low_tile) : 0;
+    const uint32_t sink_tiles = (uint32_t)(((uint64_t)h.sinks + kPagedTile - 1) / kPagedTile);
+    u.sink_tiles = h.window ? min(sink_tiles, u.low_tile) : 0;
     u.tile_begin = 0;
     u.tile_end = u.key_end ? (u.key_end - 1) / kPagedTile + 1 - u.low_tile + u.sink_tiles : 0;
     u.partial = kPagedWhole;
-    u.pad = 0;
+    u.next = kPagedNone;
     return u;
 }
 
 __device__ __forceinline__ uint32_t tile_cost(uint32_t rows, uint32_t units) {
-    const uint32_t compute = rows <= 32 ? 4 : rows <= 64 ? 8 : 16;
-    return max(compute, kHbmCost / units);
+    return max(unit_rows_for(rows) / 32 * kRowCost, kHbmCost / units);
 }
 
-// Pieces of a unit of `tiles` tiles and cost `cost` under `cap`.  Units of up
-// to 32 rows are split in pairs of tiles, one 32-key half per wave.
-__device__ __forceinline__ uint32_t pieces_of(uint32_t cost, uint32_t tiles, uint32_t rows, float inv_cap) {
-    const uint32_t most = rows <= 32 ? (tiles + 1) / 2 : tiles;
-    const float want = ceilf((float)cost * inv_cap - 1e-3f);
-    return want <= 1.0f ? 1 : min((uint32_t)fminf(want, 65536.0f), max(most, 1u));
+// Sizes of the ranges of level v of `levels`, in parts of a lane's share.
+constexpr uint32_t kParts = 16;
+__device__ __forceinline__ uint32_t level_parts(uint32_t v, uint32_t levels) {
+    return levels == 1 ? kParts : levels == 2 ? (v ? 2 : 14) : levels == 3 ? (v ? 1 : 14) : v == 0 ? 12 : v == 1 ? 2 : 1;
 }
 
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs a) {
-    constexpr uint32_t kBuckets = 1024;
-    __shared__ uint32_t s_first[kPagedMaxBatch + 1];  // first unit of each request
+    constexpr uint32_t kBuckets = kPlanThreads;
+    __shared__ Request s_req[kPagedMaxBatch];
+    __shared__ uint32_t s_first[kPagedMaxBatch + 1];   // first unit of each request
+    __shared__ uint64_t s_cost[kLocalUnits + 1];       // cost of the units before each
+    __shared__ uint32_t s_cut_unit[kPagedLevels * kPagedSlots + 1], s_cut_tile[kPagedLevels * kPagedSlots + 1];
+    __shared__ uint32_t s_item[kPagedLevels * kPagedSlots + 1];  // first item of each range
     __shared__ uint32_t s_bucket[kBuckets];
-    __shared__ float s_est[kCaps];
-    __shared__ uint32_t s_pick;
-    const uint32_t tid = threadIdx.x, batch = a.head.batch, hkv = a.head.hkv, group = a.head.hq / hkv;
+    __shared__ uint64_t s_sum[kPlanWaves][2 * kSizes + 1];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t batch = a.head.batch, hkv = a.head.hkv, group = a.head.hq / hkv;
     const uint32_t lanes = paged_lanes(hkv), max_units = paged_max_units(batch, a.head.num_tokens, group);
     const PagedPlanLayout lay = paged_plan_layout(batch, a.head.num_tokens, a.head.hq, hkv);
     char* const base = static_cast<char*>(a.plan);
     PagedItem* const items = reinterpret_cast<PagedItem*>(base + lay.items);
     PagedItem* const units = reinterpret_cast<PagedItem*>(base + lay.units);
     PagedSplitBlock* const split = reinterpret_cast<PagedSplitBlock*>(base + lay.split_blocks);
-    uint32_t* const costs = reinterpret_cast<uint32_t*>(base + lay.costs);
-    uint32_t* const offsets = costs + max_units + 1;
 
-    // Rows per unit.
-    uint64_t n_units[3] = {0, 0, 0}, n_tiles[3] = {0, 0, 0};
+    // Lengths as the kernels may use them whatever the arrays hold: tokens
+    // inside q, keys inside the block table.  Sums for the rows per unit.
+    uint64_t sums[2 * kSizes + 1] = {};  // units and tiles at each size; the sizes that a request fills
+    const uint32_t room = (uint32_t)min((uint64_t)a.head.max_blocks * a.head.page_size, (uint64_t)0x7fffffffu);
     for (uint32_t b = tid; b < batch; b += kPlanThreads) {
-        const Request r = request(a, b);
+        const uint32_t s = min(a.query_start[b], a.head.num_tokens), e = min(a.query_start[b + 1], a.head.num_tokens);
+        Request r;
+        r.token0 = s;
+        r.n = e > s ? e - s : 0;
+        r.len = min(a.seq_lens[b], room);
+        s_req[b] = r;
         const uint32_t rows = r.n * group;
         if (!rows) continue;
-        // The tiles that the request's middle rows see.
-        const PagedItem mid = unit_of(a, b, r, group, rows / 2, 1);
+        // The tiles that the request's middle row sees.
+        const uint32_t tiles = unit_of(a.head, b, r, group, rows / 2, 1).tile_end;
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            const uint32_t R = min(32u << i, unit_rows_for(rows));
-            n_units[i] += (rows + R - 1) / R;
-            n_tiles[i] += (uint64_t)((rows + R - 1) / R) * mid.tile_end;
+        for (int i = 0; i < (int)kSizes; ++i) {
+            const uint32_t R = min(32u << i, unit_rows_for(rows)), n = (rows + R - 1) / R;
+            sums[i] += n;
+            sums[kSizes + i] += (uint64_t)n * tiles;
         }
+        sums[2 * kSizes] |= unit_rows_for(rows);
     }
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        n_units[i] = block_sum64(n_units[i]);
-        n_tiles[i] = block_sum64(n_tiles[i]);
+    for (int i = 0; i < 2 * (int)kSizes; ++i) sums[i] = wave_sum64(sums[i]);
+    {
+        const uint64_t fills = sums[2 * kSizes];
+        sums[2 * kSizes] = __any(fills & 256) ? 256 : __any(fills & 128) ? 128 : __any(fills & 64) ? 64 : 32;
     }
-    uint32_t unit_rows = 32;
-    if (n_units[2] >= 2 * lanes) unit_rows = 128;
-    else if (n_units[1] >= 2 * lanes) unit_rows = 64;
-    else if (n_units[0] >= 2 * lanes) unit_rows = 32;
-    else if (n_tiles[2] >= (uint64_t)kWalkTiles * lanes) unit_rows = 128;
-    else if (n_tiles[1] >= (uint64_t)kWalkTiles * lanes) unit_rows = 64;
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i <= 2 * (int)kSizes; ++i) s_sum[wave][i] = sums[i];
+    }
+    s_bucket[tid] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2 * (int)kSizes; ++i) {
+        sums[i] = 0;
+#pragma unroll
+        for (int w = 0; w < kPlanWaves; ++w) sums[i] += s_sum[w][i];
+    }
+    uint32_t most_rows = 32;
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) most_rows = max(most_rows, (uint32_t)s_sum[w][2 * kSizes]);
+    uint32_t unit_rows = 0;
+#pragma unroll
+    for (int i = kSizes - 1; i >= 0; --i)
+        if (!unit_rows && sums[i] >= 2 * lanes) unit_rows = 32u << i;
+#pragma unroll
+    for (int i = kSizes - 1; i >= 0; --i)
+        if (!unit_rows && sums[kSizes + i] >= (uint64_t)kWalkTiles * lanes) unit_rows = 32u << i;
+    unit_rows = min(unit_rows ? unit_rows : 32u, most_rows);
 
-    // The units.
+    // The units.  Their bound holds for any ascending query_start; the clamp
+    // also keeps the units of an array that is none inside the plan.
     uint32_t U = 0;
     for (uint32_t b0 = 0; b0 < batch; b0 += kPlanThreads) {
         const uint32_t b = b0 + tid;
         uint32_t n = 0, sum;
         if (b < batch) {
-            const uint32_t rows = request(a, b).n * group, R = min(unit_rows, unit_rows_for(rows));
+            const uint32_t rows = s_req[b].n * group, R = min(unit_rows, unit_rows_for(rows));
             n = (rows + R - 1) / R;
         }
-        // The bound holds for any ascending query_start; it also keeps units
-        // of an array that is none inside the plan.
         const uint32_t at = block_scan(n, &sum);
         if (b < batch) s_first[b] = min(U + at, max_units);
         U = min(U + sum, max_units);
     }
     if (tid == 0) s_first[batch] = U;
     __syncthreads();
-    uint64_t my_cost = 0;
-    uint32_t my_max = 0;
-    for (uint32_t i = tid; i < U; i += kPlanThreads) {
-        uint32_t lo = 0, hi = batch;  // s_first[lo] <= i < s_first[hi]
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (s_first[mid] <= i)
-                lo = mid;
-            else
-                hi = mid;
-        }
-        const Request r = request(a, lo);
-        const uint32_t rows = r.n * group, R = min(unit_rows, unit_rows_for(rows)), row0 = (i - s_first[lo]) * R;
-        const PagedItem u = unit_of(a, lo, r, group, row0, min(R, rows - row0));
-        const uint32_t cost = u.tile_end * tile_cost(u.rows, s_first[lo + 1] - s_first[lo]) + kItemCost;
-        units[i] = u;
-        costs[i] = cost;
-        my_cost += cost;
-        my_max = max(my_max, cost);
-    }
-    const uint64_t work = block_sum64(my_cost);  // (also orders units and costs)
-    const float share = (float)work / lanes;
-
-    // Each wave estimates two candidates for the cap.
-    const int lane = tid & 63, wave = tid >> 6;
-    for (int k = wave; k < kCaps; k += kPlanWaves) {
-        const float inv_cap = kCapOver[k] > 1.0e30f ? 0.0f : 1.0f / (kCapOver[k] * share);
-        uint64_t n = 0;
-        uint32_t longest = 0;
-        for (uint32_t i = lane; i < U; i += 64) {
-            const uint32_t tiles = units[i].tile_end, p = pieces_of(costs[i], tiles, units[i].rows, inv_cap);
-            n += p;
-            longest = max(longest, (costs[i] - kItemCost) / p + (p > 1 ? 1 : 0) + kItemCost);
-        }
-        n = wave_sum64(n);
-        longest = wave_max32(longest);
-        const float rounds = ceilf((float)n / lanes);
-        const float even = share + (float)(n - U) * kItemCost / lanes + (float)longest;
-        if (lane == 0) s_est[k] = fminf(rounds * longest, even);
-    }
-    __syncthreads();
-    if (tid == 0) {
-        uint32_t best = kCaps - 1;
-        for (int k = kCaps - 2; k >= 0; --k)
-            if (s_est[k] < s_est[best]) best = k;
-        s_pick = best;
-    }
-    for (uint32_t i = tid; i < kBuckets; i += kPlanThreads) s_bucket[i] = 0;
-    __syncthreads();
-    const uint32_t pick = s_pick;
-    const float inv_cap = kCapOver[pick] > 1.0e30f ? 0.0f : 1.0f / (kCapOver[pick] * share);
-
-    // Items and partial blocks of each unit: offsets[i] = first item, and the
-    // unit's `partial` = its first partial block.
-    uint32_t N = 0, blocks = 0, split_blocks = 0;
-    uint32_t longest = 0;
+    uint64_t* const cost = U <= kLocalUnits ? s_cost : reinterpret_cast<uint64_t*>(base + lay.costs);
+    uint64_t work = 0, longest = 0;
     for (uint32_t i0 = 0; i0 < U; i0 += kPlanThreads) {
         const uint32_t i = i0 + tid;
-        uint32_t p = 0, nb = 0, sum;
-        PagedItem u{};
+        uint64_t c = 0, sum;
         if (i < U) {
-            u = units[i];
-            p = pieces_of(costs[i], u.tile_end, u.rows, inv_cap);
-            nb = (u.rows + kPagedBlockRows - 1) / kPagedBlockRows;
-            longest = max(longest, costs[i] / p);
+            const uint32_t b = last_at_most(s_first, batch, i);
+            const Request r = s_req[b];
+            const uint32_t rows = r.n * group, R = min(unit_rows, unit_rows_for(rows)), row0 = (i - s_first[b]) * R;
+            PagedItem u = unit_of(a.head, b, r, group, row0, min(R, rows - row0));
+            const uint32_t per_tile = tile_cost(u.rows, s_first[b + 1] - s_first[b]);
+            u.next = per_tile;  // (here; the items' own below)
+            units[i] = u;
+            c = (uint64_t)u.tile_end * per_tile + kItemCost;
+            longest = max(longest, c);
         }
-        const uint32_t at = block_scan(p, &sum);
-        if (i < U) offsets[i] = N + at;
-        N += sum;
-        const uint32_t pb = block_scan(p > 1 ? p * nb : 0, &sum), first = blocks + pb;
-        blocks += sum;
-        const uint32_t sb = block_scan(p > 1 ? nb : 0, &sum);
-        if (p > 1) {
-            units[i].partial = first;
-            for (uint32_t k = 0; k < nb; ++k) {
-                PagedSplitBlock s{};
-                s.token0 = u.token0;
-                s.row0 = u.row0 + k * kPagedBlockRows;
-                s.rows = min(kPagedBlockRows, u.rows - k * kPagedBlockRows);
-                s.first = first + k;
-                s.stride = nb;
-                s.pieces = p;
-                split[split_blocks + sb + k] = s;
-            }
-        }
-        split_blocks += sum;
+        const uint64_t at = block_scan(c, &sum);
+        if (i < U) cost[i] = work + at;
+        work += sum;
     }
-    __shared__ uint32_t s_max[kPlanWaves];
-    longest = wave_max32(longest);
-    if (lane == 0) s_max[wave] = longest;
-    if (tid == 0) offsets[U] = N;
+    if (tid == 0) cost[U] = work;
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) longest = max(longest, (uint64_t)__shfl_xor(longest, m));
+    if (lane == 0) s_sum[wave][0] = longest;
     __syncthreads();
-    longest = 1;
-    for (int w = 0; w < kPlanWaves; ++w) longest = max(longest, s_max[w]);
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) longest = max(longest, s_sum[w][0]);
 
-    // The items, longest first (by cost buckets; order within a bucket decides
-    // only which lane runs an item, never a result).
-    const float to_bucket = (float)(kBuckets - 1) / (float)longest;
-    for (int pass = 0; pass < 2; ++pass) {
-        for (uint32_t i = tid; i < N; i += kPlanThreads) {
-            uint32_t lo = 0, hi = U;
-            while (hi - lo > 1) {
-                const uint32_t mid = (lo + hi) / 2;
-                if (offsets[mid] <= i)
-                    lo = mid;
-                else
-                    hi = mid;
-            }
-            const uint32_t p = offsets[lo + 1] - offsets[lo], k = i - offsets[lo];
-            const uint32_t bucket = kBuckets - 1 - min(kBuckets - 1, (uint32_t)((float)(costs[lo] / p) * to_bucket));
-            if (pass == 0) {
-                atomicAdd(&s_bucket[bucket], 1u);
-            } else {
-                PagedItem u = units[lo];
-                if (p > 1) {
-                    const uint32_t nb = (u.rows + kPagedBlockRows - 1) / kPagedBlockRows;
-                    const uint32_t quantum = u.rows <= 32 ? 2 : 1, q = (u.tile_end + quantum - 1) / quantum;
-                    const uint32_t tiles = u.tile_end;
-                    u.tile_begin = quantum * (uint32_t)((uint64_t)q * k / p);
-                    u.tile_end = min(tiles, quantum * (uint32_t)((uint64_t)q * (k + 1) / p));
-                    u.partial += k * nb;
+    const uint64_t share = work / lanes;
+    const uint32_t levels = share >= kLevelShare ? min(kPagedLevels, kPagedMaxRows / unit_rows) : 1;
+    const uint64_t rounds = U ? (uint64_t)((U + lanes - 1) / lanes) * work / U : 0;
+    const uint64_t whole = max(longest, rounds) + (unit_rows == 32 ? longest / 4 : 0);
+    const uint64_t cut = share + kItemCost * levels + 8 + unit_rows / 2;  // and the pieces' results
+    uint32_t n_items = U, split_blocks = 0, ranges = max(U, lanes);
+    if (whole <= cut) {
+        // Whole units, longest first (by cost buckets; the order within one
+        // decides only which lane runs a unit, never a result).
+        const float to_bucket = (float)(kBuckets - 1) / (float)max(longest, (uint64_t)1);
+        for (int pass = 0; pass < 2; ++pass) {
+            for (uint32_t i = tid; i < U; i += kPlanThreads) {
+                const uint32_t q = (uint32_t)((float)(cost[i + 1] - cost[i]) * to_bucket);
+                const uint32_t bucket = kBuckets - 1 - min(kBuckets - 1, q), at = atomicAdd(&s_bucket[bucket], 1u);
+                if (pass == 1) {
+                    PagedItem u = units[i];
+                    u.next = kPagedNone;
+                    items[at] = u;
                 }
-                items[atomicAdd(&s_bucket[bucket], 1u)] = u;
             }
+            __syncthreads();
+            if (pass == 0) {
+                uint32_t sum;
+                const uint32_t at = block_scan(s_bucket[tid], &sum);
+                s_bucket[tid] = at;
+                __syncthreads();
+            }
+        }
+        if (tid < lanes && tid >= U) items[tid].rows = 0;
+    } else {
+        // Cut r: the start of range r, its unit and the tile in it.  Ranges of
+        // level v, one per lane, are 1/2, 1/4, ... of the share, the last two
+        // levels alike.
+        ranges = levels * lanes;
+        for (uint32_t r = tid; r <= ranges; r += kPlanThreads) {
+            const uint32_t level = r / lanes, nth = r % lanes;
+            const uint32_t size = levels == 1 ? kParts : level_parts(level, levels);
+            uint32_t before = level >= levels ? kParts : 0;
+            for (uint32_t v = 0; v < level && level < levels; ++v) before += level_parts(v, levels);
+            const uint64_t x = work * ((uint64_t)before * lanes + (uint64_t)size * nth) / ((uint64_t)kParts * lanes);
+            uint32_t i = r == ranges ? U : last_at_most(cost, U, x), t = 0;
+            if (i < U) {
+                const uint32_t tiles = units[i].tile_end, per_tile = units[i].next;
+                const uint64_t off = x - cost[i];
+                if (off > kItemCost)
+                    t = (uint32_t)((off - kItemCost + per_tile * kPieceTiles / 2) / (per_tile * kPieceTiles)) * kPieceTiles;
+                if (t + kPieceTiles > tiles && t > 0) {
+                    t = 0;
+                    ++i;
+                }
+            }
+            s_cut_unit[r] = i;
+            s_cut_tile[r] = t;
         }
         __syncthreads();
-        if (pass == 0) {
-            uint32_t sum;
-            const uint32_t c = s_bucket[tid];
-            const uint32_t at = block_scan(c, &sum);
-            s_bucket[tid] = at;
-            __syncthreads();
+        n_items = 0;
+        for (uint32_t r0 = 0; r0 < ranges; r0 += kPlanThreads) {
+            const uint32_t r = r0 + tid;
+            uint32_t n = 0, sum;
+            if (r < ranges) {
+                const uint32_t u0 = s_cut_unit[r], u1 = s_cut_unit[r + 1];
+                n = u1 - u0 + (s_cut_tile[r + 1] > (u0 == u1 ? s_cut_tile[r] : 0));
+                if (n == 0) items[r].rows = 0;
+            }
+            const uint32_t at = block_scan(n, &sum);
+            if (r < ranges) s_item[r] = n_items + at;
+            n_items += sum;
+        }
+        if (tid == 0) s_item[ranges] = n_items;
+        __syncthreads();
+        uint32_t blocks = 0;
+        for (uint32_t j0 = 0; j0 < n_items; j0 += kPlanThreads) {
+            const uint32_t j = j0 + tid;
+            uint32_t r = 0, i = 0, nb = 0, sum;
+            PagedItem u{};
+            if (j < n_items) {
+                r = last_at_most(s_item, ranges, j);
+                i = s_cut_unit[r] + (j - s_item[r]);
+                u = units[i];
+                const uint32_t tiles = u.tile_end;
+                if (j == s_item[r]) u.tile_begin = s_cut_tile[r];
+                if (i == s_cut_unit[r + 1]) u.tile_end = s_cut_tile[r + 1];
+                if (u.tile_begin > 0 || u.tile_end < tiles) nb = (u.rows + kPagedBlockRows - 1) / kPagedBlockRows;
+                u.next = j + 1 < s_item[r + 1] ? ranges + j + 1 : kPagedNone;
+            }
+            const bool opens = nb && u.tile_begin == 0;
+            const uint32_t first = blocks + block_scan(nb, &sum);
+            blocks += sum;
+            const uint32_t sb = split_blocks + block_scan(opens ? nb : 0u, &sum);
+            split_blocks += sum;
+            if (j < n_items) {
+                if (nb) u.partial = first;
+                items[j == s_item[r] ? r : ranges + j] = u;
+            }
+            if (opens) {
+                // The range of the unit's last piece: the one before the first
+                // cut past the unit.
+                uint32_t lo = r, hi = ranges;
+                while (hi - lo > 1) {
+                    const uint32_t mid = (lo + hi) / 2;
+                    if (s_cut_unit[mid] > i)
+                        hi = mid;
+                    else
+                        lo = mid;
+                }
+                units[i].partial = 0;  // (split; the pieces' own places are in the items)
+                const uint32_t pieces = s_item[lo] + (i - s_cut_unit[lo]) - j + 1;
+                for (uint32_t k = 0; k < nb; ++k) {
+                    PagedSplitBlock s{};
+                    s.token0 = u.token0;
+                    s.row0 = u.row0 + k * kPagedBlockRows;
+                    s.rows = min(kPagedBlockRows, u.rows - k * kPagedBlockRows);
+                    s.first = first + k;
+                    s.stride = nb;
+                    s.pieces = pieces;
+                    s.req = u.req;
+                    s.pos0 = u.pos0;
+                    split[sb + k] = s;
+                }
+            }
         }
     }
-    static_assert(kBuckets == kPlanThreads, "one bucket per thread in the scan");
     if (tid == 0) {
         PagedPlanHeader h = a.head;
         h.magic = kPagedMagic;
-        h.units = U;
-        h.items = N;
+        h.items = n_items;
         h.split_blocks = split_blocks;
+        h.ranges = ranges;
+        h.units = U;
         *reinterpret_cast<PagedPlanHeader*>(base) = h;
     }
 }
