@@ -4,24 +4,25 @@
 // One workgroup.  A request of n new tokens has n * group rows per KV head;
 // they are cut into units of up to 32, 64, 128 or 256 rows that walk the request's
 // key tiles together.  Larger units read each key tile for more rows, smaller
-// ones spread better: the size is the largest that gives every lane (a
-// workgroup of the attention kernel) two units, or, for fewer rows than that,
-// the largest whose tiles, spread over all lanes, still make a walk of
-// kWalkTiles each.  The lanes draw lists of items as they come free, for their
-// speeds differ: of two workgroups of a compute unit the older is served first
-// (64 requests of 4096 keys, one equal share per lane: 130 and 160 us), and
-// the dies reach memory unequally.  Either
+// ones spread better over the lanes (a lane: a workgroup of the attention
+// kernel).  The lanes draw lists of items as they come free, for their speeds
+// differ: of two workgroups of a compute unit the older is served first (64
+// requests of 4096 keys, one equal share per lane: 130 and 160 us), and the dies
+// reach memory unequally.  Either
 // * a list is a whole unit, longest first, or
-// * the units' tiles laid end to end are cut into ranges, of half a lane's even
-//   share first, then a quarter, then an eighth.  A unit with a cut inside
+// * the units' tiles laid end to end are cut into ranges, of most of a lane's
+//   even share first, then of smaller parts of it.  A unit with a cut inside
 //   leaves partial results of each piece, merged by a second kernel.
-// The estimate of whichever is shorter decides: rounds of whole units times
-// their mean, or the longest of them, against the even share plus the pieces'
-// overhead.
+// The size and the way are those with the shortest estimate: rounds of whole
+// units times their mean, or the longest of them, against the even share plus
+// the pieces' overhead.  At 32 query and 8 KV heads of 128, forced sizes of
+// 32 / 64 / 128 / 256 rows took, in us (* the choice): 512 tokens on 8192 keys
+// 201 / 92 / 89 / 84*, a prompt of 512 - / 16* / 20 / 26, of 2048 - / 76 / 66* /
+// 80, of 8192 1494 / 733 / 576 / 528*.
 //
-// Costs are in units of about 0.12 us of a lane: a 64-key tile takes kRowCost
-// per 32 rows of products, or kHbmCost for its bytes from HBM, shared by the
-// units of the request that read them.
+// Costs are in units of about 0.12 us of a lane: a 64-key tile takes its
+// products, or its bytes' time from HBM shared by the units of the request that
+// read them, whichever is longer.
 #include "common.hpp"
 #include "paged.hpp"
 
@@ -30,9 +31,7 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
-constexpr uint32_t kRowCost = 2, kHbmCost = 11;
 constexpr uint32_t kItemCost = 24;  // starting and finishing an item
-constexpr uint32_t kWalkTiles = 8;
 constexpr uint32_t kPieceTiles = 2;  // cuts lie on multiples of it, one 32-key half per wave
 constexpr uint32_t kLocalUnits = 2048;
 constexpr uint32_t kSizes = 4;         // 32, 64, 128 or 256 rows per unit
@@ -111,8 +110,26 @@ __device__ __forceinline__ PagedItem unit_of(const PagedPlanHeader& h, uint32_t 
     return u;
 }
 
-__device__ __forceinline__ uint32_t tile_cost(uint32_t rows, uint32_t units) {
-    return max(unit_rows_for(rows) / 32 * kRowCost, kHbmCost / units);
+// Of one of `units` units of a request, per tile.
+__device__ __forceinline__ uint32_t tile_cost(uint32_t rows, uint32_t units, uint32_t d) {
+    const uint32_t products = rows <= 64 ? 6 : rows <= 128 ? 9 : 17, bytes = 11;
+    return max(d == 64 ? (2 * products + 2) / 3 : products, (d == 64 ? (bytes + 1) / 2 : bytes) / units);
+}
+
+// The whole step, for U units of this total and longest cost: each as a list of
+// its own, or cut into even shares.
+struct Estimate {
+    uint64_t whole, cut;
+    uint32_t levels;
+};
+__device__ __forceinline__ Estimate estimate(uint32_t U, uint64_t work, uint64_t longest, uint32_t rows, uint32_t lanes) {
+    const uint64_t share = work / lanes;
+    Estimate e;
+    e.levels = share >= kLevelShare ? min(kPagedLevels, kPagedMaxRows / rows) : 1;
+    const uint64_t rounds = U ? (uint64_t)((U + lanes - 1) / lanes) * work / U : 0;
+    e.whole = max(longest, rounds) + (rows == 32 ? longest / 4 : 0);
+    e.cut = share + kItemCost * e.levels + 8 + rows / 2;  // and the pieces' results
+    return e;
 }
 
 // Sizes of the ranges of level v of `levels`, in parts of a lane's share.
@@ -129,7 +146,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
     __shared__ uint32_t s_cut_unit[kPagedLevels * kPagedSlots + 1], s_cut_tile[kPagedLevels * kPagedSlots + 1];
     __shared__ uint32_t s_item[kPagedLevels * kPagedSlots + 1];  // first item of each range
     __shared__ uint32_t s_bucket[kBuckets];
-    __shared__ uint64_t s_sum[kPlanWaves][2 * kSizes + 1];
+    __shared__ uint64_t s_work[kPlanWaves][kSizes];
+    __shared__ uint32_t s_units[kPlanWaves][kSizes], s_long[kPlanWaves][kSizes], s_most[kPlanWaves];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t batch = a.head.batch, hkv = a.head.hkv, group = a.head.hq / hkv;
     const uint32_t lanes = paged_lanes(hkv), max_units = paged_max_units(batch, a.head.num_tokens, group);
@@ -140,8 +158,10 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
     PagedSplitBlock* const split = reinterpret_cast<PagedSplitBlock*>(base + lay.split_blocks);
 
     // Lengths as the kernels may use them whatever the arrays hold: tokens
-    // inside q, keys inside the block table.  Sums for the rows per unit.
-    uint64_t sums[2 * kSizes + 1] = {};  // units and tiles at each size; the sizes that a request fills
+    // inside q, keys inside the block table.  For each size its units, their
+    // cost (by the request's middle unit) and the longest (by its last).
+    uint64_t work_of[kSizes] = {};
+    uint32_t units_of[kSizes] = {}, long_of[kSizes] = {}, most_rows = 32;
     const uint32_t room = (uint32_t)min((uint64_t)a.head.max_blocks * a.head.page_size, (uint64_t)0x7fffffffu);
     for (uint32_t b = tid; b < batch; b += kPlanThreads) {
         const uint32_t s = min(a.query_start[b], a.head.num_tokens), e = min(a.query_start[b + 1], a.head.num_tokens);
@@ -152,45 +172,58 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
         s_req[b] = r;
         const uint32_t rows = r.n * group;
         if (!rows) continue;
-        // The tiles that the request's middle row sees.
-        const uint32_t tiles = unit_of(a.head, b, r, group, rows / 2, 1).tile_end;
+        most_rows = max(most_rows, unit_rows_for(rows));
 #pragma unroll
         for (int i = 0; i < (int)kSizes; ++i) {
             const uint32_t R = min(32u << i, unit_rows_for(rows)), n = (rows + R - 1) / R;
-            sums[i] += n;
-            sums[kSizes + i] += (uint64_t)n * tiles;
+            const uint32_t mid = n / 2 * R, last = (n - 1) * R, per_tile = tile_cost(min(R, rows), n, a.head.d);
+            units_of[i] += n;
+            work_of[i] += (uint64_t)n * (unit_of(a.head, b, r, group, mid, min(R, rows - mid)).tile_end * per_tile + kItemCost);
+            long_of[i] = max(long_of[i], unit_of(a.head, b, r, group, last, min(R, rows - last)).tile_end * per_tile + kItemCost);
         }
-        sums[2 * kSizes] |= unit_rows_for(rows);
     }
+    if (wave * 64 < batch) {
 #pragma unroll
-    for (int i = 0; i < 2 * (int)kSizes; ++i) sums[i] = wave_sum64(sums[i]);
-    {
-        const uint64_t fills = sums[2 * kSizes];
-        sums[2 * kSizes] = __any(fills & 256) ? 256 : __any(fills & 128) ? 128 : __any(fills & 64) ? 64 : 32;
+        for (int i = 0; i < (int)kSizes; ++i) {
+            work_of[i] = wave_sum64(work_of[i]);
+#pragma unroll
+            for (int m = 32; m >= 1; m >>= 1) {
+                units_of[i] += __shfl_xor(units_of[i], m);
+                long_of[i] = max(long_of[i], (uint32_t)__shfl_xor(long_of[i], m));
+            }
+        }
+        most_rows = __any(most_rows == 256) ? 256 : __any(most_rows == 128) ? 128 : __any(most_rows == 64) ? 64 : 32;
     }
     if (lane == 0) {
 #pragma unroll
-        for (int i = 0; i <= 2 * (int)kSizes; ++i) s_sum[wave][i] = sums[i];
+        for (int i = 0; i < (int)kSizes; ++i) {
+            s_work[wave][i] = work_of[i];
+            s_units[wave][i] = units_of[i];
+            s_long[wave][i] = long_of[i];
+        }
+        s_most[wave] = most_rows;
     }
     s_bucket[tid] = 0;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 2 * (int)kSizes; ++i) {
-        sums[i] = 0;
-#pragma unroll
-        for (int w = 0; w < kPlanWaves; ++w) sums[i] += s_sum[w][i];
+    for (int w = 0; w < kPlanWaves; ++w) most_rows = max(most_rows, s_most[w]);
+    uint32_t unit_rows = 32;
+    uint64_t best = ~0ull;
+#pragma unroll 1
+    for (int i = 0; i < (int)kSizes && 32u << i <= most_rows; ++i) {
+        uint64_t work = 0;
+        uint32_t U = 0, longest = 0;
+        for (int w = 0; w < kPlanWaves; ++w) {
+            work += s_work[w][i];
+            U += s_units[w][i];
+            longest = max(longest, s_long[w][i]);
+        }
+        const Estimate e = estimate(U, work, longest, 32u << i, lanes);
+        const uint64_t t = min(e.whole, e.cut);
+        if (t <= best) {
+            best = t;
+            unit_rows = 32u << i;
+        }
     }
-    uint32_t most_rows = 32;
-#pragma unroll
-    for (int w = 0; w < kPlanWaves; ++w) most_rows = max(most_rows, (uint32_t)s_sum[w][2 * kSizes]);
-    uint32_t unit_rows = 0;
-#pragma unroll
-    for (int i = kSizes - 1; i >= 0; --i)
-        if (!unit_rows && sums[i] >= 2 * lanes) unit_rows = 32u << i;
-#pragma unroll
-    for (int i = kSizes - 1; i >= 0; --i)
-        if (!unit_rows && sums[kSizes + i] >= (uint64_t)kWalkTiles * lanes) unit_rows = 32u << i;
-    unit_rows = min(unit_rows ? unit_rows : 32u, most_rows);
 
     // The units.  Their bound holds for any ascending query_start; the clamp
     // also keeps the units of an array that is none inside the plan.
@@ -209,7 +242,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
     if (tid == 0) s_first[batch] = U;
     __syncthreads();
     uint64_t* const cost = U <= kLocalUnits ? s_cost : reinterpret_cast<uint64_t*>(base + lay.costs);
-    uint64_t work = 0, longest = 0;
+    uint64_t work = 0;
+    uint32_t longest = 0;
     for (uint32_t i0 = 0; i0 < U; i0 += kPlanThreads) {
         const uint32_t i = i0 + tid;
         uint64_t c = 0, sum;
@@ -218,11 +252,11 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
             const Request r = s_req[b];
             const uint32_t rows = r.n * group, R = min(unit_rows, unit_rows_for(rows)), row0 = (i - s_first[b]) * R;
             PagedItem u = unit_of(a.head, b, r, group, row0, min(R, rows - row0));
-            const uint32_t per_tile = tile_cost(u.rows, s_first[b + 1] - s_first[b]);
+            const uint32_t per_tile = tile_cost(R, s_first[b + 1] - s_first[b], a.head.d);
             u.next = per_tile;  // (here; the items' own below)
             units[i] = u;
             c = (uint64_t)u.tile_end * per_tile + kItemCost;
-            longest = max(longest, c);
+            longest = max(longest, (uint32_t)c);
         }
         const uint64_t at = block_scan(c, &sum);
         if (i < U) cost[i] = work + at;
@@ -230,22 +264,19 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
     }
     if (tid == 0) cost[U] = work;
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) longest = max(longest, (uint64_t)__shfl_xor(longest, m));
-    if (lane == 0) s_sum[wave][0] = longest;
+    for (int m = 32; m >= 1; m >>= 1) longest = max(longest, (uint32_t)__shfl_xor(longest, m));
+    if (lane == 0) s_long[wave][0] = longest;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kPlanWaves; ++w) longest = max(longest, s_sum[w][0]);
+    for (int w = 0; w < kPlanWaves; ++w) longest = max(longest, s_long[w][0]);
 
-    const uint64_t share = work / lanes;
-    const uint32_t levels = share >= kLevelShare ? min(kPagedLevels, kPagedMaxRows / unit_rows) : 1;
-    const uint64_t rounds = U ? (uint64_t)((U + lanes - 1) / lanes) * work / U : 0;
-    const uint64_t whole = max(longest, rounds) + (unit_rows == 32 ? longest / 4 : 0);
-    const uint64_t cut = share + kItemCost * levels + 8 + unit_rows / 2;  // and the pieces' results
+    const Estimate e = estimate(U, work, longest, unit_rows, lanes);
+    const uint32_t levels = e.levels;
     uint32_t n_items = U, split_blocks = 0, ranges = max(U, lanes);
-    if (whole <= cut) {
+    if (e.whole <= e.cut) {
         // Whole units, longest first (by cost buckets; the order within one
         // decides only which lane runs a unit, never a result).
-        const float to_bucket = (float)(kBuckets - 1) / (float)max(longest, (uint64_t)1);
+        const float to_bucket = (float)(kBuckets - 1) / (float)max(longest, 1u);
         for (int pass = 0; pass < 2; ++pass) {
             for (uint32_t i = tid; i < U; i += kPlanThreads) {
                 const uint32_t q = (uint32_t)((float)(cost[i + 1] - cost[i]) * to_bucket);
