@@ -490,31 +490,49 @@ def sample_topk_topp_f32(logits, vocab: int, temperature: float, top_k: int, top
 
 # ------------------------------------------------------------- paged cache
 
-def _need(fn: str, dtype: str, *pairs) -> None:
-    """Each (tensor, elements): on the current device, dense, of the dtype
-    ("bf16", "u32" as int32 or uint32, "f32", "any") and holding at least that
-    many elements.  The C ABI sees addresses only."""
+@functools.lru_cache(maxsize=None)
+def _types():
+    """bf16, u32 (as int32 or uint32) and f32 as tuples of torch dtypes."""
     import torch
 
-    types = {"bf16": (torch.bfloat16,), "u32": (torch.int32, torch.uint32),
-             "f32": (torch.float32,)}.get(dtype)
-    device = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    return (torch.bfloat16,), (torch.int32, torch.uint32), (torch.float32,)
+
+
+@functools.lru_cache(maxsize=None)
+def _current_device_lookup():
+    import torch
+
+    return getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _on_device(fn: str, t) -> int:
+    """The current device, which `t` has to be on.  These checks are made on
+    every call and cost it 0.4 us a tensor (asking torch whether there is a
+    device at all, 1 us, is not needed: a tensor on one says so)."""
+    device = t.get_device()
+    if device < 0 or device != _current_device_lookup()():
+        raise ToyInferError(fn, ERR_INVALID_ARGUMENT)
+    return device
+
+
+def _need(fn: str, device: int, dtypes, *pairs) -> None:
+    """Each (tensor, elements): on the device, dense, of one of the dtypes and
+    holding at least that many elements.  The C ABI sees addresses only."""
     for t, n in pairs:
-        if (not t.is_contiguous() or t.numel() < n or t.get_device() != device or device < 0
-                or (types and t.dtype not in types)):
+        if (t.get_device() != device or t.dtype not in dtypes or t.numel() < n
+                or not t.is_contiguous()):
             raise ToyInferError(fn, ERR_INVALID_ARGUMENT)
 
 
-def _need_cache(fn: str, num_pages: int, page_size: int, page_stride: int, num_kv_heads: int,
-                head_dim: int, *caches) -> None:
+def _need_cache(fn: str, device: int, num_pages: int, page_size: int, page_stride: int,
+                num_kv_heads: int, head_dim: int, *caches) -> None:
     """Caches may be views with pages further apart than a page is long; what
     they span from their first element has to lie in their storage."""
-    import torch
-
+    bf16 = _types()[0]
     span = (num_pages - 1) * page_stride + page_size * num_kv_heads * head_dim
     for t in caches:
-        room = t.untyped_storage().nbytes() // 2 - t.storage_offset()
-        if t.dtype is not torch.bfloat16 or room < span or not t.is_cuda:
+        if (t.get_device() != device or t.dtype not in bf16
+                or t.untyped_storage().nbytes() // 2 - t.storage_offset() < span):
             raise ToyInferError(fn, ERR_INVALID_ARGUMENT)
 
 
@@ -525,9 +543,10 @@ def paged_tables_u32(context_lens, new_lens, batch: int, free_pages, free_capaci
     new pages from the top of the stack free_pages[:num_free]; status = (pages
     left, requests refused)."""
     fn = "paged_tables_u32"
-    _need(fn, "u32", (context_lens, batch), (new_lens, batch), (free_pages, free_capacity),
-          (num_free, 1), (block_tables, batch * max_blocks), (query_start, batch + 1),
-          (seq_lens, batch), (positions, num_tokens), (slot_mapping, num_tokens), (status, 2))
+    _need(fn, _on_device(fn, context_lens), _types()[1], (context_lens, batch), (new_lens, batch),
+          (free_pages, free_capacity), (num_free, 1), (block_tables, batch * max_blocks),
+          (query_start, batch + 1), (seq_lens, batch), (positions, num_tokens),
+          (slot_mapping, num_tokens), (status, 2))
     _check(fn, LIB.toyinfer_paged_tables_u32(
         _ptr(context_lens), _ptr(new_lens), batch, _ptr(free_pages), free_capacity, _ptr(num_free),
         page_size, _ptr(block_tables), max_blocks, num_tokens, _ptr(query_start), _ptr(seq_lens),
@@ -543,11 +562,14 @@ def paged_qkv_prologue_bf16(q, k, v, q_norm_weight, k_norm_weight, rope_cos_sin,
     slots, for num_tokens tokens (one launch)."""
     fn = "paged_qkv_prologue_bf16"
     row = num_tokens * head_dim
-    _need(fn, "bf16", (q, row * num_q_heads), (k, row * num_kv_heads), (v, row * num_kv_heads),
+    bf16, u32, f32 = _types()
+    device = _on_device(fn, q)
+    _need(fn, device, bf16, (q, row * num_q_heads), (k, row * num_kv_heads), (v, row * num_kv_heads),
           (q_norm_weight, head_dim), (k_norm_weight, head_dim), (q_out, row * num_q_heads))
-    _need(fn, "f32", (rope_cos_sin, num_positions * head_dim))
-    _need(fn, "u32", (positions, num_tokens), (slot_mapping, num_tokens))
-    _need_cache(fn, num_pages, page_size, page_stride, num_kv_heads, head_dim, k_cache, v_cache)
+    _need(fn, device, f32, (rope_cos_sin, num_positions * head_dim))
+    _need(fn, device, u32, (positions, num_tokens), (slot_mapping, num_tokens))
+    _need_cache(fn, device, num_pages, page_size, page_stride, num_kv_heads, head_dim, k_cache,
+                v_cache)
     _check(fn, LIB.toyinfer_paged_qkv_prologue_bf16(
         _ptr(q), _ptr(k), _ptr(v), _ptr(q_norm_weight), _ptr(k_norm_weight), _ptr(rope_cos_sin),
         num_positions, _ptr(positions), _ptr(slot_mapping), num_tokens, rms_norm_eps, _ptr(q_out),
@@ -587,8 +609,9 @@ def paged_attention_plan(query_start, seq_lens, batch: int, num_tokens: int, pag
                          num_kv_heads: int, heads_dim: int, plan, stream=None) -> None:
     """The work list of one step's paged attention, shared by its layers."""
     fn = "paged_attention_plan"
-    _need(fn, "u32", (query_start, batch + 1), (seq_lens, batch))
-    _need(fn, "any", (plan, 1))
+    device = _on_device(fn, query_start)
+    _need(fn, device, _types()[1], (query_start, batch + 1), (seq_lens, batch))
+    _need(fn, device, (plan.dtype,), (plan, 1))
     _check(fn, LIB.toyinfer_paged_attention_plan(
         _ptr(query_start), _ptr(seq_lens), batch, num_tokens, page_size, max_blocks, window, sinks,
         num_q_heads, num_kv_heads, heads_dim, _ptr(plan), plan.numel() * plan.element_size(),
@@ -604,10 +627,14 @@ def paged_attention_bf16(q, k_cache, v_cache, o, block_tables, plan, batch: int,
     paged_attention_plan with the same sizes."""
     fn = "paged_attention_bf16"
     rows = num_tokens * num_q_heads * heads_dim
-    _need(fn, "bf16", (q, rows), (o, rows))
-    _need(fn, "u32", (block_tables, batch * max_blocks))
-    _need(fn, "any", (plan, 1), (workspace, 1))
-    _need_cache(fn, num_pages, page_size, page_stride, num_kv_heads, heads_dim, k_cache, v_cache)
+    bf16, u32, _ = _types()
+    device = _on_device(fn, q)
+    _need(fn, device, bf16, (q, rows), (o, rows))
+    _need(fn, device, u32, (block_tables, batch * max_blocks))
+    _need(fn, device, (plan.dtype,), (plan, 1))
+    _need(fn, device, (workspace.dtype,), (workspace, 1))
+    _need_cache(fn, device, num_pages, page_size, page_stride, num_kv_heads, heads_dim, k_cache,
+                v_cache)
     _check(fn, LIB.toyinfer_paged_attention_bf16(
         _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(o), _ptr(block_tables), _ptr(plan),
         plan.numel() * plan.element_size(), batch, num_tokens, num_pages, page_size, page_stride,
