@@ -34,26 +34,46 @@ constexpr int kPlanWaves = kPlanThreads / 64;
 constexpr uint32_t kItemCost = 24;  // starting and finishing an item
 constexpr uint32_t kPieceTiles = 2;  // cuts lie on multiples of it, one 32-key half per wave
 constexpr uint32_t kLocalUnits = 2048;
-constexpr uint32_t kSizes = 4;         // 32, 64, 128 or 256 rows per unit
+constexpr uint32_t kSizes = 4;         // of units: 32, 64, 128 or 256 rows
 constexpr uint32_t kLevelShare = 800;  // a lane's share from which its ranges shrink by level
 
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t x) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) x += __shfl_xor(x, m);
-    return x;
+// x of the lane that a DPP control names, 0 where there is none.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t from(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
 }
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint64_t from(uint64_t x) {
+    return (uint64_t)from<CTRL, ROWS>((uint32_t)(x >> 32)) << 32 | from<CTRL, ROWS>((uint32_t)x);
+}
+// Inclusive over the wave's lanes: rows of 16 first, then the last lane of a
+// row into the next, then of the lower half into the upper.  (By shuffles
+// through LDS the kernel's scans and sums took 3 us longer.)
+template <typename T, typename F>
+__device__ __forceinline__ T wave_scan(T x, F op) {
+    x = op(x, from<0x111>(x));
+    x = op(x, from<0x112>(x));
+    x = op(x, from<0x114>(x));
+    x = op(x, from<0x118>(x));
+    x = op(x, from<0x142, 0xa>(x));
+    return op(x, from<0x143, 0xc>(x));
+}
+struct Sum {
+    template <typename T>
+    __device__ __forceinline__ T operator()(T x, T y) const {
+        return x + y;
+    }
+};
+struct Max {
+    __device__ __forceinline__ uint32_t operator()(uint32_t x, uint32_t y) const { return max(x, y); }
+};
 
 // Exclusive sums over the workgroup's threads in thread order, total in *sum.
 template <typename T>
 __device__ __forceinline__ T block_scan(T x, T* sum) {
     __shared__ T s_tot[kPlanWaves];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    T inc = x;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const T u = __shfl_up(inc, m);
-        if (lane >= m) inc += u;
-    }
+    const T inc = wave_scan(x, Sum{});
     if (lane == 63) s_tot[wave] = inc;
     __syncthreads();
     T before = 0, all = 0;
@@ -81,7 +101,8 @@ __device__ __forceinline__ uint32_t last_at_most(const T* a, uint32_t n, T x) {
     return lo;
 }
 
-__device__ __forceinline__ uint32_t unit_rows_for(uint32_t rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
+// Unit sizes are 32 << index.
+__device__ __forceinline__ uint32_t size_for(uint32_t rows) { return (rows > 32) + (rows > 64) + (rows > 128); }
 
 struct Request {
     uint32_t token0, n, len;
@@ -148,6 +169,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
     __shared__ uint32_t s_bucket[kBuckets];
     __shared__ uint64_t s_work[kPlanWaves][kSizes];
     __shared__ uint32_t s_units[kPlanWaves][kSizes], s_long[kPlanWaves][kSizes], s_most[kPlanWaves];
+    __shared__ uint64_t s_time[kSizes];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t batch = a.head.batch, hkv = a.head.hkv, group = a.head.hq / hkv;
     const uint32_t lanes = paged_lanes(hkv), max_units = paged_max_units(batch, a.head.num_tokens, group);
@@ -161,7 +183,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
     // inside q, keys inside the block table.  For each size its units, their
     // cost (by the request's middle unit) and the longest (by its last).
     uint64_t work_of[kSizes] = {};
-    uint32_t units_of[kSizes] = {}, long_of[kSizes] = {}, most_rows = 32;
+    uint32_t units_of[kSizes] = {}, long_of[kSizes] = {}, most = 0;
     const uint32_t room = (uint32_t)min((uint64_t)a.head.max_blocks * a.head.page_size, (uint64_t)0x7fffffffu);
     for (uint32_t b = tid; b < batch; b += kPlanThreads) {
         const uint32_t s = min(a.query_start[b], a.head.num_tokens), e = min(a.query_start[b + 1], a.head.num_tokens);
@@ -172,58 +194,60 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
         s_req[b] = r;
         const uint32_t rows = r.n * group;
         if (!rows) continue;
-        most_rows = max(most_rows, unit_rows_for(rows));
+        const uint32_t top = size_for(rows);
+        most = max(most, top);
+        uint32_t n = 0, mid_cost = 0, long_cost = 0;
 #pragma unroll
-        for (int i = 0; i < (int)kSizes; ++i) {
-            const uint32_t R = min(32u << i, unit_rows_for(rows)), n = (rows + R - 1) / R;
-            const uint32_t mid = n / 2 * R, last = (n - 1) * R, per_tile = tile_cost(min(R, rows), n, a.head.d);
+        for (uint32_t i = 0; i < kSizes; ++i) {
+            if (i <= top) {  // (at larger sizes the request is the same one unit)
+                const uint32_t R = 32u << i;
+                n = (rows + R - 1) >> (5 + i);
+                const uint32_t mid = n / 2 * R, last = (n - 1) * R, per_tile = tile_cost(R, n, a.head.d);
+                long_cost = unit_of(a.head, b, r, group, last, min(R, rows - last)).tile_end * per_tile + kItemCost;
+                mid_cost = mid == last ? long_cost
+                                       : unit_of(a.head, b, r, group, mid, R).tile_end * per_tile + kItemCost;
+            }
             units_of[i] += n;
-            work_of[i] += (uint64_t)n * (unit_of(a.head, b, r, group, mid, min(R, rows - mid)).tile_end * per_tile + kItemCost);
-            long_of[i] = max(long_of[i], unit_of(a.head, b, r, group, last, min(R, rows - last)).tile_end * per_tile + kItemCost);
+            work_of[i] += (uint64_t)n * mid_cost;
+            long_of[i] = max(long_of[i], long_cost);
         }
     }
     if (wave * 64 < batch) {
+        most = wave_scan(most, Max{});
 #pragma unroll
-        for (int i = 0; i < (int)kSizes; ++i) {
-            work_of[i] = wave_sum64(work_of[i]);
-#pragma unroll
-            for (int m = 32; m >= 1; m >>= 1) {
-                units_of[i] += __shfl_xor(units_of[i], m);
-                long_of[i] = max(long_of[i], (uint32_t)__shfl_xor(long_of[i], m));
-            }
+        for (uint32_t i = 0; i < kSizes; ++i) {
+            work_of[i] = wave_scan(work_of[i], Sum{});
+            units_of[i] = wave_scan(units_of[i], Sum{});
+            long_of[i] = wave_scan(long_of[i], Max{});
         }
-        most_rows = __any(most_rows == 256) ? 256 : __any(most_rows == 128) ? 128 : __any(most_rows == 64) ? 64 : 32;
     }
-    if (lane == 0) {
+    if (lane == 63) {
 #pragma unroll
-        for (int i = 0; i < (int)kSizes; ++i) {
+        for (uint32_t i = 0; i < kSizes; ++i) {
             s_work[wave][i] = work_of[i];
             s_units[wave][i] = units_of[i];
             s_long[wave][i] = long_of[i];
         }
-        s_most[wave] = most_rows;
+        s_most[wave] = most;
     }
     s_bucket[tid] = 0;
     __syncthreads();
-    for (int w = 0; w < kPlanWaves; ++w) most_rows = max(most_rows, s_most[w]);
-    uint32_t unit_rows = 32;
-    uint64_t best = ~0ull;
-#pragma unroll 1
-    for (int i = 0; i < (int)kSizes && 32u << i <= most_rows; ++i) {
-        uint64_t work = 0;
-        uint32_t U = 0, longest = 0;
-        for (int w = 0; w < kPlanWaves; ++w) {
-            work += s_work[w][i];
-            U += s_units[w][i];
-            longest = max(longest, s_long[w][i]);
-        }
-        const Estimate e = estimate(U, work, longest, 32u << i, lanes);
-        const uint64_t t = min(e.whole, e.cut);
-        if (t <= best) {
-            best = t;
-            unit_rows = 32u << i;
-        }
+    if (wave < kSizes) {  // a wave estimates a size
+        const uint32_t w = lane % kPlanWaves;
+        const bool own = lane < kPlanWaves;
+        const uint64_t work = wave_scan(own ? s_work[w][wave] : (uint64_t)0, Sum{});
+        const uint32_t U = wave_scan(own ? s_units[w][wave] : 0u, Sum{});
+        const uint32_t longest = wave_scan(own ? s_long[w][wave] : 0u, Max{});
+        most = wave_scan(s_most[w], Max{});
+        const Estimate e = estimate(U, work, longest, 32u << wave, lanes);
+        if (lane == 63) s_time[wave] = wave > most ? ~0ull : min(e.whole, e.cut);
     }
+    __syncthreads();
+    uint32_t size = 0;
+#pragma unroll
+    for (uint32_t i = 1; i < kSizes; ++i)
+        if (s_time[i] <= s_time[size] && s_time[i] != ~0ull) size = i;
+    const uint32_t unit_rows = 32u << size;
 
     // The units.  Their bound holds for any ascending query_start; the clamp
     // also keeps the units of an array that is none inside the plan.
@@ -232,8 +256,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
         const uint32_t b = b0 + tid;
         uint32_t n = 0, sum;
         if (b < batch) {
-            const uint32_t rows = s_req[b].n * group, R = min(unit_rows, unit_rows_for(rows));
-            n = (rows + R - 1) / R;
+            const uint32_t rows = s_req[b].n * group;
+            n = ((uint64_t)rows + unit_rows - 1) >> (5 + size);
         }
         const uint32_t at = block_scan(n, &sum);
         if (b < batch) s_first[b] = min(U + at, max_units);
@@ -250,9 +274,9 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
         if (i < U) {
             const uint32_t b = last_at_most(s_first, batch, i);
             const Request r = s_req[b];
-            const uint32_t rows = r.n * group, R = min(unit_rows, unit_rows_for(rows)), row0 = (i - s_first[b]) * R;
-            PagedItem u = unit_of(a.head, b, r, group, row0, min(R, rows - row0));
-            const uint32_t per_tile = tile_cost(R, s_first[b + 1] - s_first[b], a.head.d);
+            const uint32_t rows = r.n * group, row0 = (i - s_first[b]) << (5 + size);
+            PagedItem u = unit_of(a.head, b, r, group, row0, min(unit_rows, rows - row0));
+            const uint32_t per_tile = tile_cost(u.rows, s_first[b + 1] - s_first[b], a.head.d);
             u.next = per_tile;  // (here; the items' own below)
             units[i] = u;
             c = (uint64_t)u.tile_end * per_tile + kItemCost;
@@ -263,9 +287,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
         work += sum;
     }
     if (tid == 0) cost[U] = work;
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) longest = max(longest, (uint32_t)__shfl_xor(longest, m));
-    if (lane == 0) s_long[wave][0] = longest;
+    longest = wave_scan(longest, Max{});
+    if (lane == 63) s_long[wave][0] = longest;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kPlanWaves; ++w) longest = max(longest, s_long[w][0]);
@@ -390,13 +413,21 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
         }
     }
     if (tid == 0) {
-        PagedPlanHeader h = a.head;
+        PagedPlanHeader& h = *reinterpret_cast<PagedPlanHeader*>(base);
+        h.batch = batch;
+        h.num_tokens = a.head.num_tokens;
+        h.page_size = a.head.page_size;
+        h.max_blocks = a.head.max_blocks;
+        h.window = a.head.window;
+        h.sinks = a.head.sinks;
+        h.hq = a.head.hq;
+        h.hkv = hkv;
+        h.d = a.head.d;
         h.magic = kPagedMagic;
         h.items = n_items;
         h.split_blocks = split_blocks;
         h.ranges = ranges;
         h.units = U;
-        *reinterpret_cast<PagedPlanHeader*>(base) = h;
     }
 }
 
