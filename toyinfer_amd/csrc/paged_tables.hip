@@ -159,6 +159,18 @@ __global__ __launch_bounds__(kTabThreads) void paged_tables_kernel(PagedTablesAr
     }
 }
 
+// Each input row is read once and each output row written once here, so both
+// bypass the caches' retention: 8192 tokens of 32 + 2 * 8 heads 40.2 -> 36.7 us
+// (5.5 TB/s, the rate of a large copy), 1371 tokens 7.0 -> 5.3.
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint4 load_once16(const uint16_t* p) {
+    const u32x4_t x = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
+    return make_uint4(x.x, x.y, x.z, x.w);
+}
+__device__ __forceinline__ void store_once16(uint16_t* p, uint4 x) {
+    __builtin_nontemporal_store(u32x4_t{x.x, x.y, x.z, x.w}, reinterpret_cast<u32x4_t*>(p));
+}
+
 // D / 16 lanes per row, lane c the eight pairs (8c + k, 8c + k + D/2); U rows
 // per lane group, so that a position's angles and the weights are read once
 // for U rows.
@@ -180,8 +192,8 @@ __global__ __launch_bounds__(256) void paged_prologue_kernel(PagedPrologueArgs a
         const uint16_t* src = j < a.hq           ? a.q + ((uint64_t)t * a.hq + j) * D
                               : j < a.hq + a.hkv ? a.k + ((uint64_t)t * a.hkv + (j - a.hq)) * D
                                                  : a.v + ((uint64_t)t * a.hkv + (j - a.hq - a.hkv)) * D;
-        xr[u] = ldg16(src + 8 * c);
-        xi[u] = ldg16(src + 8 * c + HALF);
+        xr[u] = load_once16(src + 8 * c);
+        xi[u] = load_once16(src + 8 * c + HALF);
     }
     const uint4 qwr = ldg16(a.q_weight + 8 * c), qwi = ldg16(a.q_weight + 8 * c + HALF);
     const uint4 kwr = ldg16(a.k_weight + 8 * c), kwi = ldg16(a.k_weight + 8 * c + HALF);
@@ -233,8 +245,8 @@ __global__ __launch_bounds__(256) void paged_prologue_kernel(PagedPrologueArgs a
             dst = j < a.hq + a.hkv ? a.k_cache + cache_row + (uint64_t)(j - a.hq) * D
                                    : a.v_cache + cache_row + (uint64_t)(j - a.hq - a.hkv) * D;
         if (dst) {
-            *reinterpret_cast<uint4*>(dst + 8 * c) = xr[u];
-            *reinterpret_cast<uint4*>(dst + 8 * c + HALF) = xi[u];
+            store_once16(dst + 8 * c, xr[u]);
+            store_once16(dst + 8 * c + HALF, xi[u]);
         }
     }
 }
