@@ -366,4 +366,78 @@ inline size_t decode_workspace_bytes(uint32_t batch, uint32_t num_q_heads, uint3
     return toyinfer_decode_workspace_bytes(batch, num_q_heads, heads_dim, num_splits);
 }
 
+// ------------------------------------------- many requests: paged KV cache
+// Block tables on the device, the pre-attention pass into cache slots and the
+// attention of new tokens over pages; include/toyinfer_attn.h has the layouts.
+
+// One step's block tables, positions and slots from the requests' lengths.
+inline void paged_tables_u32(const uint32_t* context_lens, const uint32_t* new_lens, uint32_t batch,
+                             const uint32_t* free_pages, uint32_t free_capacity,
+                             const uint32_t* num_free, uint32_t page_size, uint32_t* block_tables,
+                             uint32_t max_blocks, uint32_t num_tokens, uint32_t* query_start,
+                             uint32_t* seq_lens, uint32_t* positions, uint32_t* slot_mapping,
+                             uint32_t* status, hipStream_t stream_d = nullptr) {
+    TOYINFER_CHECK(toyinfer_paged_tables_u32(context_lens, new_lens, batch, free_pages,
+                                             free_capacity, num_free, page_size, block_tables,
+                                             max_blocks, num_tokens, query_start, seq_lens,
+                                             positions, slot_mapping, status, stream_d),
+                   "paged_tables_u32");
+}
+
+// decode_qkv_prologue_bf16 for many tokens, each at its own position and slot.
+inline void paged_qkv_prologue_bf16(const bf16* q, const bf16* k, const bf16* v,
+                                    const bf16* q_norm_weight, const bf16* k_norm_weight,
+                                    const float* rope_cos_sin, uint32_t num_positions,
+                                    const uint32_t* positions, const uint32_t* slot_mapping,
+                                    uint32_t num_tokens, float rms_norm_eps, bf16* q_out,
+                                    bf16* k_cache, bf16* v_cache, uint32_t num_pages,
+                                    uint32_t page_size, uint64_t page_stride, uint32_t num_q_heads,
+                                    uint32_t num_kv_heads, uint32_t head_dim,
+                                    hipStream_t stream_d = nullptr) {
+    TOYINFER_CHECK(toyinfer_paged_qkv_prologue_bf16(
+                       q, k, v, q_norm_weight, k_norm_weight, rope_cos_sin, num_positions,
+                       positions, slot_mapping, num_tokens, rms_norm_eps, q_out, k_cache, v_cache,
+                       num_pages, page_size, page_stride, num_q_heads, num_kv_heads, head_dim,
+                       stream_d),
+                   "paged_qkv_prologue_bf16");
+}
+
+inline size_t paged_attention_plan_bytes(uint32_t batch, uint32_t num_tokens, uint32_t num_q_heads,
+                                         uint32_t num_kv_heads, uint32_t heads_dim) {
+    return toyinfer_paged_attention_plan_bytes(batch, num_tokens, num_q_heads, num_kv_heads,
+                                               heads_dim);
+}
+inline size_t paged_attention_workspace_bytes(uint32_t num_q_heads, uint32_t num_kv_heads,
+                                              uint32_t heads_dim) {
+    return toyinfer_paged_attention_workspace_bytes(num_q_heads, num_kv_heads, heads_dim);
+}
+
+// The work list of one step's paged attention, shared by its layers.
+inline void paged_attention_plan(const uint32_t* query_start, const uint32_t* seq_lens,
+                                 uint32_t batch, uint32_t num_tokens, uint32_t page_size,
+                                 uint32_t max_blocks, uint32_t window, uint32_t sinks,
+                                 uint32_t num_q_heads, uint32_t num_kv_heads, uint32_t heads_dim,
+                                 void* plan, size_t plan_bytes, hipStream_t stream_d = nullptr) {
+    TOYINFER_CHECK(toyinfer_paged_attention_plan(query_start, seq_lens, batch, num_tokens,
+                                                 page_size, max_blocks, window, sinks, num_q_heads,
+                                                 num_kv_heads, heads_dim, plan, plan_bytes,
+                                                 stream_d),
+                   "paged_attention_plan");
+}
+
+// Causal or sliding-window attention of the requests' new tokens.
+inline void paged_attention_bf16(const bf16* q, const bf16* k_cache, const bf16* v_cache, bf16* o,
+                                 const uint32_t* block_tables, const void* plan, size_t plan_bytes,
+                                 uint32_t batch, uint32_t num_tokens, uint32_t num_pages,
+                                 uint32_t page_size, uint64_t page_stride, uint32_t max_blocks,
+                                 uint32_t window, uint32_t sinks, uint32_t num_q_heads,
+                                 uint32_t num_kv_heads, uint32_t heads_dim, void* workspace,
+                                 size_t workspace_bytes, hipStream_t stream_d = nullptr) {
+    TOYINFER_CHECK(toyinfer_paged_attention_bf16(
+                       q, k_cache, v_cache, o, block_tables, plan, plan_bytes, batch, num_tokens,
+                       num_pages, page_size, page_stride, max_blocks, window, sinks, num_q_heads,
+                       num_kv_heads, heads_dim, workspace, workspace_bytes, stream_d),
+                   "paged_attention_bf16");
+}
+
 }  // namespace toyinfer
