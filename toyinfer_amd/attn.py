@@ -548,9 +548,9 @@ def paged_tables_u32(context_lens, new_lens, batch: int, free_pages, free_capaci
           (query_start, batch + 1), (seq_lens, batch), (positions, num_tokens),
           (slot_mapping, num_tokens), (status, 2))
     _check(fn, LIB.toyinfer_paged_tables_u32(
-        _ptr(context_lens), _ptr(new_lens), batch, _ptr(free_pages), free_capacity, _ptr(num_free),
-        page_size, _ptr(block_tables), max_blocks, num_tokens, _ptr(query_start), _ptr(seq_lens),
-        _ptr(positions), _ptr(slot_mapping), _ptr(status), _stream(stream)))
+        context_lens.data_ptr(), new_lens.data_ptr(), batch, free_pages.data_ptr(), free_capacity, num_free.data_ptr(),
+        page_size, block_tables.data_ptr(), max_blocks, num_tokens, query_start.data_ptr(), seq_lens.data_ptr(),
+        positions.data_ptr(), slot_mapping.data_ptr(), status.data_ptr(), _stream(stream)))
 
 
 def paged_qkv_prologue_bf16(q, k, v, q_norm_weight, k_norm_weight, rope_cos_sin,
@@ -571,9 +571,9 @@ def paged_qkv_prologue_bf16(q, k, v, q_norm_weight, k_norm_weight, rope_cos_sin,
     _need_cache(fn, device, num_pages, page_size, page_stride, num_kv_heads, head_dim, k_cache,
                 v_cache)
     _check(fn, LIB.toyinfer_paged_qkv_prologue_bf16(
-        _ptr(q), _ptr(k), _ptr(v), _ptr(q_norm_weight), _ptr(k_norm_weight), _ptr(rope_cos_sin),
-        num_positions, _ptr(positions), _ptr(slot_mapping), num_tokens, rms_norm_eps, _ptr(q_out),
-        _ptr(k_cache), _ptr(v_cache), num_pages, page_size, page_stride, num_q_heads, num_kv_heads,
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), rope_cos_sin.data_ptr(),
+        num_positions, positions.data_ptr(), slot_mapping.data_ptr(), num_tokens, rms_norm_eps, q_out.data_ptr(),
+        k_cache.data_ptr(), v_cache.data_ptr(), num_pages, page_size, page_stride, num_q_heads, num_kv_heads,
         head_dim, _stream(stream)))
 
 
@@ -613,8 +613,8 @@ def paged_attention_plan(query_start, seq_lens, batch: int, num_tokens: int, pag
     _need(fn, device, _types()[1], (query_start, batch + 1), (seq_lens, batch))
     _need(fn, device, (plan.dtype,), (plan, 1))
     _check(fn, LIB.toyinfer_paged_attention_plan(
-        _ptr(query_start), _ptr(seq_lens), batch, num_tokens, page_size, max_blocks, window, sinks,
-        num_q_heads, num_kv_heads, heads_dim, _ptr(plan), plan.numel() * plan.element_size(),
+        query_start.data_ptr(), seq_lens.data_ptr(), batch, num_tokens, page_size, max_blocks, window, sinks,
+        num_q_heads, num_kv_heads, heads_dim, plan.data_ptr(), plan.numel() * plan.element_size(),
         _stream(stream)))
 
 
@@ -636,7 +636,7 @@ def paged_attention_bf16(q, k_cache, v_cache, o, block_tables, plan, batch: int,
     _need_cache(fn, device, num_pages, page_size, page_stride, num_kv_heads, heads_dim, k_cache,
                 v_cache)
     _check(fn, LIB.toyinfer_paged_attention_bf16(
-        _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(o), _ptr(block_tables), _ptr(plan),
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), block_tables.data_ptr(), plan.data_ptr(),
         plan.numel() * plan.element_size(), batch, num_tokens, num_pages, page_size, page_stride,
-        max_blocks, window, sinks, num_q_heads, num_kv_heads, heads_dim, _ptr(workspace),
+        max_blocks, window, sinks, num_q_heads, num_kv_heads, heads_dim, workspace.data_ptr(),
         workspace.numel() * workspace.element_size(), _stream(stream)))
