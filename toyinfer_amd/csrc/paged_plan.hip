@@ -15,14 +15,19 @@
 //   leaves partial results of each piece, merged by a second kernel.
 // The size and the way are those with the shortest estimate: rounds of whole
 // units times their mean, or the longest of them, against the even share plus
-// the pieces' overhead.  At 32 query and 8 KV heads of 128, forced sizes of
-// 32 / 64 / 128 / 256 rows took, in us (* the choice): 512 tokens on 8192 keys
-// 201 / 92 / 89 / 84*, a prompt of 512 - / 16* / 20 / 26, of 2048 - / 76 / 66* /
-// 80, of 8192 1494 / 733 / 576 / 528*.
+// the pieces' overhead.  Forced ones took, in us, at 32 query and 8 KV heads of
+// 128 (w whole, c cut, * the choice):
+//                              64 w / c     128 w / c    256 w / c rows
+//   512 tokens on 8192 keys    93 / 123     119 / 87*    204 / 83
+//   a prompt of 512            16* / 23      20 / 23      26 / 28
+//   a prompt of 2048           76 / 83       66* / 73     64 / 70
+//   a prompt of 8192          757 / 800     587 / 662    533* / 580
+//   33 decoded and 5 chunks   182 / 211     156 / 174    181 / 158*
+// (32 rows: 201 for the first and 1494 for the fourth.)
 //
-// Costs are in units of about 0.12 us of a lane: a 64-key tile takes its
-// products, or its bytes' time from HBM shared by the units of the request that
-// read them, whichever is longer.
+// Costs are in units of about 0.12 us of a lane.  A 64-key tile takes its
+// products (up to 32 rows: the latency of its bytes), or, for requests of up to
+// 32 rows in a step bound by the keys' bytes, its share of the bandwidth.
 #include "common.hpp"
 #include "paged.hpp"
 
@@ -31,7 +36,8 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
-constexpr uint32_t kItemCost = 24;  // starting and finishing an item
+constexpr uint32_t kStreamTile = 8;  // of up to 32 rows: the latency of its bytes, at either head_dim
+constexpr uint32_t kStreamItem = 24, kSharedItem = 80;  // starting and finishing an item
 constexpr uint32_t kPieceTiles = 2;  // cuts lie on multiples of it, one 32-key half per wave
 constexpr uint32_t kLocalUnits = 2048;
 constexpr uint32_t kSizes = 4;         // of units: 32, 64, 128 or 256 rows
@@ -131,25 +137,37 @@ __device__ __forceinline__ PagedItem unit_of(const PagedPlanHeader& h, uint32_t 
     return u;
 }
 
-// Of one of `units` units of a request, per tile.
-__device__ __forceinline__ uint32_t tile_cost(uint32_t rows, uint32_t units, uint32_t d) {
-    const uint32_t products = rows <= 64 ? 6 : rows <= 128 ? 9 : 17, bytes = 11;
-    return max(d == 64 ? (2 * products + 2) / 3 : products, (d == 64 ? (bytes + 1) / 2 : bytes) / units);
+// A tile's products, by the unit's rows; its bytes' time where all lanes stream
+// at once.
+__device__ __forceinline__ uint32_t product_cost(uint32_t rows, uint32_t d) {
+    if (rows <= 32) return kStreamTile;
+    const uint32_t c = rows <= 64 ? 6 : rows <= 128 ? 9 : 17;
+    return d == 64 ? (2 * c + 2) / 3 : c;
 }
+__device__ __forceinline__ uint32_t bytes_cost(uint32_t d) { return d == 64 ? 6 : 11; }
+// Of a request with up to 32 rows in a step that streams.
+__device__ __forceinline__ uint32_t stream_cost(uint32_t d) { return max(kStreamTile, bytes_cost(d)); }
+__device__ __forceinline__ uint32_t item_cost(uint32_t rows) { return rows <= 32 ? kStreamItem : kSharedItem; }
 
 // The whole step, for U units of this total and longest cost: each as a list of
-// its own, or cut into even shares.
+// its own, or cut into even shares.  `streamed`: the cost of the units of
+// requests with up to 32 rows.
 struct Estimate {
     uint64_t whole, cut;
     uint32_t levels;
 };
-__device__ __forceinline__ Estimate estimate(uint32_t U, uint64_t work, uint64_t longest, uint32_t rows, uint32_t lanes) {
+__device__ __forceinline__ Estimate estimate(uint32_t U, uint64_t work, uint64_t longest, uint64_t streamed,
+                                             uint32_t rows, uint32_t lanes) {
     const uint64_t share = work / lanes;
     Estimate e;
     e.levels = share >= kLevelShare ? min(kPagedLevels, kPagedMaxRows / rows) : 1;
     const uint64_t rounds = U ? (uint64_t)((U + lanes - 1) / lanes) * work / U : 0;
     e.whole = max(longest, rounds) + (rows == 32 ? longest / 4 : 0);
-    e.cut = share + kItemCost * e.levels + 8 + rows / 2;  // and the pieces' results
+    // A cut costs a lane another item and its piece's results (half a unit per
+    // row), by what it falls into.
+    const float in_stream = rows == 32 || !work ? 1.0f : (float)streamed / (float)work;
+    const float per_cut = in_stream * (item_cost(32) + 16) + (1.0f - in_stream) * (item_cost(rows) + rows / 2);
+    e.cut = share + 8 + (uint64_t)(per_cut * e.levels);
     return e;
 }
 
@@ -169,7 +187,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
     __shared__ uint32_t s_bucket[kBuckets];
     __shared__ uint64_t s_work[kPlanWaves][kSizes];
     __shared__ uint32_t s_units[kPlanWaves][kSizes], s_long[kPlanWaves][kSizes], s_most[kPlanWaves];
-    __shared__ uint64_t s_time[kSizes];
+    __shared__ uint64_t s_time[kSizes], s_bytes[kPlanWaves], s_products[kPlanWaves], s_streamed[kPlanWaves + 1];
+    __shared__ uint32_t s_streams[kPlanWaves + 1], s_stream_long[kPlanWaves];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t batch = a.head.batch, hkv = a.head.hkv, group = a.head.hq / hkv;
     const uint32_t lanes = paged_lanes(hkv), max_units = paged_max_units(batch, a.head.num_tokens, group);
@@ -181,9 +200,11 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
 
     // Lengths as the kernels may use them whatever the arrays hold: tokens
     // inside q, keys inside the block table.  For each size its units, their
-    // cost (by the request's middle unit) and the longest (by its last).
-    uint64_t work_of[kSizes] = {};
-    uint32_t units_of[kSizes] = {}, long_of[kSizes] = {}, most = 0;
+    // cost (by the request's middle unit) and the longest (by its last).  The
+    // step streams if its keys' bytes take longer than its products: then each
+    // lane gets its share of the bandwidth, and else as much as it asks for.
+    uint64_t work_of[kSizes] = {}, bytes = 0, products = 0, streamed = 0;
+    uint32_t units_of[kSizes] = {}, long_of[kSizes] = {}, most = 0, stream_long = 0, streams = 0;
     const uint32_t room = (uint32_t)min((uint64_t)a.head.max_blocks * a.head.page_size, (uint64_t)0x7fffffffu);
     for (uint32_t b = tid; b < batch; b += kPlanThreads) {
         const uint32_t s = min(a.query_start[b], a.head.num_tokens), e = min(a.query_start[b + 1], a.head.num_tokens);
@@ -196,24 +217,37 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
         if (!rows) continue;
         const uint32_t top = size_for(rows);
         most = max(most, top);
-        uint32_t n = 0, mid_cost = 0, long_cost = 0;
+        uint32_t n = 0, mid_tiles = 0, mid_cost = 0, long_tiles = 0, long_cost = 0;
 #pragma unroll
         for (uint32_t i = 0; i < kSizes; ++i) {
             if (i <= top) {  // (at larger sizes the request is the same one unit)
                 const uint32_t R = 32u << i;
                 n = (rows + R - 1) >> (5 + i);
-                const uint32_t mid = n / 2 * R, last = (n - 1) * R, per_tile = tile_cost(R, n, a.head.d);
-                long_cost = unit_of(a.head, b, r, group, last, min(R, rows - last)).tile_end * per_tile + kItemCost;
-                mid_cost = mid == last ? long_cost
-                                       : unit_of(a.head, b, r, group, mid, R).tile_end * per_tile + kItemCost;
+                const uint32_t mid = n / 2 * R, last = (n - 1) * R, per_tile = product_cost(R, a.head.d);
+                long_tiles = unit_of(a.head, b, r, group, last, min(R, rows - last)).tile_end;
+                mid_tiles = mid == last ? long_tiles : unit_of(a.head, b, r, group, mid, R).tile_end;
+                long_cost = long_tiles * per_tile + item_cost(R);
+                mid_cost = mid_tiles * per_tile + item_cost(R);
             }
             units_of[i] += n;
             work_of[i] += (uint64_t)n * mid_cost;
             long_of[i] = max(long_of[i], long_cost);
         }
+        bytes += mid_tiles * bytes_cost(a.head.d);
+        products += (uint64_t)n * mid_tiles * product_cost(32u << top, a.head.d);
+        if (top == 0) {
+            ++streams;
+            streamed += mid_tiles;
+            stream_long = max(stream_long, mid_tiles);
+        }
     }
     if (wave * 64 < batch) {
         most = wave_scan(most, Max{});
+        bytes = wave_scan(bytes, Sum{});
+        products = wave_scan(products, Sum{});
+        streams = wave_scan(streams, Sum{});
+        streamed = wave_scan(streamed, Sum{});
+        stream_long = wave_scan(stream_long, Max{});
 #pragma unroll
         for (uint32_t i = 0; i < kSizes; ++i) {
             work_of[i] = wave_scan(work_of[i], Sum{});
@@ -229,20 +263,45 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
             s_long[wave][i] = long_of[i];
         }
         s_most[wave] = most;
+        s_bytes[wave] = bytes;
+        s_products[wave] = products;
+        s_streams[wave] = streams;
+        s_streamed[wave] = streamed;
+        s_stream_long[wave] = stream_long;
     }
     s_bucket[tid] = 0;
     __syncthreads();
     if (wave < kSizes) {  // a wave estimates a size
         const uint32_t w = lane % kPlanWaves;
         const bool own = lane < kPlanWaves;
-        const uint64_t work = wave_scan(own ? s_work[w][wave] : (uint64_t)0, Sum{});
+        uint64_t work = wave_scan(own ? s_work[w][wave] : (uint64_t)0, Sum{});
         const uint32_t U = wave_scan(own ? s_units[w][wave] : 0u, Sum{});
-        const uint32_t longest = wave_scan(own ? s_long[w][wave] : 0u, Max{});
+        uint32_t longest = wave_scan(own ? s_long[w][wave] : 0u, Max{});
         most = wave_scan(s_most[w], Max{});
-        const Estimate e = estimate(U, work, longest, 32u << wave, lanes);
-        if (lane == 63) s_time[wave] = wave > most ? ~0ull : min(e.whole, e.cut);
+        bytes = wave_scan(own ? s_bytes[w] : (uint64_t)0, Sum{});
+        products = wave_scan(own ? s_products[w] : (uint64_t)0, Sum{});
+        streams = wave_scan(own ? s_streams[w] : 0u, Sum{});
+        streamed = wave_scan(own ? s_streamed[w] : (uint64_t)0, Sum{});
+        stream_long = wave_scan(s_stream_long[w], Max{});
+        uint32_t per_tile = kStreamTile;
+        if (bytes > products) {
+            per_tile = stream_cost(a.head.d);
+            work += streamed * (per_tile - kStreamTile);
+            if (streams) longest = max(longest, stream_long * per_tile + item_cost(32));
+        }
+        streamed = streamed * per_tile + (uint64_t)streams * item_cost(32);
+        const Estimate e = estimate(U, work, longest, streamed, 32u << wave, lanes);
+        if (lane == 63) {
+            s_time[wave] = wave > most ? ~0ull : min(e.whole, e.cut);
+            if (wave == 0) {
+                s_streamed[kPlanWaves] = streamed;
+                s_streams[kPlanWaves] = per_tile;
+            }
+        }
     }
     __syncthreads();
+    streamed = s_streamed[kPlanWaves];
+    const uint32_t stream_tile = s_streams[kPlanWaves];
     uint32_t size = 0;
 #pragma unroll
     for (uint32_t i = 1; i < kSizes; ++i)
@@ -276,10 +335,10 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
             const Request r = s_req[b];
             const uint32_t rows = r.n * group, row0 = (i - s_first[b]) << (5 + size);
             PagedItem u = unit_of(a.head, b, r, group, row0, min(unit_rows, rows - row0));
-            const uint32_t per_tile = tile_cost(u.rows, s_first[b + 1] - s_first[b], a.head.d);
+            const uint32_t per_tile = rows <= 32 ? stream_tile : product_cost(u.rows, a.head.d);
             u.next = per_tile;  // (here; the items' own below)
             units[i] = u;
-            c = (uint64_t)u.tile_end * per_tile + kItemCost;
+            c = (uint64_t)u.tile_end * per_tile + item_cost(u.rows);
             longest = max(longest, (uint32_t)c);
         }
         const uint64_t at = block_scan(c, &sum);
@@ -293,7 +352,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
 #pragma unroll
     for (int w = 0; w < kPlanWaves; ++w) longest = max(longest, s_long[w][0]);
 
-    const Estimate e = estimate(U, work, longest, unit_rows, lanes);
+    const Estimate e = estimate(U, work, longest, streamed, unit_rows, lanes);
     const uint32_t levels = e.levels;
     uint32_t n_items = U, split_blocks = 0, ranges = max(U, lanes);
     if (e.whole <= e.cut) {
@@ -332,10 +391,10 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
             const uint64_t x = work * ((uint64_t)before * lanes + (uint64_t)size * nth) / ((uint64_t)kParts * lanes);
             uint32_t i = r == ranges ? U : last_at_most(cost, U, x), t = 0;
             if (i < U) {
-                const uint32_t tiles = units[i].tile_end, per_tile = units[i].next;
+                const uint32_t tiles = units[i].tile_end, per_tile = units[i].next, item = item_cost(units[i].rows);
                 const uint64_t off = x - cost[i];
-                if (off > kItemCost)
-                    t = (uint32_t)((off - kItemCost + per_tile * kPieceTiles / 2) / (per_tile * kPieceTiles)) * kPieceTiles;
+                if (off > item)
+                    t = (uint32_t)((off - item + per_tile * kPieceTiles / 2) / (per_tile * kPieceTiles)) * kPieceTiles;
                 if (t + kPieceTiles > tiles && t > 0) {
                     t = 0;
                     ++i;
