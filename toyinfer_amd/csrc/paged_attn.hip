@@ -183,15 +183,21 @@ __device__ __forceinline__ void probabilities(f32x16_t (&st)[NB], RowState<D>& s
     s.l += ts;
 }
 
+// Minus infinity over the scores of keys that this lane's row does not see.
 template <int D, int NB>
 __device__ __forceinline__ void hide(f32x16_t (&st)[NB], const RowView& rv, uint32_t k0, int kg) {
     // Keeps the branch around this: as selects it would run for every tile.
     asm volatile("; hidden keys");
+    const int32_t ago = rv.pos - (int32_t)k0 - 4 * kg;  // of the lane's first key; key c of it lies ago - c behind the row
+    const int32_t sinks = min((int32_t)min(rv.sinks, 0x7fffffffu), rv.pos + 1) - (int32_t)k0 - 4 * kg;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (!rv.sees(k0 + 32 * nb + 8 * (i / 4) + 4 * kg + i % 4)) st[nb][i] = -INFINITY;
+        for (int i = 0; i < 16; ++i) {
+            const int32_t c = 32 * nb + 8 * (i / 4) + i % 4;
+            const float x = c < sinks ? st[nb][i] : -INFINITY;
+            st[nb][i] = (uint32_t)(ago - c) < rv.window ? st[nb][i] : x;
+        }
 }
 
 // V^T operand of k-step tt (16 keys), d-block db.
@@ -252,7 +258,7 @@ template <int D, int NB>
 __device__ __forceinline__ void tile(RowState<D>& s, const uint16_t* kb, const uint16_t* vb,
                                      const int (&k_off)[D / 16], const int (&v_off)[D / 32],
                                      const bf16x8_t (&qf)[D / 16], const RowView& rv, uint32_t k0, uint32_t key_end,
-                                     float scale_log2, int lane, uint32_t* flag) {
+                                     float scale_log2, int lane, bool& bad) {
     const int kg = lane >> 5;
     constexpr int KSTEPS = D / 16;
     f32x16_t st[NB];
@@ -285,15 +291,37 @@ __device__ __forceinline__ void tile(RowState<D>& s, const uint16_t* kb, const u
     if (hidden) hide<D, NB>(st, rv, k0, kg);
     bf16x8_t pf[2 * NB];
     probabilities<D, NB>(st, s, pf, scale_log2);
-    if (hidden && rv.some_hidden(k0, min(k1, key_end - 1)) && any_nonfinite<D, NB>(vb, lane)) *flag = 1;
+    if (hidden && rv.some_hidden(k0, min(k1, key_end - 1)) && any_nonfinite<D, NB>(vb, lane)) bad = true;
     values<D, NB>(s, vb, v_off, pf);
+}
+
+// What the workgroup runs next, in LDS: an item or, of a streamed one, as many
+// of its tiles as a table holds.
+constexpr uint32_t kSegEntries = kTabEntries / 2;
+struct Segment {
+    PagedItem it;      // tile_end is the segment's; the item's is below
+    uint32_t kvh, kind, item_end, opens;
+    uint32_t token, head;  // of the unit's first row, the head in its group
+    int32_t pos;
+    uint32_t pad;
+};
+
+// The kernel's arguments, read again where they are used: in registers
+// throughout, they would push the loops' own out.
+__device__ __forceinline__ const PagedAttnArgs& arguments() {
+    typedef __attribute__((address_space(4))) const PagedAttnArgs* args_t;
+    args_t p = (args_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const PagedAttnArgs*)p;
 }
 
 // What every form needs of an item.
 struct ItemView {
     PagedItem it;
     KeySource src;
-    uint32_t kvh, group;
+    uint32_t kvh, group, token, head;
+    int32_t pos;
+    float inv_group;
 };
 
 __device__ __forceinline__ void point_at(ItemView& v, const PagedAttnArgs& a, const PagedItem& it, uint32_t kvh) {
@@ -305,29 +333,49 @@ __device__ __forceinline__ void point_at(ItemView& v, const PagedAttnArgs& a, co
     v.src.k = reinterpret_cast<const char*>(a.k_cache + (uint64_t)kvh * a.head.d);
     v.src.v = reinterpret_cast<const char*>(a.v_cache + (uint64_t)kvh * a.head.d);
 }
+__device__ __forceinline__ void point_at(ItemView& v, const PagedAttnArgs& a, const Segment& s) {
+    point_at(v, a, s.it, s.kvh);
+    v.token = s.token;
+    v.head = s.head;
+    v.pos = s.pos;
+}
 
-// The bases of tiles [c0, c1), by `threads` threads: entry i of a tile is for
-// its keys from i << entry_shift on.  Past the last key seen: its entry.
-__device__ __forceinline__ void fill_table(const PagedAttnArgs& a, const ItemView& v, uint2* tab, uint32_t c0,
-                                           uint32_t c1, uint32_t tid, uint32_t threads) {
-    const uint32_t per_shift = 6 - v.src.entry_shift, n = (c1 - c0) << per_shift;
+// Tokens that row `row` (< 256) of the unit lies behind its first row's.  The
+// quotient is exact: it is at least 0.5 / group from an integer, and its error
+// below 2^-22 of itself.
+__device__ __forceinline__ uint32_t tokens_on(const ItemView& v, uint32_t row) {
+    return (uint32_t)(((float)(v.head + row) + 0.5f) * v.inv_group);
+}
+// Offset of its row of q and o, in rows of D.
+__device__ __forceinline__ uint64_t row_of(const PagedAttnArgs& a, const ItemView& v, uint32_t row) {
+    const uint32_t t = tokens_on(v, row);
+    return (uint64_t)(v.token + t) * a.head.hq + v.kvh * v.group + (v.head + row - t * v.group);
+}
+
+// The page that holds a key, and its rows' base in the caches, by the entry that
+// the key lies in.  Past the last key seen: that one's.
+__device__ __forceinline__ uint32_t page_of(const PagedAttnArgs& a, const ItemView& v, uint32_t key) {
+    const uint32_t k = min(key, v.src.key_end - 1);
+    return a.block_tables[(uint64_t)v.it.req * a.head.max_blocks + (k >> v.src.page_shift)];
+}
+__device__ __forceinline__ uint2 base_in(const PagedAttnArgs& a, const ItemView& v, uint32_t key, uint32_t page) {
     const uint32_t in_page = (1u << v.src.page_shift) - 1, in_entry = (1u << v.src.entry_shift) - 1;
-    const uint32_t* const row = a.block_tables + (uint64_t)v.it.req * a.head.max_blocks;
-    for (uint32_t i = tid; i < n; i += threads) {
-        const uint32_t key = v.src.key0(c0 + (i >> per_shift)) + ((i & ((1u << per_shift) - 1)) << v.src.entry_shift);
-        const uint32_t k = min(key, (v.src.key_end - 1) & ~in_entry);
-        const uint32_t page = min(row[k >> v.src.page_shift], a.num_pages - 1);
-        const uint64_t base = page * v.src.page_bytes + (uint64_t)(k & in_page) * v.src.row_bytes;
-        tab[i] = make_uint2((uint32_t)base, (uint32_t)(base >> 32));
-    }
+    const uint32_t k = min(key, (v.src.key_end - 1) & ~in_entry);
+    const uint64_t base = min(page, a.num_pages - 1) * v.src.page_bytes + (uint64_t)(k & in_page) * v.src.row_bytes;
+    return make_uint2((uint32_t)base, (uint32_t)(base >> 32));
+}
+// First key of entry i of the tiles from c0 on: entry e of a tile is for its
+// keys from e << entry_shift on.
+__device__ __forceinline__ uint32_t entry_key(const ItemView& v, uint32_t c0, uint32_t i) {
+    const uint32_t per_shift = 6 - v.src.entry_shift;
+    return v.src.key0(c0 + (i >> per_shift)) + ((i & ((1u << per_shift) - 1)) << v.src.entry_shift);
 }
 
 // Q^T operand of this lane's row.
 template <int D>
 __device__ __forceinline__ void load_rows(bf16x8_t (&qf)[D / 16], const PagedAttnArgs& a, const ItemView& v,
                                           uint32_t row, int kg) {
-    const uint32_t r = v.it.row0 + row, token = v.it.token0 + r / v.group, head = v.kvh * v.group + r % v.group;
-    const uint16_t* q = a.q + ((uint64_t)token * a.head.hq + head) * D + 8 * kg;
+    const uint16_t* q = a.q + row_of(a, v, row) * D + 8 * kg;
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) qf[ks] = as_bf16x8(ldg16(q + 16 * ks));
 }
@@ -344,9 +392,8 @@ __device__ __forceinline__ void put(const PagedAttnArgs& a, const ItemView& v, u
         reinterpret_cast<float4*>(a.part_o)[(blk * PaShape<D>::NF + f) * 64 + lane] = x;
         return;
     }
-    const uint32_t r = v.it.row0 + row, token = v.it.token0 + r / v.group, head = v.kvh * v.group + r % v.group;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a row that saw nothing: 0
-    uint16_t* o = a.o + ((uint64_t)token * a.head.hq + head) * D + 8 * f + 4 * (lane >> 5);
+    uint16_t* o = a.o + row_of(a, v, row) * D + 8 * f + 4 * (lane >> 5);
     *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
 }
 __device__ __forceinline__ void put_ml(const PagedAttnArgs& a, const ItemView& v, uint32_t row_block, int lane,
@@ -366,6 +413,32 @@ __device__ __forceinline__ void finish(const PagedAttnArgs& a, const ItemView& v
     const int rb = wave % RB, part = wave / RB;
     const float l = xor32_sum(s.l);
     if constexpr (KS == 1) {
+        if (v.it.partial == kPagedWhole) {
+            // Through LDS into rows, 16 bytes a lane: as the lanes hold them, each
+            // store would touch 32 rows.
+            constexpr int CPR = PaShape<D>::CPR, RI = PaShape<D>::RI;
+            uint16_t* const own = (wave < 4 ? s_a : s_b) + (wave & 3) * 32 * D;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // a row that saw nothing: 0
+            int at = (lane & 31) * D + 8 * (lane & (CPR - 1)) + 4 * (lane >> 5);
+            asm volatile("" : "+v"(at));
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+                const float x0 = s.o[f / 4][4 * (f % 4)] * inv, x1 = s.o[f / 4][4 * (f % 4) + 1] * inv;
+                const float x2 = s.o[f / 4][4 * (f % 4) + 2] * inv, x3 = s.o[f / 4][4 * (f % 4) + 3] * inv;
+                *reinterpret_cast<uint2*>(own + (at ^ 8 * f)) =
+                    make_uint2(pack_bf16x2(x0, x1), pack_bf16x2(x2, x3));
+            }
+            int ln = lane;
+            asm volatile("" : "+v"(ln) : : "memory");  // (the rows' places are made after the accumulators are gone)
+#pragma unroll
+            for (int i = 0; i < 32 / RI; ++i) {
+                const int r = RI * i + ln / CPR, c = ln % CPR;
+                const uint32_t row = rb * kPagedBlockRows + r;
+                const uint4 x = *reinterpret_cast<const uint4*>(own + r * D + 8 * (c ^ (r & (CPR - 1))));
+                if (row < v.it.rows) *reinterpret_cast<uint4*>(a.o + row_of(a, v, row) * D + 8 * c) = x;
+            }
+            return;
+        }
 #pragma unroll
         for (int f = 0; f < NF; ++f)
             put<D>(a, v, rb, lane, f,
@@ -419,6 +492,10 @@ __device__ __forceinline__ void finish(const PagedAttnArgs& a, const ItemView& v
     }
 }
 
+// Workgroup barrier that waits for this wave's LDS operations only and leaves
+// its loads in flight.
+__device__ __forceinline__ void lds_ops_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // More than 32 rows: RB = 8, 4 or 2 row blocks.  A step is one tile (RB = 8) or
 // two, filled by all waves; stream s of the 8 / RB takes its own 64 (RB >= 4) or
 // 32 keys of it.
@@ -454,19 +531,30 @@ __device__ __forceinline__ void run_shared(const PagedAttnArgs& a, const ItemVie
     }
     const uint32_t last_row = v.it.rows - 1, row = min((uint32_t)(rb * 32 + ql), last_row);
     const uint32_t w_first = min((uint32_t)rb * 32, last_row), w_last = min((uint32_t)rb * 32 + 31, last_row);
-    rv.pos = v.it.pos0 + (int32_t)((v.it.row0 + row) / v.group);
-    rv.span(v.it.pos0 + (int32_t)((v.it.row0 + w_first) / v.group), v.it.pos0 + (int32_t)((v.it.row0 + w_last) / v.group));
+    rv.pos = v.pos + (int32_t)tokens_on(v, row);
+    rv.span(v.pos + (int32_t)__builtin_amdgcn_readfirstlane(tokens_on(v, w_first)),
+            v.pos + (int32_t)__builtin_amdgcn_readfirstlane(tokens_on(v, w_last)));
     const bool live = rb * 32 < (int)v.it.rows;
     bf16x8_t qf[P::KSTEPS];
     load_rows<D>(qf, a, v, row, kg);
     RowState<D> s;
     clear(s);
+    bool bad = false;
 
     for (uint32_t c0 = v.it.tile_begin; c0 < v.it.tile_end; c0 += chunk) {
         const uint32_t c1 = min(v.it.tile_end, c0 + chunk);
-        __syncthreads();  // the last chunk's page numbers and tiles are done with
-        fill_table(a, v, s_tab, c0, c1, threadIdx.x, kPaThreads);
-        __syncthreads();
+        // The first step's loads wait for their own table entries only, not for
+        // the whole table.
+        constexpr int OWN = kTabEntries / kPaThreads;
+        const uint32_t n = (c1 - c0) << per_shift;
+        const uint32_t own_key = entry_key(v, min(c0 + fill_tile, c1 - 1) , lane & ((1u << per_shift) - 1));
+        const uint32_t own_page = page_of(a, v, own_key);
+        uint32_t page[OWN];
+#pragma unroll
+        for (int u = 0; u < OWN; ++u) {
+            const uint32_t i = threadIdx.x + u * kPaThreads;
+            page[u] = i < n ? page_of(a, v, entry_key(v, c0, i)) : 0;
+        }
         // This wave's part of the step from tile t on (its tile may lie past the
         // last).
         auto bases_of = [&](uint32_t t) __attribute__((always_inline)) {
@@ -503,7 +591,14 @@ __device__ __forceinline__ void run_shared(const PagedAttnArgs& a, const ItemVie
             }
             __syncthreads();
         };
-        fill(c0, bases_of(c0), s_a);
+        lds_ops_barrier();  // the table's and the tiles' last readers are done
+        fill(c0, base_in(a, v, own_key, own_page), s_a);
+#pragma unroll
+        for (int u = 0; u < OWN; ++u) {
+            const uint32_t i = threadIdx.x + u * kPaThreads;
+            if (i < n) s_tab[i] = base_in(a, v, entry_key(v, c0, i), page[u]);
+        }
+        lds_ops_barrier();
         uint2 bases = bases_of(c0 + TILES);
         land(c0, s_a);
         // The step from tile t out of `cur` while the next streams into `nxt`,
@@ -518,7 +613,7 @@ __device__ __forceinline__ void run_shared(const PagedAttnArgs& a, const ItemVie
             const uint32_t k0 = v.src.key0(t + my_tile) + my_row;
             const uint16_t* const kb = cur + P::TILE * my_tile + D * my_row;
             if (live && (TILES == 1 || t + my_tile < c1) && !rv.none(k0, k0 + KEYS - 1))
-                tile<D, NB>(s, kb, kb + 64 * D, k_off, v_off, qf, rv, k0, v.src.key_end, scale_log2, lane, a.flags);
+                tile<D, NB>(s, kb, kb + 64 * D, k_off, v_off, qf, rv, k0, v.src.key_end, scale_log2, lane, bad);
             land(t + TILES, nxt);
         };
         for (uint32_t t = c0; t < c1; t += 2 * TILES) {
@@ -526,7 +621,8 @@ __device__ __forceinline__ void run_shared(const PagedAttnArgs& a, const ItemVie
             if (t + TILES < c1) step(t + TILES, s_b, s_a);
         }
     }
-    finish<D, RB, KS>(a, v, s, s_a, s_b, s_ml, wave, lane);
+    if (bad) arguments().flags[0] = 1;
+    finish<D, RB, KS>(arguments(), v, s, s_a, s_b, s_ml, wave, lane);
 }
 
 // Operand reads of the streaming form, in asm: to the compiler they are no LDS
@@ -658,13 +754,6 @@ struct PlanHead {
     }
 };
 
-// What the workgroup runs next, in LDS: an item or, of a streamed one, as many
-// of its tiles as a table holds.
-constexpr uint32_t kSegEntries = kTabEntries / 2;
-struct Segment {
-    PagedItem it;      // tile_end is the segment's; the item's is below
-    uint32_t kvh, kind, item_end, opens;
-};
 enum : uint32_t { kSegNone = 0, kSegStream = 1, kSegShared = 2 };
 
 // By one wave: `it` of KV head `kvh` from tile `from` on as a segment, with the
@@ -674,8 +763,11 @@ __device__ __forceinline__ void stage(const PagedAttnArgs& a, ItemView& v, Paged
                                       Segment* seg, uint2* tab, uint16_t* q) {
     const uint32_t lane = threadIdx.x & 63;
     const bool opens = from == it.tile_begin;
-    const uint32_t item_end = it.tile_end;
+    const uint32_t item_end = it.tile_end, ahead = it.row0 / v.group;
     point_at(v, a, it, kvh);
+    v.token = it.token0 + ahead;
+    v.head = it.row0 - ahead * v.group;
+    v.pos = it.pos0 + (int32_t)ahead;
     uint32_t kind = kSegShared;
     if (it.rows <= 32) {
         kind = kSegStream;
@@ -685,13 +777,15 @@ __device__ __forceinline__ void stage(const PagedAttnArgs& a, ItemView& v, Paged
         if (opens) {
             constexpr uint32_t CPR = D / 8;
             for (uint32_t i = lane; i < it.rows * CPR; i += 64) {
-                const uint32_t row = i / CPR, c = i % CPR, r = it.row0 + row;
-                const uint32_t token = it.token0 + r / v.group, head = kvh * v.group + r % v.group;
+                const uint32_t row = i / CPR, c = i % CPR;
                 *reinterpret_cast<uint4*>(q + row * D + 8 * (c ^ pk_swz<D>(row))) =
-                    ldg16(a.q + ((uint64_t)token * a.head.hq + head) * D + 8 * c);
+                    ldg16(a.q + row_of(a, v, row) * D + 8 * c);
             }
         }
-        fill_table(a, v, tab, it.tile_begin, it.tile_end, lane, 64);
+        for (uint32_t i = lane; i < (it.tile_end - it.tile_begin) << per_shift; i += 64) {
+            const uint32_t key = entry_key(v, it.tile_begin, i);
+            tab[i] = base_in(a, v, key, page_of(a, v, key));
+        }
     }
     if (lane == 0) {
         Segment s;
@@ -700,6 +794,10 @@ __device__ __forceinline__ void stage(const PagedAttnArgs& a, ItemView& v, Paged
         s.kind = kind;
         s.item_end = item_end;
         s.opens = opens;
+        s.token = v.token;
+        s.head = v.head;
+        s.pos = v.pos;
+        s.pad = 0;
         *seg = s;
     }
 }
@@ -742,10 +840,6 @@ __device__ __forceinline__ void advance(const PagedAttnArgs& a, ItemView& v, con
     }
     if (lane == 0) seg->kind = kSegNone;
 }
-
-// Workgroup barrier that waits for this wave's LDS operations only and leaves
-// its loads in flight.
-__device__ __forceinline__ void lds_ops_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Up to 32 rows: wave w < kStreams streams the 32-key halves w, w + kStreams,
 // ... of a segment's tiles, and on into the next segment, which wave kStreams
@@ -876,7 +970,7 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
         while (true) {
             const Segment seg = segment(slot);
             if (seg.kind != kSegStream) return slot;
-            point_at(v, a, seg.it, seg.kvh);
+            point_at(v, a, seg);
             const bool closes = seg.it.tile_end == seg.item_end;
             if (wave == kStreams) {
                 const uint32_t to = slot ^ 1;
@@ -900,12 +994,12 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
     while (true) {
         const Segment seg = segment(slot);
         if (seg.kind != kSegStream) return slot;
-        point_at(v, a, seg.it, seg.kvh);
+        point_at(v, a, seg);
         const bool closes = seg.it.tile_end == seg.item_end;
         bool next_has = false;
         const uint32_t last_row = seg.it.rows - 1, row = min((uint32_t)ql, last_row);
-        rv.pos = seg.it.pos0 + (int32_t)((seg.it.row0 + row) / v.group);
-        rv.span(seg.it.pos0 + (int32_t)(seg.it.row0 / v.group), seg.it.pos0 + (int32_t)((seg.it.row0 + last_row) / v.group));
+        rv.pos = v.pos + (int32_t)tokens_on(v, row);
+        rv.span(v.pos, v.pos + (int32_t)__builtin_amdgcn_readfirstlane(tokens_on(v, last_row)));
         const uint32_t c0 = seg.it.tile_begin, end = end_of(seg.it);
         uint32_t h = 2 * c0 + wave;
         const uint32_t n = h < end ? (end - h + kStreams - 1) / kStreams : 0;
@@ -1032,6 +1126,7 @@ __global__ __launch_bounds__(kPaThreads, 1) void paged_attn_kernel(PagedAttnArgs
     rv.sinks = a.head.window ? a.head.sinks : 0;
     ItemView v{};
     v.group = a.head.hq / hkv;
+    v.inv_group = 1.0f / (float)v.group;
     v.src.page_shift = 31 - __builtin_clz(a.head.page_size);
     v.src.entry_shift = min(v.src.page_shift, 6u);
     v.src.row_bytes = hkv * D * 2;
@@ -1048,7 +1143,7 @@ __global__ __launch_bounds__(kPaThreads, 1) void paged_attn_kernel(PagedAttnArgs
     __syncthreads();
     while (s_seg[slot].kind != kSegNone) {
         if (s_seg[slot].kind == kSegStream) {
-            slot = run_streams<D>(a, v, head, slot, s_seg, s_a, s_b, s_tab, s_q, s_ml, scale_log2, rv);
+            slot = run_streams<D>(arguments(), v, head, slot, s_seg, s_a, s_b, s_tab, s_q, s_ml, scale_log2, rv);
             continue;
         }
         Segment seg;
@@ -1059,24 +1154,24 @@ __global__ __launch_bounds__(kPaThreads, 1) void paged_attn_kernel(PagedAttnArgs
                 w[i] = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t*>(s_seg + slot)[i]);
             __builtin_memcpy(&seg, w, sizeof(seg));
         }
-        point_at(v, a, seg.it, seg.kvh);
+        point_at(v, a, seg);
         // A ticket for the list after this one, drawn now and looked at below.
         const bool draws = head.ranges > lanes && seg.it.next == kPagedNone;
         uint32_t ticket = 0;
         if (draws && threadIdx.x == 0) ticket = atomicAdd(a.tickets + seg.kvh, 1u);
         if (v.it.rows > 128)
-            run_shared<D, 8>(a, v, s_a, s_b, s_tab, s_ml, scale_log2, rv);
+            run_shared<D, 8>(arguments(), v, s_a, s_b, s_tab, s_ml, scale_log2, rv);
         else if (v.it.rows > 64)
-            run_shared<D, 4>(a, v, s_a, s_b, s_tab, s_ml, scale_log2, rv);
+            run_shared<D, 4>(arguments(), v, s_a, s_b, s_tab, s_ml, scale_log2, rv);
         else
-            run_shared<D, 2>(a, v, s_a, s_b, s_tab, s_ml, scale_log2, rv);
-        __syncthreads();  // every wave is done with the tiles
+            run_shared<D, 2>(arguments(), v, s_a, s_b, s_tab, s_ml, scale_log2, rv);
+        lds_ops_barrier();  // every wave is done with the tiles (its stores may still be under way)
         if (wave == 0) {
             ItemView w = v;
-            advance<D>(a, w, head, seg.it, seg.kvh, draws, ticket, s_seg, s_tab, s_q);
+            advance<D>(arguments(), w, head, seg.it, seg.kvh, draws, ticket, s_seg, s_tab, s_q);
         }
         slot = 0;
-        __syncthreads();
+        lds_ops_barrier();
     }
 }
 

@@ -22,7 +22,7 @@
 //   a prompt of 512            16* / 23      20 / 23      26 / 28
 //   a prompt of 2048           76 / 83       66* / 73     64 / 70
 //   a prompt of 8192          757 / 800     587 / 662    533* / 580
-//   33 decoded and 5 chunks   182 / 211     156 / 174    181 / 158*
+//   30 decoded and 5 chunks   182 / 211     156 / 174    181 / 158*
 // (32 rows: 201 for the first and 1494 for the fourth.)
 //
 // Costs are in units of about 0.12 us of a lane.  A 64-key tile takes its
