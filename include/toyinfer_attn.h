@@ -379,8 +379,8 @@ int toyinfer_sample_topk_topp_f32(const float* logits, uint32_t vocab, float tem
  * new token is one row of q, k, v and o, the requests' rows back to back from
  * row 0 in request order.
  * Limits: batch <= TOYINFER_PAGED_MAX_BATCH; num_tokens * Hq/Hkv < 2^31;
- * max_blocks * page_size < 2^31; num_pages * page_size < 2^32
- * (TOYINFER_ERR_UNSUPPORTED beyond). */
+ * max_blocks * page_size < 2^31; num_pages * page_size < 2^32; page_stride < 2^40,
+ * (num_pages - 1) * page_stride <= 2^46 (TOYINFER_ERR_UNSUPPORTED beyond). */
 #define TOYINFER_PAGED_MAX_BATCH 4096u
 
 /* Block tables, positions and slots of one step from the requests' lengths:
@@ -397,8 +397,8 @@ int toyinfer_sample_topk_topp_f32(const float* logits, uint32_t vocab, float tem
  * A request is refused whose pages the stack does not hold after the requests
  * before it (refused ones counted), whose row would pass max_blocks or whose
  * token rows would pass num_tokens: it takes no page, seq_lens[b] =
- * context_lens[b], and its token rows get slot 0xFFFFFFFF.  Token rows past the
- * last request's get position 0 and slot 0xFFFFFFFF.  *num_free counts at most
+ * context_lens[b], and its token rows get slot 0xFFFFFFFF (what the attention
+ * gives them is of no use).  Token rows past the last request's get position 0 and slot 0xFFFFFFFF.  *num_free counts at most
  * free_capacity pages.  No output may overlap an input or another output. */
 int toyinfer_paged_tables_u32(const uint32_t* context_lens, const uint32_t* new_lens,
                               uint32_t batch, const uint32_t* free_pages, uint32_t free_capacity,

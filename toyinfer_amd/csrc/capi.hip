@@ -789,7 +789,8 @@ static int check_caches(const void* k_cache, const void* v_cache, uint32_t num_p
     if (!aligned(k_cache, 16) || !aligned(v_cache, 16)) return TOYINFER_ERR_INVALID_ARGUMENT;
     const uint64_t page = (uint64_t)page_size * hkv * d;
     if (page_stride < page || page_stride % 8 != 0) return TOYINFER_ERR_INVALID_ARGUMENT;
-    if ((uint64_t)num_pages * page_size >= (1ull << 32) || page_stride >= (1ull << 40))
+    if ((uint64_t)num_pages * page_size >= (1ull << 32) || page_stride >= (1ull << 40) ||
+        num_pages - 1 > (1ull << 46) / page_stride)  // more than 2^47 bytes: no memory holds it
         return TOYINFER_ERR_UNSUPPORTED;
     *bytes = 2 * ((num_pages - 1) * page_stride + page);
     // Pages of one cache may lie between pages of the other, not on them.
