@@ -70,10 +70,10 @@ inline __host__ __device__ uint32_t paged_lanes(uint32_t hkv) {
     return hkv >= kPagedSlots ? 1 : kPagedSlots / hkv;
 }
 // A plan of cut units has up to kPagedLevels ranges per lane, one with units of
-// 256 rows, two with 128.  A cut leaves two pieces of its unit, so per KV head
-// the workspace holds this many 32-row blocks of partial results, and the plan
-// half as many blocks that are in pieces.
-constexpr uint32_t kPagedLevels = 4;
+// 256 rows.  A cut leaves two pieces of its unit, so per KV head the workspace
+// holds this many 32-row blocks of partial results, and the plan half as many
+// blocks that are in pieces.
+constexpr uint32_t kPagedLevels = 2;
 inline __host__ __device__ uint32_t paged_partial_blocks(uint32_t hkv) {
     return 2 * (kPagedMaxRows / kPagedBlockRows) * paged_lanes(hkv);
 }

@@ -5,14 +5,17 @@
 // they are cut into units of up to 32, 64, 128 or 256 rows that walk the request's
 // key tiles together.  Larger units read each key tile for more rows, smaller
 // ones spread better over the lanes (a lane: a workgroup of the attention
-// kernel).  The lanes draw lists of items as they come free, for their speeds
-// differ: of two workgroups of a compute unit the older is served first (64
-// requests of 4096 keys, one equal share per lane: 130 and 160 us), and the dies
-// reach memory unequally.  Either
-// * a list is a whole unit, longest first, or
-// * the units' tiles laid end to end are cut into ranges, of most of a lane's
-//   even share first, then of smaller parts of it.  A unit with a cut inside
+// kernel).  Either
+// * each unit is a list, longest first, and the lanes draw lists as they come
+//   free, or
+// * the units' tiles laid end to end are cut into ranges, one per lane of its even
+//   share; or, with units of 64 or 128 rows, of 7/8 of it, and as many of 1/8 that
+//   the lanes draw afterwards, for their speeds differ.  A unit with a cut inside
 //   leaves partial results of each piece, merged by a second kernel.
+// Streamed requests take even shares only: every range more is a piece more to
+// start and merge (32 requests of 8192 keys 167 us, 179 with the two ranges and
+// 180 with whole requests; mixed batches with units of 128 rows are 1 to 7 %
+// faster with the two).
 // The size and the way are those with the shortest estimate: rounds of whole
 // units times their mean, or the longest of them, against the even share plus
 // the pieces' overhead.  Forced ones took, in us, at 32 query and 8 KV heads of
@@ -45,7 +48,7 @@ constexpr uint32_t kStreamItem = 24, kSharedItem = 80;  // starting and finishin
 constexpr uint32_t kPieceTiles = 2;  // cuts lie on multiples of it, one 32-key half per wave
 constexpr uint32_t kLocalUnits = 2048;
 constexpr uint32_t kSizes = 4;         // of units: 32, 64, 128 or 256 rows
-constexpr uint32_t kLevelShare = 800;  // a lane's share from which its ranges shrink by level
+constexpr uint32_t kTwoRanges = 500;   // a lane's share from which it is in two ranges
 
 // x of the lane that a DPP control names, 0 where there is none.
 template <int CTRL, int ROWS = 0xf>
@@ -164,7 +167,7 @@ __device__ __forceinline__ Estimate estimate(uint32_t U, uint64_t work, uint64_t
                                              uint32_t rows, uint32_t lanes) {
     const uint64_t share = work / lanes;
     Estimate e;
-    e.levels = share >= kLevelShare ? min(kPagedLevels, kPagedMaxRows / rows) : 1;
+    e.levels = (rows == 64 || rows == 128) && share >= kTwoRanges ? kPagedLevels : 1;
     const uint64_t rounds = U ? (uint64_t)((U + lanes - 1) / lanes) * work / U : 0;
     e.whole = max(longest, rounds) + (rows == 32 ? longest / 4 : 0);
     // A cut costs a lane another item and its piece's results (half a unit per
@@ -175,11 +178,8 @@ __device__ __forceinline__ Estimate estimate(uint32_t U, uint64_t work, uint64_t
     return e;
 }
 
-// Sizes of the ranges of level v of `levels`, in parts of a lane's share.
-constexpr uint32_t kParts = 16;
-__device__ __forceinline__ uint32_t level_parts(uint32_t v, uint32_t levels) {
-    return levels == 1 ? kParts : levels == 2 ? (v ? 2 : 14) : levels == 3 ? (v ? 1 : 14) : v == 0 ? 12 : v == 1 ? 2 : 1;
-}
+// Sizes of a lane's ranges, in parts of its share.
+constexpr uint32_t kParts = 16, kFirstParts = 14;
 
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs a) {
     constexpr uint32_t kBuckets = kPlanThreads;
@@ -383,15 +383,12 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
         }
         if (tid < lanes && tid >= U) items[tid].rows = 0;
     } else {
-        // Cut r: the start of range r, its unit and the tile in it.  Ranges of
-        // level v, one per lane, are 1/2, 1/4, ... of the share, the last two
-        // levels alike.
+        // Cut r: the start of range r, its unit and the tile in it.
         ranges = levels * lanes;
         for (uint32_t r = tid; r <= ranges; r += kPlanThreads) {
             const uint32_t level = r / lanes, nth = r % lanes;
-            const uint32_t size = levels == 1 ? kParts : level_parts(level, levels);
-            uint32_t before = level >= levels ? kParts : 0;
-            for (uint32_t v = 0; v < level && level < levels; ++v) before += level_parts(v, levels);
+            const uint32_t before = level >= levels ? kParts : level ? kFirstParts : 0;
+            const uint32_t size = (levels == 1 || level ? kParts : kFirstParts) - before;
             const uint64_t x = work * ((uint64_t)before * lanes + (uint64_t)size * nth) / ((uint64_t)kParts * lanes);
             uint32_t i = r == ranges ? U : last_at_most(cost, U, x), t = 0;
             if (i < U) {
