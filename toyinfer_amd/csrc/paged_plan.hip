@@ -188,6 +188,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
     __shared__ uint64_t s_cost[kLocalUnits + 1];       // cost of the units before each
     __shared__ uint32_t s_cut_unit[kPagedLevels * kPagedSlots + 1], s_cut_tile[kPagedLevels * kPagedSlots + 1];
     __shared__ uint32_t s_item[kPagedLevels * kPagedSlots + 1];  // first item of each range
+    __shared__ PagedItem s_unit[kPlanThreads];  // the first units, as in the plan
     __shared__ uint32_t s_bucket[kBuckets];
     __shared__ uint64_t s_work[kPlanWaves][kSizes];
     __shared__ uint32_t s_units[kPlanWaves][kSizes], s_long[kPlanWaves][kSizes], s_most[kPlanWaves];
@@ -342,6 +343,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
             const uint32_t per_tile = rows <= 32 ? stream_tile : product_cost(u.rows, a.head.d);
             u.next = per_tile;  // (here; the items' own below)
             units[i] = u;
+            if (i < kPlanThreads) s_unit[i] = u;
             c = (uint64_t)u.tile_end * per_tile + item_cost(u.rows);
             longest = max(longest, (uint32_t)c);
         }
@@ -356,6 +358,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
 #pragma unroll
     for (int w = 0; w < kPlanWaves; ++w) longest = max(longest, s_long[w][0]);
 
+    auto unit = [&](uint32_t i) -> PagedItem { return i < kPlanThreads ? s_unit[i] : units[i]; };
     const Estimate e = estimate(U, work, longest, streamed, unit_rows, lanes);
     const uint32_t levels = e.levels;
     uint32_t n_items = U, split_blocks = 0, ranges = max(U, lanes);
@@ -368,7 +371,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
                 const uint32_t q = (uint32_t)((float)(cost[i + 1] - cost[i]) * to_bucket);
                 const uint32_t bucket = kBuckets - 1 - min(kBuckets - 1, q), at = atomicAdd(&s_bucket[bucket], 1u);
                 if (pass == 1) {
-                    PagedItem u = units[i];
+                    PagedItem u = unit(i);
                     u.next = kPagedNone;
                     items[at] = u;
                 }
@@ -392,7 +395,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
             const uint64_t x = work * ((uint64_t)before * lanes + (uint64_t)size * nth) / ((uint64_t)kParts * lanes);
             uint32_t i = r == ranges ? U : last_at_most(cost, U, x), t = 0;
             if (i < U) {
-                const uint32_t tiles = units[i].tile_end, per_tile = units[i].next, item = item_cost(units[i].rows);
+                const PagedItem u = unit(i);
+                const uint32_t tiles = u.tile_end, per_tile = u.next, item = item_cost(u.rows);
                 const uint64_t off = x - cost[i];
                 if (off > item)
                     t = (uint32_t)((off - item + per_tile * kPieceTiles / 2) / (per_tile * kPieceTiles)) * kPieceTiles;
@@ -428,7 +432,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
             if (j < n_items) {
                 r = last_at_most(s_item, ranges, j);
                 i = s_cut_unit[r] + (j - s_item[r]);
-                u = units[i];
+                u = unit(i);
                 const uint32_t tiles = u.tile_end;
                 if (j == s_item[r]) u.tile_begin = s_cut_tile[r];
                 if (i == s_cut_unit[r + 1]) u.tile_end = s_cut_tile[r + 1];
@@ -436,10 +440,11 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
                 u.next = j + 1 < s_item[r + 1] ? ranges + j + 1 : kPagedNone;
             }
             const bool opens = nb && u.tile_begin == 0;
-            const uint32_t first = blocks + block_scan(nb, &sum);
-            blocks += sum;
-            const uint32_t sb = split_blocks + block_scan(opens ? nb : 0u, &sum);
-            split_blocks += sum;
+            // Two sums in one: each stays below 2^16 (paged_partial_blocks).
+            const uint32_t at = block_scan(nb | (opens ? nb << 16 : 0u), &sum);
+            const uint32_t first = blocks + (at & 0xffffu), sb = split_blocks + (at >> 16);
+            blocks += sum & 0xffffu;
+            split_blocks += sum >> 16;
             if (j < n_items) {
                 if (nb) u.partial = first;
                 items[j == s_item[r] ? r : ranges + j] = u;
