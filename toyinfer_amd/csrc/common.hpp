@@ -217,4 +217,36 @@ __device__ __forceinline__ f32x4_t mfma16x16x32(bf16x8_t a, bf16x8_t b, f32x4_t 
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
+// ------------------------------------------------------- scans of a wave
+// x of the lane that a DPP control names, 0 where there is none.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t lane_from(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint64_t lane_from(uint64_t x) {
+    return (uint64_t)lane_from<CTRL, ROWS>((uint32_t)(x >> 32)) << 32 | lane_from<CTRL, ROWS>((uint32_t)x);
+}
+// Inclusive over the wave's lanes: rows of 16 first, then the last lane of a
+// row into the next, then of the lower half into the upper.  (By shuffles
+// through LDS the scans and sums of the paged attention's plan took 3 us longer.)
+template <typename T, typename F>
+__device__ __forceinline__ T wave_scan(T x, F op) {
+    x = op(x, lane_from<0x111>(x));
+    x = op(x, lane_from<0x112>(x));
+    x = op(x, lane_from<0x114>(x));
+    x = op(x, lane_from<0x118>(x));
+    x = op(x, lane_from<0x142, 0xa>(x));
+    return op(x, lane_from<0x143, 0xc>(x));
+}
+struct Sum {
+    template <typename T>
+    __device__ __forceinline__ T operator()(T x, T y) const {
+        return x + y;
+    }
+};
+struct Max {
+    __device__ __forceinline__ uint32_t operator()(uint32_t x, uint32_t y) const { return max(x, y); }
+};
+
 }  // namespace tiattn

@@ -50,37 +50,6 @@ constexpr uint32_t kLocalUnits = 2048;
 constexpr uint32_t kSizes = 4;         // of units: 32, 64, 128 or 256 rows
 constexpr uint32_t kTwoRanges = 500;   // a lane's share from which it is in two ranges
 
-// x of the lane that a DPP control names, 0 where there is none.
-template <int CTRL, int ROWS = 0xf>
-__device__ __forceinline__ uint32_t from(uint32_t x) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
-}
-template <int CTRL, int ROWS = 0xf>
-__device__ __forceinline__ uint64_t from(uint64_t x) {
-    return (uint64_t)from<CTRL, ROWS>((uint32_t)(x >> 32)) << 32 | from<CTRL, ROWS>((uint32_t)x);
-}
-// Inclusive over the wave's lanes: rows of 16 first, then the last lane of a
-// row into the next, then of the lower half into the upper.  (By shuffles
-// through LDS the kernel's scans and sums took 3 us longer.)
-template <typename T, typename F>
-__device__ __forceinline__ T wave_scan(T x, F op) {
-    x = op(x, from<0x111>(x));
-    x = op(x, from<0x112>(x));
-    x = op(x, from<0x114>(x));
-    x = op(x, from<0x118>(x));
-    x = op(x, from<0x142, 0xa>(x));
-    return op(x, from<0x143, 0xc>(x));
-}
-struct Sum {
-    template <typename T>
-    __device__ __forceinline__ T operator()(T x, T y) const {
-        return x + y;
-    }
-};
-struct Max {
-    __device__ __forceinline__ uint32_t operator()(uint32_t x, uint32_t y) const { return max(x, y); }
-};
-
 // Exclusive sums over the workgroup's threads in thread order, total in *sum.
 template <typename T>
 __device__ __forceinline__ T block_scan(T x, T* sum) {

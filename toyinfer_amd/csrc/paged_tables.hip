@@ -33,15 +33,7 @@ __device__ __forceinline__ void block_scan2(uint64_t& a, uint64_t& b, uint64_t* 
     constexpr int NW = kTabThreads / 64;
     __shared__ uint64_t s_tot[NW][2];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint64_t ia = a, ib = b;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const uint64_t ua = __shfl_up(ia, m), ub = __shfl_up(ib, m);
-        if (lane >= m) {
-            ia += ua;
-            ib += ub;
-        }
-    }
+    const uint64_t ia = wave_scan(a, Sum{}), ib = wave_scan(b, Sum{});
     if (lane == 63) {
         s_tot[wave][0] = ia;
         s_tot[wave][1] = ib;
@@ -103,18 +95,17 @@ __global__ __launch_bounds__(kTabThreads) void paged_tables_kernel(PagedTablesAr
     if (blockIdx.x == 0) {
         // Accepted requests that need pages are a prefix of those that do, so
         // the pages taken are the largest end among them.
-        __shared__ uint64_t s_taken[kTabThreads];
-        s_taken[tid] = taken;
-        __syncthreads();
-        for (int m = kTabThreads / 2; m >= 1; m >>= 1) {
-            if (tid < (uint32_t)m) s_taken[tid] = max(s_taken[tid], s_taken[tid + m]);
-            __syncthreads();
-        }
+        __shared__ uint32_t s_taken[kTabThreads / 64];
+        const uint32_t most = wave_scan((uint32_t)taken, Max{});
+        if ((tid & 63) == 63) s_taken[tid >> 6] = most;
         uint64_t unused = 0, sum_r, sum_u;
         block_scan2(refused, unused, &sum_r, &sum_u);
         if (tid == 0) {
             a.query_start[a.batch] = clamp32(tokens);
-            a.status[0] = num_free - (uint32_t)s_taken[0];
+            uint32_t all = 0;
+#pragma unroll
+            for (int w = 0; w < kTabThreads / 64; ++w) all = max(all, s_taken[w]);
+            a.status[0] = num_free - all;
             a.status[1] = (uint32_t)sum_r;
         }
     }
@@ -160,21 +151,11 @@ __global__ __launch_bounds__(kTabThreads) void paged_tables_kernel(PagedTablesAr
     }
 }
 
-// Each input row is read once and each output row written once here, so both
-// bypass the caches' retention: 8192 tokens of 32 + 2 * 8 heads 40.2 -> 36.7 us
-// (5.5 TB/s, the rate of a large copy), 1371 tokens 7.0 -> 5.3.
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ uint4 load_once16(const uint16_t* p) {
-    const u32x4_t x = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
-    return make_uint4(x.x, x.y, x.z, x.w);
-}
-__device__ __forceinline__ void store_once16(uint16_t* p, uint4 x) {
-    __builtin_nontemporal_store(u32x4_t{x.x, x.y, x.z, x.w}, reinterpret_cast<u32x4_t*>(p));
-}
-
 // D / 16 lanes per row, lane c the eight pairs (8c + k, 8c + k + D/2); U rows
 // per lane group, so that a position's angles and the weights are read once
-// for U rows.
+// for U rows.  Each input row is read once and each output row written once, and
+// both bypass the caches' retention: 8192 tokens of 32 + 2 * 8 heads 40.2 -> 36.7 us
+// (5.5 TB/s, the rate of a large copy), 1371 tokens 7.0 -> 5.3.
 template <int D, int U>
 __global__ __launch_bounds__(256) void paged_prologue_kernel(PagedPrologueArgs a, uint32_t parts) {
     constexpr int LPR = D / 16, G = 64 / LPR, HALF = D / 2;
@@ -193,8 +174,8 @@ __global__ __launch_bounds__(256) void paged_prologue_kernel(PagedPrologueArgs a
         const uint16_t* src = j < a.hq           ? a.q + ((uint64_t)t * a.hq + j) * D
                               : j < a.hq + a.hkv ? a.k + ((uint64_t)t * a.hkv + (j - a.hq)) * D
                                                  : a.v + ((uint64_t)t * a.hkv + (j - a.hq - a.hkv)) * D;
-        xr[u] = load_once16(src + 8 * c);
-        xi[u] = load_once16(src + 8 * c + HALF);
+        xr[u] = ldg16_nt(src + 8 * c);
+        xi[u] = ldg16_nt(src + 8 * c + HALF);
     }
     const uint4 qwr = ldg16(a.q_weight + 8 * c), qwi = ldg16(a.q_weight + 8 * c + HALF);
     const uint4 kwr = ldg16(a.k_weight + 8 * c), kwi = ldg16(a.k_weight + 8 * c + HALF);
@@ -246,8 +227,8 @@ __global__ __launch_bounds__(256) void paged_prologue_kernel(PagedPrologueArgs a
             dst = j < a.hq + a.hkv ? a.k_cache + cache_row + (uint64_t)(j - a.hq) * D
                                    : a.v_cache + cache_row + (uint64_t)(j - a.hq - a.hkv) * D;
         if (dst) {
-            store_once16(dst + 8 * c, xr[u]);
-            store_once16(dst + 8 * c + HALF, xi[u]);
+            stg16_nt(dst + 8 * c, xr[u]);
+            stg16_nt(dst + 8 * c + HALF, xi[u]);
         }
     }
 }
