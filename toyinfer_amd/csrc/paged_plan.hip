@@ -21,15 +21,15 @@
 // the pieces' overhead.  Forced ones took, in us, at 32 query and 8 KV heads of
 // 128 (w whole, c cut, * the choice):
 //                              64 w / c     128 w / c    256 w / c rows
-//   512 tokens on 8192 keys    93 / 123     119 / 87*    204 / 83
+//   512 tokens on 8192 keys    93 / 123     119 / 82*    204 / 83
 //   a prompt of 512            16* / 23      20 / 23      26 / 28
 //   a prompt of 2048           76 / 83       66* / 73     64 / 70
 //   a prompt of 8192          757 / 800     587 / 662    533* / 580
 //   30 decoded and 5 chunks   182 / 211     156 / 174    181 / 158*
 // (32 rows: 201 for the first and 1494 for the fourth.)
 //
-// One workgroup, because each phase needs the sums of the one before: 12 us for
-// 32 requests, 20 for 1000, once per step; half of it are waits for memory and
+// One workgroup, because each phase needs the sums of the one before: 9.4 us for
+// 32 requests, 15.7 for 1000, once per step; half of it are waits for memory and
 // between phases.
 //
 // Costs are in units of about 0.12 us of a lane.  A 64-key tile takes its
