@@ -113,6 +113,19 @@ def test_head_layouts(dev, hq, hkv, d, requests):
     Wide(dev, requests, hq, hkv, d, 16, seed=hq).run()
 
 
+@pytest.mark.parametrize("hq,hkv,d,requests", [
+    (25, 5, 128, [(2042, 373)]),                              # a last unit of 73 rows
+    *[(8, 8, 128, [(6000, n)]) for n in (70, 96, 129, 160, 170, 200, 224)],
+    (8, 8, 64, [(5000, 140), (3000, 200), (4000, 90)]),
+    (16, 8, 128, [(7000, 300), (100, 1), (3000, 70)]),
+])
+def test_pieces_of_units_with_idle_waves(dev, hq, hkv, d, requests):
+    """A split unit of fewer rows than its form's waves hold: the idle waves
+    leave the next piece's results alone."""
+    print(f"[paged] idle waves {hq}/{hkv} D={d} {requests}", flush=True)
+    Wide(dev, requests, hq, hkv, d, 16, seed=hq).run()
+
+
 @pytest.mark.parametrize("window,sinks", [(0, 0), (9000, 100)])
 @pytest.mark.parametrize("ps", [8, 64])
 def test_long_contexts(dev, ps, window, sinks):

@@ -411,7 +411,8 @@ __device__ __forceinline__ void put(const PagedAttnArgs& a, const ItemView& v, u
 }
 __device__ __forceinline__ void put_ml(const PagedAttnArgs& a, const ItemView& v, uint32_t row_block, int lane,
                                        float m, float l) {
-    if (v.it.partial == kPagedWhole || lane >= 32) return;
+    // (The block behind the unit's last is another piece's.)
+    if (v.it.partial == kPagedWhole || lane >= 32 || row_block * kPagedBlockRows >= v.it.rows) return;
     const uint64_t blk = (uint64_t)v.kvh * paged_partial_blocks(a.head.hkv) + v.it.partial + row_block;
     a.part_ml[blk * kPagedBlockRows + lane] = make_float2(m, l);
 }
