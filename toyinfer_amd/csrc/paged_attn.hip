@@ -718,18 +718,19 @@ __device__ __forceinline__ void read_v(uint4 (&v)[2][4], uint32_t at) {
 __device__ __forceinline__ void read_v(uint4 (&v)[2][2], uint32_t at) {
     typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
     u2_t r[8];
+    constexpr int kRows8 = 8 * 64 * 2;  // bytes of eight rows
     asm volatile(
         "ds_read_b64_tr_b16 %0, %8\n\t"
-        "ds_read_b64_tr_b16 %1, %8 offset:1024\n\t"
-        "ds_read_b64_tr_b16 %2, %8 offset:2048\n\t"
-        "ds_read_b64_tr_b16 %3, %8 offset:3072\n\t"
+        "ds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
+        "ds_read_b64_tr_b16 %2, %8 offset:%11\n\t"
+        "ds_read_b64_tr_b16 %3, %8 offset:%12\n\t"
         "ds_read_b64_tr_b16 %4, %9\n\t"
-        "ds_read_b64_tr_b16 %5, %9 offset:1024\n\t"
-        "ds_read_b64_tr_b16 %6, %9 offset:2048\n\t"
-        "ds_read_b64_tr_b16 %7, %9 offset:3072\n\t"
+        "ds_read_b64_tr_b16 %5, %9 offset:%10\n\t"
+        "ds_read_b64_tr_b16 %6, %9 offset:%11\n\t"
+        "ds_read_b64_tr_b16 %7, %9 offset:%12\n\t"
         "s_waitcnt lgkmcnt(0)"
         : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
-        : "v"(at), "v"(at ^ 64)
+        : "v"(at), "v"(at ^ 64), "n"(kRows8), "n"(2 * kRows8), "n"(3 * kRows8)
         : "memory");
 #pragma unroll
     for (int tt = 0; tt < 2; ++tt)
