@@ -113,12 +113,11 @@ __device__ __forceinline__ PagedItem unit_of(const PagedPlanHeader& h, uint32_t 
     return u;
 }
 
-// A tile's products, by the unit's rows; its bytes' time where all lanes stream
-// at once.
-__device__ __forceinline__ uint32_t product_cost(uint32_t rows, uint32_t d) {
-    if (rows <= 32) return kStreamTile;
-    const uint32_t c = rows <= 64 ? 6 : rows <= 128 ? 9 : 17;
-    return d == 64 ? (2 * c + 2) / 3 : c;
+// A tile's products, by the unit's rows (at head_dim 64 less than at 128, but not
+// in a batch with streamed requests: with two thirds there, mixed ones took 7 to
+// 15 % longer); its bytes' time where all lanes stream at once.
+__device__ __forceinline__ uint32_t product_cost(uint32_t rows) {
+    return rows <= 32 ? kStreamTile : rows <= 64 ? 6 : rows <= 128 ? 9 : 17;
 }
 __device__ __forceinline__ uint32_t bytes_cost(uint32_t d) { return d == 64 ? 6 : 11; }
 // Of a request with up to 32 rows in a step that streams.
@@ -197,7 +196,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
             if (i <= top) {  // (at larger sizes the request is the same one unit)
                 const uint32_t R = 32u << i;
                 n = (rows + R - 1) >> (5 + i);
-                const uint32_t mid = n / 2 * R, last = (n - 1) * R, per_tile = product_cost(R, a.head.d);
+                const uint32_t mid = n / 2 * R, last = (n - 1) * R, per_tile = product_cost(R);
                 long_tiles = unit_of(a.head, b, r, group, last, min(R, rows - last)).tile_end;
                 mid_tiles = mid == last ? long_tiles : unit_of(a.head, b, r, group, mid, R).tile_end;
                 long_cost = long_tiles * per_tile + item_cost(R);
@@ -208,7 +207,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
             long_of[i] = max(long_of[i], long_cost);
         }
         bytes += mid_tiles * bytes_cost(a.head.d);
-        products += (uint64_t)n * mid_tiles * product_cost(32u << top, a.head.d);
+        products += (uint64_t)n * mid_tiles * product_cost(32u << top);
         if (top == 0) {
             ++streams;
             streamed += mid_tiles;
@@ -309,7 +308,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
             const Request r = s_req[b];
             const uint32_t rows = r.n * group, row0 = (i - s_first[b]) << (5 + size);
             PagedItem u = unit_of(a.head, b, r, group, row0, min(unit_rows, rows - row0));
-            const uint32_t per_tile = rows <= 32 ? stream_tile : product_cost(u.rows, a.head.d);
+            const uint32_t per_tile = rows <= 32 ? stream_tile : product_cost(u.rows);
             u.next = per_tile;  // (here; the items' own below)
             units[i] = u;
             if (i < kPlanThreads) s_unit[i] = u;
