@@ -29,7 +29,7 @@
 //   streaming, 32 requests of 2208..8193 keys (704 MB): 114 us, 6.2 TB/s of keys
 //     and values where a contiguous cache streams at 6.5; 64 KB of loads in flight per
 //     compute unit is what LDS leaves beside the merge;
-//   > 128 rows, a prompt of 8192: 511 us, 1.07 PFLOP/s; matrix cores busy for 49 %
+//   > 128 rows, a prompt of 8192: 511 to 522 us, 1.05 to 1.07 PFLOP/s; matrix cores busy for 49 %
 //     of the cycles, waves waiting for 29 %.  Lanes end up to 6 % from their mean; the
 //     contiguous prefill attention, without pages and lists, takes 480.
 // What a SIMD's two waves do is in step, from barrier to barrier.  Two groups of
