@@ -155,7 +155,9 @@ __global__ __launch_bounds__(kTabThreads) void paged_tables_kernel(PagedTablesAr
 // per lane group, so that a position's angles and the weights are read once
 // for U rows.  Each input row is read once and each output row written once, and
 // both bypass the caches' retention: 8192 tokens of 32 + 2 * 8 heads 40.2 -> 36.7 us
-// (5.5 TB/s, the rate of a large copy), 1371 tokens 7.0 -> 5.3.
+// (5.5 TB/s, the rate of a large copy), 1371 tokens 7.0 -> 5.3.  One row per lane
+// group is launched: two and four gave up to 2 % on 8192 tokens and cost a small call
+// 0.3 and 1.1 us of 2.5.
 template <int D, int U>
 __global__ __launch_bounds__(256) void paged_prologue_kernel(PagedPrologueArgs a, uint32_t parts) {
     constexpr int LPR = D / 16, G = 64 / LPR, HALF = D / 2;
