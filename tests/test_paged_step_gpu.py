@@ -379,3 +379,58 @@ def test_binding_refuses_on_the_gpu(dev):
     attend()
     H.sync()
     st.check()
+
+
+def test_no_new_tokens(dev):
+    """A step in which no request has a token: nothing is written."""
+    st = Step(dev, [(40, 0), (0, 0), (300, 0)], 8, 2, 128, 16)
+    st.run()
+    assert (st.o == 3.0).all() and not st.ws[:4 * (st.hkv + 2)].any()
+
+
+def test_graphs_that_share_a_workspace(dev):
+    """Two captured steps with one workspace, replayed in turn on one stream with
+    eager calls between, each with tickets, pieces and results of its own."""
+    one = Step(dev, [(700, 1), (300, 40), (900, 1)], 8, 2, 128, 16, seed=21)
+    two = Step(dev, [(3000, 1), (64, 64), (100, 5)], 8, 2, 128, 16, 70, 4, seed=22)
+    two.ws = one.ws
+    stream, graphs = torch.cuda.Stream(), []
+    for st in (one, two):
+        st.run()
+        graph = torch.cuda.CUDAGraph()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(graph, stream=stream):
+            st.make_plan(stream)
+            st.attend(stream)
+        graphs.append(graph)
+    for _ in range(3):
+        for st, graph in zip((one, two), graphs):
+            st.o.fill_(3.0)
+            graph.replay()
+        H.sync()
+        one.check()
+        two.check()
+        one.attend()
+        two.attend()
+        H.sync()
+        one.check()
+        two.check()
+
+
+def test_one_plan_on_two_streams(dev):
+    """Two layers' calls with one plan at a time on two streams, each with a
+    workspace of its own."""
+    st = Step(dev, [(3000, 1), (500, 120), (60, 3)], 16, 8, 64, 16, seed=23)
+    st.run()
+    ws = attn.paged_attention_workspace(st.hq, st.hkv, st.d, dev)
+    mine, other, first = st.o, torch.full_like(st.o, 3.0), st.o.clone()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    mine.fill_(3.0)
+    H.sync()
+    for _ in range(5):
+        for stream, o, w in zip(streams, (mine, other), (st.ws, ws)):
+            st.o, st.ws, keep = o, w, st.ws
+            st.attend(stream)
+            st.ws = keep
+    H.sync()
+    assert torch.equal(mine, first) and torch.equal(other, first)
