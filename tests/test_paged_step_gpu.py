@@ -434,3 +434,44 @@ def test_one_plan_on_two_streams(dev):
             st.ws = keep
     H.sync()
     assert torch.equal(mine, first) and torch.equal(other, first)
+
+
+class Early(Wide):
+    """Requests with more new tokens than keys: rows before position 0 give 0,
+    the others are as many tokens as keys."""
+
+    def check(self, got=None):
+        got = self.o if got is None else got
+        assert (got[self.total:] == 3.0).all(), "rows behind the last request were written"
+        for b, (length, new) in enumerate(self.requests):
+            zero, first, end = int(self.start[b]), int(self.start[b]) + max(0, new - length), int(self.start[b + 1])
+            assert (got[zero:first] == 0).all(), (b, "rows before position 0")
+            if first < end:
+                k, v = (x.to(self.dev) for x in self.kv[b])
+                check_rows(got[first:end], self.q_d[first:end], k, v, self.window, self.sinks, b)
+
+
+# With no window in forms of 32, 64, 128 (two) and 256 rows, the last in pieces.
+EARLY = [
+    (32, 8, 128, [(50, 100)]),
+    (8, 8, 64, [(3005, 4096)]),
+    (32, 8, 128, [(901, 1024)]),
+    (64, 64, 64, [(30, 64), (71, 128), (1, 40), (9, 13)]),
+    (32, 8, 128, [(53 - i, 100) for i in range(12)]),
+    (8, 1, 128, [(9000, 1), (299, 2000), (5, 12)]),
+]
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (37, 2), (0x7FFFFFFE, 3), (0x7FFFFFFF, 0), (1 << 31, 5)])
+@pytest.mark.parametrize("case", range(len(EARLY)))
+def test_rows_on_both_sides_of_position_0(dev, case, window, sinks):
+    """In each form, waves that hold rows before position 0 beside rows from it
+    on, whatever window stands for none."""
+    hq, hkv, d, requests = EARLY[case]
+    st = Early(dev, requests, hq, hkv, d, 16, window, sinks, seed=case)
+    st.make_plan()
+    H.sync()
+    print(f"[paged] before 0: {hq}/{hkv} D={d} {requests[:4]} window {window}: {shape_of(st)}", flush=True)
+    st.run()
+    if window == 0:
+        assert shape_of(st)[0] == (32, 64, 128, 128, 256, 32)[case]

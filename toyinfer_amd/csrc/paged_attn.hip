@@ -109,14 +109,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const char* base) { re
 struct RowView {
     int32_t pos, first, last, first_low, last_low;
     uint32_t window, sinks;  // window 2^31: none
+    // (Of a row before position 0, whose subtraction could wrap: key 0.)
+    __device__ __forceinline__ int32_t low_of(int32_t p) const {
+        return (int32_t)(max((uint32_t)(max(p, -1) + 1), window) - window);
+    }
     __device__ __forceinline__ void span(int32_t f, int32_t l) {
         first = f;
         last = l;
-        first_low = max(0, (int32_t)((uint32_t)f + 1 - window));
-        last_low = max(0, (int32_t)((uint32_t)l + 1 - window));
-    }
-    __device__ __forceinline__ bool sees(uint32_t key) const {
-        return ((uint32_t)(pos - (int32_t)key) < window) | (((int32_t)key <= pos) & (key < sinks));
+        first_low = low_of(f);
+        last_low = low_of(l);
     }
     // No row of the wave sees a key of [k0, k1].
     __device__ __forceinline__ bool none(int32_t k0, int32_t k1) const {
