@@ -448,8 +448,9 @@ int toyinfer_paged_qkv_prologue_bf16(const void* q, const void* k, const void* v
  * toyinfer_paged_attention_workspace_bytes() bytes (independent of the
  * lengths); both 256-byte aligned.  The plan needs no initialisation; the
  * workspace's first 4 * (num_kv_heads + 2) bytes must be zero before its first
- * use (every call leaves them so).  Calls that share a workspace must be ordered on
- * one stream. */
+ * use (every call leaves them so; calls of several head counts may share one
+ * that was zeroed for the largest).  Calls that share a workspace must be
+ * ordered on one stream. */
 size_t toyinfer_paged_attention_plan_bytes(uint32_t batch, uint32_t num_tokens,
                                            uint32_t num_q_heads, uint32_t num_kv_heads,
                                            uint32_t heads_dim);

@@ -475,3 +475,20 @@ def test_rows_on_both_sides_of_position_0(dev, case, window, sinks):
     st.run()
     if window == 0:
         assert shape_of(st)[0] == (32, 64, 128, 128, 256, 32)[case]
+
+
+def test_head_counts_that_share_a_workspace(dev):
+    """A call of few heads, whose units are in pieces, leaves the counters of a
+    call of many heads alone."""
+    few = Wide(dev, [(5000, 1), (3000, 40)], 16, 2, 128, 16, seed=31)
+    many = Wide(dev, [(300, 1), (90, 40), (700, 3)], 130, 130, 64, 16, seed=32)
+    ws = few.ws if few.ws.numel() > many.ws.numel() else many.ws
+    few.ws = many.ws = ws
+    for _ in range(2):
+        few.run()
+        assert shape_of(few)[1]
+        assert not ws[:4 * (130 + 2)].any()
+        many.o.fill_(3.0)
+        many.run()
+        assert shape_of(many)[2]
+        few.o.fill_(3.0)

@@ -909,8 +909,10 @@ static PagedPlanHeader plan_header(uint32_t batch, uint32_t num_tokens, uint32_t
 }
 
 // The workspace holds a ticket per KV head and two flags, the partial outputs,
-// then their statistics.
-static size_t paged_ticket_bytes(uint32_t hkv) { return align_up((hkv + 2) * sizeof(uint32_t), 256); }
+// then their statistics.  The first part is as long as the most heads need
+// (check_heads), so that no call's results lie where another one with more heads
+// looks for its counters.
+constexpr size_t kPagedCounterBytes = ((65535 + 2) * sizeof(uint32_t) + 255) / 256 * 256;
 static size_t paged_part_o_bytes(uint32_t hkv, uint32_t d) {
     return (size_t)hkv * paged_partial_blocks(hkv) * kPagedBlockRows * d * sizeof(float);
 }
@@ -923,7 +925,7 @@ size_t toyinfer_paged_attention_plan_bytes(uint32_t batch, uint32_t num_tokens, 
 
 size_t toyinfer_paged_attention_workspace_bytes(uint32_t num_q_heads, uint32_t num_kv_heads, uint32_t heads_dim) {
     if (check_heads(num_q_heads, num_kv_heads, heads_dim)) return 0;
-    return paged_ticket_bytes(num_kv_heads) + paged_part_o_bytes(num_kv_heads, heads_dim) +
+    return kPagedCounterBytes + paged_part_o_bytes(num_kv_heads, heads_dim) +
            (size_t)num_kv_heads * paged_partial_blocks(num_kv_heads) * kPagedBlockRows * sizeof(float2);
 }
 
@@ -985,7 +987,7 @@ int toyinfer_paged_attention_bf16(const void* q, const void* k_cache, const void
     a.page_stride = page_stride;
     a.tickets = static_cast<uint32_t*>(workspace);
     a.flags = a.tickets + num_kv_heads;
-    char* const part = static_cast<char*>(workspace) + paged_ticket_bytes(num_kv_heads);
+    char* const part = static_cast<char*>(workspace) + kPagedCounterBytes;
     a.part_o = reinterpret_cast<float*>(part);
     a.part_ml = reinterpret_cast<float2*>(part + paged_part_o_bytes(num_kv_heads, heads_dim));
     return from_hip(launch_paged_attention(a, as_stream(stream)));
