@@ -435,7 +435,8 @@ int toyinfer_paged_qkv_prologue_bf16(const void* q, const void* k, const void* v
  * window == 0, or p - j < window, or j < sinks: a sliding window with the first
  * `sinks` tokens kept in sight.  o = softmax(q.k / sqrt(D)) v over those; a row
  * that sees none (p < 0) gives 0, and what a row does not see, infinities and
- * NaN included, does not reach it.  Rows past query_start[batch] are left as
+ * NaN included, does not reach it (to keep them out a call that meets some may
+ * take ten times as long).  Rows past query_start[batch] are left as
  * they are.  o overlaps neither q nor the caches.
  *
  * The plan is the step's work list.  toyinfer_paged_attention_plan builds it on

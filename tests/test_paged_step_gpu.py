@@ -492,3 +492,105 @@ def test_head_counts_that_share_a_workspace(dev):
         many.run()
         assert shape_of(many)[2]
         few.o.fill_(3.0)
+
+
+def put_nan(st, at):
+    """NaN (or infinities) at (request, key, dim) of V, for every KV head."""
+    for b, j, dim, x in at:
+        st.v[int(st.table[b, j // st.ps]), j % st.ps, :, dim] = x
+
+
+def check_nan(st, at):
+    """An element is what its row's keys make of it: NaN or infinity by one that
+    it sees, within the bound of the finite values' result elsewhere."""
+    for b, (length, n) in enumerate(st.requests):
+        rows = slice(int(st.start[b]), int(st.start[b + 1]))
+        if not n:
+            continue
+        k, v = (x.to(st.dev) for x in st.kv[b])
+        got, q = st.o[rows], st.q_d[rows]
+        spoilt = torch.zeros(n, st.d, dtype=torch.bool, device=st.dev)
+        seen = torch.from_numpy(PO.visible(n, length, st.window, st.sinks)).to(st.dev)
+        for rb, j, dim, _ in at:
+            if rb == b:
+                spoilt[:, dim] |= seen[:, j]
+        o, size = wide_attention(q, k, v, st.window, st.sinks)
+        bound = 2.0 ** -8 * (size + 2 * o.abs()) * (1 + 2.0 ** -6) + 2.0 ** -12 * size
+        ok = (got.double() - o).abs() <= bound
+        spoilt = spoilt[:, None].expand_as(ok)
+        assert ok[~spoilt].all(), (b, (~ok & ~spoilt).nonzero()[:3].tolist())
+        assert not torch.isfinite(got[spoilt]).any(), b
+    assert (st.o[st.total:] == 3.0).all() and not st.ws[:4 * (st.hkv + 2)].any()
+
+
+NAN, INF = float("nan"), float("inf")
+SPOILT = [
+    (32, 8, 128, [(50, 50), (700, 3)], 0, 0, [(0, 33, 5, NAN), (1, 698, 9, INF)]),
+    (8, 8, 64, [(3005, 3005)], 0, 0, [(0, 1000, 5, NAN), (0, 2900, 63, INF)]),
+    (32, 8, 128, [(901, 901)], 0, 0, [(0, 0, 0, NAN), (0, 450, 127, NAN), (0, 900, 1, NAN)]),
+    (32, 8, 128, [(100 + i, 100) for i in range(12)], 0, 0, [(b, 40 + 5 * b, b, NAN) for b in range(12)]),
+    (8, 1, 128, [(9000, 1), (2000, 300), (15, 12)], 0, 0, [(1, 1800, 7, NAN), (2, 9, 7, -INF)]),
+    (32, 8, 128, [(8192, 512)], 0, 0, [(0, 100, 3, NAN), (0, 8000, 77, NAN)]),
+    (32, 8, 128, [(8192, 1), (5000, 4), (300, 1)], 1000, 4, [(0, 7191, 2, NAN), (1, 1, 2, NAN), (1, 3999, 3, INF)]),
+    (6, 2, 64, [(5000, 300)], 1024, 16, [(0, 3700, 0, NAN), (0, 4800, 1, NAN)]),
+]
+
+
+@pytest.mark.parametrize("case", range(len(SPOILT)))
+def test_values_that_are_not_finite(dev, case):
+    """In each form, whole and in pieces: a value reaches the dims of the rows
+    that see it, and no others."""
+    hq, hkv, d, requests, window, sinks, at = SPOILT[case]
+    st = Wide(dev, requests, hq, hkv, d, 16, window, sinks, seed=case)
+    st.make_plan()
+    H.sync()
+    print(f"[paged] not finite: {hq}/{hkv} D={d} {requests[:3]}: {shape_of(st)}", flush=True)
+    st.run()
+    put_nan(st, at)
+    for _ in range(2):
+        st.o.fill_(3.0)
+        st.attend()
+        H.sync()
+        check_nan(st, at)
+
+
+def test_more_spoilt_blocks_than_marks(dev):
+    """NaN in one dim of every seventh token: more blocks of rows to compute again
+    than a call keeps apart."""
+    st = Wide(dev, [(5000, 5000), (900, 1)], 32, 32, 64, 16, seed=3)
+    at = [(0, j, 11, NAN) for j in range(3, 5000, 7)]
+    put_nan(st, at)
+    st.make_plan()
+    st.attend()
+    H.sync()
+    check_nan(st, at)
+
+
+def time_of(f, n=20):
+    f()
+    start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    start.record()
+    for _ in range(n):
+        f()
+    end.record()
+    H.sync()
+    return start.elapsed_time(end) / n
+
+
+@pytest.mark.parametrize("hq,hkv,d,requests,window,at", [
+    (32, 8, 128, [(2048, 2048)], 0, (0, 5, 3, NAN)),        # seen by nearly all rows
+    (32, 8, 128, [(2048, 2048)], 0, (0, 1500, 3, NAN)),
+    (32, 8, 128, [(4000, 64)], 0, (0, 3980, 3, NAN)),       # in pieces
+    (32, 8, 128, [(6000, 1)] * 8, 4096, (0, 1903, 3, NAN)),  # behind the window
+])
+def test_time_of_a_spoilt_call(dev, hq, hkv, d, requests, window, at):
+    """One NaN does not turn a call into one of another order: only the blocks of
+    rows that cannot tell it from a hidden one are computed again.  (All of a
+    call's rows with NaN computed again took 300 to 4500 times the call.)"""
+    st = Wide(dev, requests, hq, hkv, d, 16, window, seed=1)
+    st.make_plan()
+    clean = time_of(st.attend)
+    put_nan(st, [at])
+    spoilt = time_of(st.attend, 3)
+    print(f"[paged] {requests[:2]} {1e3 * clean:.0f} us, with a NaN {1e3 * spoilt:.0f}", flush=True)
+    assert spoilt < 30 * clean

@@ -908,11 +908,12 @@ static PagedPlanHeader plan_header(uint32_t batch, uint32_t num_tokens, uint32_t
     return h;
 }
 
-// The workspace holds a ticket per KV head and two flags, the partial outputs,
-// then their statistics.  The first part is as long as the most heads need
+// The workspace holds a ticket per KV head and two flags, the marks, the partial
+// outputs, then their statistics.  The first part is as long as the most heads need
 // (check_heads), so that no call's results lie where another one with more heads
 // looks for its counters.
 constexpr size_t kPagedCounterBytes = ((65535 + 2) * sizeof(uint32_t) + 255) / 256 * 256;
+constexpr size_t kPagedPartials = kPagedCounterBytes + kPagedMarks * sizeof(PagedMark);
 static size_t paged_part_o_bytes(uint32_t hkv, uint32_t d) {
     return (size_t)hkv * paged_partial_blocks(hkv) * kPagedBlockRows * d * sizeof(float);
 }
@@ -925,7 +926,7 @@ size_t toyinfer_paged_attention_plan_bytes(uint32_t batch, uint32_t num_tokens, 
 
 size_t toyinfer_paged_attention_workspace_bytes(uint32_t num_q_heads, uint32_t num_kv_heads, uint32_t heads_dim) {
     if (check_heads(num_q_heads, num_kv_heads, heads_dim)) return 0;
-    return kPagedCounterBytes + paged_part_o_bytes(num_kv_heads, heads_dim) +
+    return kPagedPartials + paged_part_o_bytes(num_kv_heads, heads_dim) +
            (size_t)num_kv_heads * paged_partial_blocks(num_kv_heads) * kPagedBlockRows * sizeof(float2);
 }
 
@@ -987,7 +988,8 @@ int toyinfer_paged_attention_bf16(const void* q, const void* k_cache, const void
     a.page_stride = page_stride;
     a.tickets = static_cast<uint32_t*>(workspace);
     a.flags = a.tickets + num_kv_heads;
-    char* const part = static_cast<char*>(workspace) + kPagedCounterBytes;
+    a.marks = reinterpret_cast<PagedMark*>(static_cast<char*>(workspace) + kPagedCounterBytes);
+    char* const part = static_cast<char*>(workspace) + kPagedPartials;
     a.part_o = reinterpret_cast<float*>(part);
     a.part_ml = reinterpret_cast<float2*>(part + paged_part_o_bytes(num_kv_heads, heads_dim));
     return from_hip(launch_paged_attention(a, as_stream(stream)));

@@ -84,7 +84,7 @@ struct PagedPlanHeader {
     uint32_t items;
     uint32_t split_blocks;  // 32-row blocks whose partials are to be merged, per KV head
     uint32_t ranges;        // lists of items: lane l runs list l, then draws further ones
-    uint32_t units;         // in the plan's array of them; a split one's `partial` is not kPagedWhole
+    uint32_t units;         // in the plan's array of them
     uint32_t pad[50];
 };
 static_assert(sizeof(PagedPlanHeader) == 256, "the items follow at a cache line");
@@ -116,6 +116,20 @@ struct PagedSplitBlock {
     int32_t pos0;  // as in PagedItem
 };
 static_assert(sizeof(PagedSplitBlock) == 32, "read by 16-byte loads");
+
+// A 32-row block one of whose tiles had an infinity or NaN in V of a key that
+// some row of the block does not see.  A workspace holds this many; if a call
+// meets more (of pieces and streams each its own), all of its rows count as such.
+constexpr uint32_t kPagedMarks = 4096;
+struct PagedMark {
+    uint32_t req;          // row of the block table
+    uint32_t token, head;  // of its first row: row of q and o, head in the group
+    uint32_t kvh;
+    int32_t pos;
+    uint32_t rows;  // 1..32
+    uint32_t pad[2];
+};
+static_assert(sizeof(PagedMark) == 32, "read by 16-byte loads");
 
 // Units of any plan for these sizes, and the places of the plan's arrays.
 inline __host__ __device__ uint32_t paged_max_units(uint32_t batch, uint32_t num_tokens, uint32_t group) {
@@ -156,7 +170,8 @@ struct PagedAttnArgs {
     uint32_t num_pages;
     uint64_t page_stride;  // elements
     uint32_t* tickets;     // [KV head], zero between calls
-    uint32_t* flags;       // [2], zero between calls: a hidden infinity or NaN was met; workgroups done
+    uint32_t* flags;       // [2], zero between calls: marks; workgroups of the merge that are done
+    PagedMark* marks;      // [kPagedMarks]
     float* part_o;         // [KV head][block][D / 4][64 lanes][4]
     float2* part_ml;       // [KV head][block][32 rows]: reference (log2), sum
 };

@@ -21,9 +21,10 @@
 // sees are some row of its last page and masked like any hidden key; V's are
 // zeroed in LDS, since 0 * NaN is NaN.  Where a tile has a key that some row
 // does not see and its V holds infinities or NaN, 0 times them turns that row
-// to NaN: the workgroup says so in a flag, and the second kernel then computes
-// the rows that hold NaN again, key by key.  (Done here instead, in registers
-// that the compiler took from the loops, it cost the streaming form 15 %.)
+// to NaN: the wave marks its block of rows, and the second kernel computes the
+// marked blocks again, key by key.  (Done here instead, in registers that the
+// compiler took from the loops, it cost the streaming form 15 %.)  A block whose
+// rows all see the value is not marked: its NaN is the result.
 //
 // Measured, at 32 query and 8 KV heads of 128:
 //   streaming, 32 requests of 2208..8193 keys (704 MB): 114 us, 6.2 TB/s of keys
@@ -317,7 +318,7 @@ struct Segment {
     uint32_t kvh, kind, item_end, opens;
     uint32_t token, head;  // of the unit's first row, the head in its group
     int32_t pos;
-    uint32_t pad;
+    uint32_t spoilt;       // a stream met an infinity or NaN in V of a hidden key
 };
 
 // The kernel's arguments, read again where they are used: in registers
@@ -416,6 +417,21 @@ __device__ __forceinline__ void put_ml(const PagedAttnArgs& a, const ItemView& v
     if (v.it.partial == kPagedWhole || lane >= 32 || row_block * kPagedBlockRows >= v.it.rows) return;
     const uint64_t blk = (uint64_t)v.kvh * paged_partial_blocks(a.head.hkv) + v.it.partial + row_block;
     a.part_ml[blk * kPagedBlockRows + lane] = make_float2(m, l);
+}
+
+// By one wave: the 32-row block of the unit from `row` on is to be computed again.
+__device__ __forceinline__ void mark(const PagedAttnArgs& a, const ItemView& v, uint32_t row) {
+    const uint32_t t = tokens_on(v, row);
+    PagedMark m{};
+    m.req = v.it.req;
+    m.token = v.token + t;
+    m.head = v.head + row - t * v.group;
+    m.kvh = v.kvh;
+    m.pos = v.pos + (int32_t)t;
+    m.rows = min(kPagedBlockRows, v.it.rows - row);
+    if ((threadIdx.x & 63) != 0) return;
+    const uint32_t n = atomicAdd(a.flags, 1u);
+    if (n < kPagedMarks) a.marks[n] = m;
 }
 
 // Merge of the KS waves (streams) that hold the same 32 rows, through s_a and
@@ -636,7 +652,7 @@ __device__ __forceinline__ void run_shared(const PagedAttnArgs& a, const ItemVie
             if (t + TILES < c1) step(t + TILES, s_b, s_a);
         }
     }
-    if (bad) arguments().flags[0] = 1;
+    if (bad) mark(arguments(), v, rb * 32);
     finish<D, RB, KS>(arguments(), v, s, s_a, s_b, s_ml, wave, lane);
 }
 
@@ -813,7 +829,7 @@ __device__ __forceinline__ void stage(const PagedAttnArgs& a, ItemView& v, Paged
         s.token = v.token;
         s.head = v.head;
         s.pos = v.pos;
-        s.pad = 0;
+        s.spoilt = 0;
         *seg = s;
     }
 }
@@ -1001,6 +1017,7 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
             lds_ops_barrier();  // the next segment is staged
             lds_ops_barrier();  // this one's results are in LDS, its table and rows done with
             if (closes) merge();
+            if (wave == kStreams && s_seg[slot].spoilt) mark(a, v, 0);
             slot ^= 1;
         }
     }
@@ -1090,7 +1107,7 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
                     if (k0 + P::RI * j + lr >= v.src.key_end)
                         *reinterpret_cast<uint4*>(sv + 512 * j + 8 * lane) = make_uint4(0, 0, 0, 0);
                 __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
-                if (rv.some_hidden(k0, min(k1, v.src.key_end - 1)) && any_nonfinite<D, 1>(sv, lane)) *a.flags = 1;
+                if (rv.some_hidden(k0, min(k1, v.src.key_end - 1)) && any_nonfinite<D, 1>(sv, lane)) s_seg[slot].spoilt = 1;
             }
             uint4 va[2][P::DBLK];
             read_v(va, v_at);
@@ -1191,37 +1208,60 @@ __global__ __launch_bounds__(kPaThreads, 1) void paged_attn_kernel(PagedAttnArgs
     }
 }
 
-// One row's attention again, by a wave, key by key over those that it sees: a
-// lane takes D / 64 of the dims.  Slow, and only for rows that an infinity or
-// NaN which they do not see has turned to NaN.
+// One row's attention again, by a workgroup, key by key over those that it sees:
+// a wave takes every fourth tile of 64 keys, the newest first, a lane a key for
+// the scores and then D / 64 of the dims.  For rows of marked blocks only.  A row
+// that the keys it sees make NaN throughout stops there.  Bound by the latency of
+// its loads, 23 us per 64 keys and wave.  One NaN in V, in us: a decode batch at
+// the edge of a window of 4096 keys 51 -> 570, 512 tokens on 8192 keys 89 -> 1541,
+// a prompt of 8192 583 -> 716 (key 819) and 1892 (key 7372); sixteen V rows in
+// flight instead of eight took up to 1.8 times that.
+struct ExactLds {
+    float4 q[2][16];  // even dims, odd dims
+    float o[4][128];
+    float2 ml[4];
+    uint32_t stop;
+};
+static_assert(sizeof(ExactLds) <= 16384, "in the merge's LDS");
 template <int D>
 __device__ __forceinline__ void exact_row(const PagedAttnArgs& a, float scale_log2, uint32_t req, int32_t pos,
-                                          uint32_t token, uint32_t kvh, uint32_t head, uint32_t dim0, uint32_t dims) {
-    constexpr int DPL = D / 64;
-    const uint32_t lane = threadIdx.x & 63, page_shift = 31 - __builtin_clz(a.head.page_size);
+                                          uint32_t token, uint32_t kvh, uint32_t head, ExactLds& lds) {
+    constexpr int DPL = D / 64, U = 8;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t page_shift = 31 - __builtin_clz(a.head.page_size);
     const uint32_t window = a.head.window, sinks = window ? a.head.sinks : 0;
     const uint32_t low = window && pos >= 0 && (uint32_t)pos + 1 > window ? (uint32_t)pos + 1 - window : 0;
     const uint32_t* const table = a.block_tables + (uint64_t)req * a.head.max_blocks;
-    const uint16_t* const q = a.q + ((uint64_t)token * a.head.hq + head) * D;
-    auto row_at = [&](const uint16_t* cache, uint32_t key) {
-        const uint32_t page = min(table[key >> page_shift], a.num_pages - 1);
-        return cache + page * a.page_stride + ((uint64_t)(key & (a.head.page_size - 1)) * a.head.hkv + kvh) * D;
-    };
+    const uint64_t row = ((uint64_t)token * a.head.hq + head) * D;
+    __syncthreads();  // the last row's results are read
+    if (threadIdx.x == 0) lds.stop = 0;
+    if (threadIdx.x < D) reinterpret_cast<float*>(lds.q[threadIdx.x & 1])[threadIdx.x / 2] = bf16_to_f32(a.q[row + threadIdx.x]);
+    __syncthreads();
     float m = -INFINITY, l = 0.0f, acc[DPL];
 #pragma unroll
     for (int e = 0; e < DPL; ++e) acc[e] = 0.0f;
-    for (int32_t k0 = 0; k0 <= pos; k0 += 64) {
-        const uint32_t key = k0 + lane;
-        const bool seen = (int32_t)key <= pos && (key >= low || key < sinks);
+    for (int32_t t = pos < 0 ? -1 : (pos >> 6) - (int32_t)wave; t >= 0; t -= 4) {
+        if (*(volatile uint32_t*)&lds.stop) break;
+        const uint32_t key = 64 * (uint32_t)t + lane;
+        const bool seen = key <= (uint32_t)pos && (key >= low || key < sinks);
         const uint64_t mask = __ballot(seen);
         if (!mask) continue;
         float sc = -INFINITY;
+        uint64_t at = 0;
         if (seen) {
-            const uint16_t* const k = row_at(a.k_cache, key);
-            float dot = 0.0f;
-#pragma unroll 1
-            for (int i = 0; i < D; ++i) dot = fmaf(bf16_to_f32(q[i]), bf16_to_f32(k[i]), dot);
-            sc = dot * scale_log2;
+            const uint32_t page = min(table[key >> page_shift], a.num_pages - 1);
+            at = page * a.page_stride + ((uint64_t)(key & (a.head.page_size - 1)) * a.head.hkv + kvh) * D;
+            float dot[2] = {0.0f, 0.0f};
+#pragma unroll 8
+            for (int c = 0; c < D / 8; ++c) {
+                const uint4 k4 = ldg16(a.k_cache + at + 8 * c);
+                const float4 q0 = lds.q[0][c], q1 = lds.q[1][c];
+                dot[0] = fmaf(q0.x, bf16_lo(k4.x), fmaf(q0.y, bf16_lo(k4.y), dot[0]));
+                dot[0] = fmaf(q0.z, bf16_lo(k4.z), fmaf(q0.w, bf16_lo(k4.w), dot[0]));
+                dot[1] = fmaf(q1.x, bf16_hi(k4.x), fmaf(q1.y, bf16_hi(k4.y), dot[1]));
+                dot[1] = fmaf(q1.z, bf16_hi(k4.z), fmaf(q1.w, bf16_hi(k4.w), dot[1]));
+            }
+            sc = (dot[0] + dot[1]) * scale_log2;
         }
         float mx = sc;
 #pragma unroll
@@ -1234,21 +1274,60 @@ __device__ __forceinline__ void exact_row(const PagedAttnArgs& a, float scale_lo
             m = mx;
         }
         const float p = seen ? __builtin_amdgcn_exp2f(sc - (m == -INFINITY ? 0.0f : m)) : 0.0f;
-        for (uint64_t left = mask; left; left &= left - 1) {
-            const int j = __builtin_ctzll(left);
-            const float pj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), j));
-            const uint16_t* const v = row_at(a.v_cache, k0 + j);
-            l += pj;
+        for (uint64_t left = mask; left;) {
+            int j[U];
+            bool has[U];
+            float v[U][DPL];
 #pragma unroll
-            for (int e = 0; e < DPL; ++e) acc[e] = fmaf(pj, bf16_to_f32(v[DPL * lane + e]), acc[e]);
+            for (int u = 0; u < U; ++u) {
+                has[u] = left != 0;
+                j[u] = has[u] ? __builtin_ctzll(left) : j[0];
+                left &= left - 1;
+                const uint16_t* const src =
+                    a.v_cache + base_of(make_uint2((uint32_t)at, (uint32_t)(at >> 32)), j[u]) + DPL * lane;
+                if constexpr (DPL == 2) {
+                    const uint32_t w = *reinterpret_cast<const uint32_t*>(src);
+                    v[u][0] = bf16_lo(w);
+                    v[u][1] = bf16_hi(w);
+                } else {
+                    v[u][0] = bf16_to_f32(*src);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (!has[u]) break;
+                const float pj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), j[u]));
+                l += pj;
+#pragma unroll
+                for (int e = 0; e < DPL; ++e) acc[e] = fmaf(pj, v[u][e], acc[e]);
+            }
+        }
+        bool nan = l != l;
+        if (!nan) {
+            nan = acc[0] != acc[0];
+            if constexpr (DPL == 2) nan = nan && acc[1] != acc[1];
+        }
+        if (__all(nan)) {
+            if (lane == 0) *(volatile uint32_t*)&lds.stop = 1;
+            break;
         }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int e = 0; e < DPL; ++e) {
-        const uint32_t d = DPL * lane + e;
-        if (d >= dim0 && d < dim0 + dims) a.o[((uint64_t)token * a.head.hq + head) * D + d] = f32_to_bf16(acc[e] * inv);
+    for (int e = 0; e < DPL; ++e) lds.o[wave][DPL * lane + e] = acc[e];
+    if (lane == 0) lds.ml[wave] = make_float2(m, l);
+    __syncthreads();
+    if (threadIdx.x >= D) return;
+    float M = -INFINITY, x = 0.0f, tot = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) M = fmaxf(M, lds.ml[k].x);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float2 ml = lds.ml[k];
+        const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);  // (0 keeps the NaN of a sum)
+        tot = fmaf(w, ml.y, tot);
+        x = fmaf(w, lds.o[k][threadIdx.x], x);
     }
+    a.o[row + threadIdx.x] = f32_to_bf16(x * (tot == 0.0f ? 0.0f : 1.0f / tot));
 }
 
 // Merge of the pieces of each split 32-row block: a workgroup takes one d-block
@@ -1264,15 +1343,30 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedAttnArg
     constexpr int DBLK = D / 32, NF = PaShape<D>::NF, U = 4;
     __shared__ float4 s_o[4][4][64];
     __shared__ float2 s_ml[4][64];
+    __shared__ int s_found[4];
     const PlanHead head = plan_load<PlanHead>(a.plan, 0);
     if (!head.fits(a.head)) return;
     const uint32_t hkv = a.head.hkv, group = a.head.hq / hkv, blocks = head.split_blocks;
-    const bool again = scalar_load(a.flags) != 0;
-    // The tickets back to zero, for the next call.
-    for (uint32_t i = blockIdx.x * kMergeThreads + threadIdx.x; i < hkv; i += gridDim.x * kMergeThreads) a.tickets[i] = 0;
-    const PagedPlanLayout lay = paged_plan_layout(a.head.batch, a.head.num_tokens, a.head.hq, hkv);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (uint32_t i = blockIdx.x; i < blocks * hkv * DBLK; i += gridDim.x) {
+    const uint32_t met = scalar_load(a.flags), marks = min(met, kPagedMarks);
+    const bool all_marked = met > kPagedMarks;
+    // Whether one of the first n marks is of this block, of the workgroup's row.
+    auto marked = [&](uint32_t n, uint32_t req, uint32_t token, uint32_t h, uint32_t kvh) {
+        bool is = false;
+        for (uint32_t i = threadIdx.x; i < n; i += kMergeThreads) {
+            const PagedMark m = arguments().marks[i];
+            is |= m.req == req && m.token == token && m.head == h && m.kvh == kvh;
+        }
+        const int any = __any(is);
+        __syncthreads();  // (the last answer is read)
+        if (lane == 0) s_found[wave] = any;
+        __syncthreads();
+        return (s_found[0] | s_found[1] | s_found[2] | s_found[3]) != 0;
+    };
+    // The tickets back to zero, for the next call.
+    for (uint32_t i = blockIdx.x * kMergeThreads + threadIdx.x; i < hkv; i += kMergeWgs * kMergeThreads) a.tickets[i] = 0;
+    const PagedPlanLayout lay = paged_plan_layout(a.head.batch, a.head.num_tokens, a.head.hq, hkv);
+    for (uint32_t i = blockIdx.x; i < blocks * hkv * DBLK; i += kMergeWgs) {
         const uint32_t db = i % DBLK, kvh = i / DBLK % hkv;
         const PagedSplitBlock sb =
             plan_load<PagedSplitBlock>(a.plan, lay.split_blocks + (uint64_t)(i / (DBLK * hkv)) * sizeof(PagedSplitBlock));
@@ -1334,44 +1428,49 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedAttnArg
             x.w = fmaf(w[k], y.w, x.w);
         }
         const float inv = tot == 0.0f ? 0.0f : 1.0f / tot;
+        // (Marked blocks are written below only.)
+        if (met && (all_marked || marked(marks, sb.req, sb.token0 + sb.row0 / group, sb.row0 % group, kvh))) continue;
         if (has) {
             const uint32_t r = sb.row0 + (lane & 31), token = sb.token0 + r / group, h = kvh * group + r % group;
             uint16_t* o = a.o + ((uint64_t)token * a.head.hq + h) * D + 32 * db + 8 * wave + 4 * (lane >> 5);
             *reinterpret_cast<uint2*>(o) =
                 make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
         }
-        if (again) {
-            // This wave's eight dims of the rows that came out as NaN.
-            const float sum = (x.x + x.y + x.z + x.w) * inv;  // (NaN for opposite infinities too: no harm)
-            uint64_t rows = __ballot(has && sum != sum);
-            rows = (rows | rows >> 32) & 0xffffffffull;
-            for (; rows; rows &= rows - 1) {
-                const uint32_t r = sb.row0 + __builtin_ctzll(rows), token = sb.token0 + r / group;
-                exact_row<D>(a, scale_log2, sb.req, sb.pos0 + (int32_t)(r / group), token, kvh, kvh * group + r % group,
-                             32 * db + 8 * wave, 8);
-            }
-        }
     }
-    if (!again) return;
-    // The rows of whole units that hold NaN.
-    const uint32_t waves = gridDim.x * (kMergeThreads / 64);
-    for (uint32_t i = blockIdx.x * (kMergeThreads / 64) + wave; i < head.units * hkv; i += waves) {
-        const PagedItem u = plan_load<PagedItem>(a.plan, lay.units + (uint64_t)(i / hkv) * sizeof(PagedItem));
-        const uint32_t kvh = i % hkv;
-        if (u.partial != kPagedWhole) continue;
-        for (uint32_t row = 0; row < u.rows; ++row) {
-            const uint32_t r = u.row0 + row, token = u.token0 + r / group, h = kvh * group + r % group;
-            const uint16_t* o = a.o + ((uint64_t)token * a.head.hq + h) * D + D / 64 * lane;
-            bool bad = false;
-#pragma unroll
-            for (int e = 0; e < D / 64; ++e) bad |= (o[e] & 0x7fffu) > 0x7f80u;
-            if (__any(bad))
-                exact_row<D>(a, scale_log2, u.req, u.pos0 + (int32_t)(r / group), token, kvh, h, 0, D);
+    if (!met) return;
+    // The rows of the marked blocks, each block by its first mark.
+    const uint64_t rows = all_marked ? (uint64_t)head.units * hkv * kPagedMaxRows : (uint64_t)marks * kPagedBlockRows;
+    for (uint64_t i = blockIdx.x; i < rows; i += kMergeWgs) {
+        uint32_t req, token, h, kvh, row;
+        int32_t pos;
+        if (all_marked) {
+            const uint64_t at = i / kPagedMaxRows;
+            const PagedItem u = plan_load<PagedItem>(a.plan, lay.units + at / hkv * sizeof(PagedItem));
+            row = u.row0 + (uint32_t)(i % kPagedMaxRows);
+            if (i % kPagedMaxRows >= u.rows) continue;
+            req = u.req;
+            token = u.token0;
+            h = 0;
+            kvh = (uint32_t)(at % hkv);
+            pos = u.pos0;
+        } else {
+            const uint32_t at = (uint32_t)(i / kPagedBlockRows);
+            const PagedMark m = plan_load<PagedMark>(arguments().marks, at * sizeof(PagedMark));
+            row = i % kPagedBlockRows;
+            if (row >= m.rows || marked(at, m.req, m.token, m.head, m.kvh)) continue;
+            req = m.req;
+            token = m.token;
+            h = m.head;
+            kvh = m.kvh;
+            pos = m.pos;
         }
+        const uint32_t ahead = (h + row) / group;
+        exact_row<D>(arguments(), scale_log2, req, pos + (int32_t)ahead, token + ahead, kvh, kvh * group + (h + row) % group,
+                     *reinterpret_cast<ExactLds*>(s_o));
     }
-    // The flag back to zero, by the last workgroup to come here (flags[1] counts).
+    // The count back to zero, by the last workgroup to come here (flags[1] counts them).
     __syncthreads();
-    if (threadIdx.x == 0 && atomicAdd(a.flags + 1, 1u) == gridDim.x - 1) {
+    if (threadIdx.x == 0 && atomicAdd(a.flags + 1, 1u) == kMergeWgs - 1) {
         a.flags[0] = 0;
         a.flags[1] = 0;
     }

@@ -428,7 +428,6 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
                     else
                         lo = mid;
                 }
-                units[i].partial = 0;  // (split; the pieces' own places are in the items)
                 const uint32_t pieces = s_item[lo] + (i - s_cut_unit[lo]) - j + 1;
                 for (uint32_t k = 0; k < nb; ++k) {
                     PagedSplitBlock s{};
