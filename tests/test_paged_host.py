@@ -142,3 +142,44 @@ def test_oracle_of_the_attention_mask():
     o, away, size = PO.attention(torch.zeros(1, 1, 1), torch.zeros(2, 1, 1),
                                  torch.tensor([[[1.0]], [[3.0]]]), 0, 0)
     assert o.item() == 2 and away.item() == 1 and size.item() == 2
+
+
+@pytest.mark.parametrize("view,stride,ok", [
+    (lambda t: t, 1, True),
+    (lambda t: t.view(-1), 1, True),
+    (lambda t: t.view(48, 2, 64), 1, True),
+    (lambda t: t[1:], 1, True),
+    (lambda t: t.view(3, 2, 8, 2, 64)[:, 0], 2, True),           # beside V's pages
+    (lambda t: t.view(3, 2, 8, 2, 64)[:, 1:], 2, True),
+    (lambda t: t.view(3, 2, 8, 2, 64), 2, True),
+    (lambda t: t.view(-1)[:2 * 8 * 2 * 64], 1, True),
+    (lambda t: t.view(3, 2, 8, 2, 64)[:, 0], 1, False),          # pages closer than they lie
+    (lambda t: t, 2, False),                                     # further apart
+    (lambda t: t.view(6, 2, 8, 64), 1, False),                   # [heads][rows]
+    (lambda t: t.view(6, 2, 8, 64).transpose(1, 2), 1, False),
+    (lambda t: t.view(6, 8, 64, 2).transpose(2, 3), 1, False),
+    (lambda t: t.view(6, 8, 4, 32)[:, :, :2], 1, False),         # heads of a wider cache
+    (lambda t: t.view(8, 6, 2, 64).transpose(0, 1), 1, False),   # pages inside rows
+    (lambda t: t.view(48, 2, 64)[::2], 1, False),
+])
+def test_binding_takes_caches_of_pages_only(view, stride, ok):
+    """A cache of another layout than the kernels read is refused, one in pages
+    at the stride that is given taken."""
+    t = view(torch.zeros(6, 8, 2, 64, dtype=torch.bfloat16))
+    args = "paged", -1, 2, 8, stride * 8 * 2 * 64, 2, 64
+    if ok:
+        attn._need_cache(*args, t)
+    else:
+        with pytest.raises(attn.ToyInferError):
+            attn._need_cache(*args, t)
+
+
+def test_binding_takes_one_page_and_one_head():
+    """Sizes of one have no stride that counts."""
+    one = torch.zeros(1, 8, 2, 64, dtype=torch.bfloat16)
+    attn._need_cache("paged", -1, 1, 8, 5000, 2, 64, one, one.view(-1))
+    wide = torch.zeros(3, 8, 4, 64, dtype=torch.bfloat16)
+    with pytest.raises(attn.ToyInferError):
+        attn._need_cache("paged", -1, 2, 8, 8 * 4 * 64, 1, 64, wide[:, :, 1:2])
+    head = torch.zeros(3, 8, 64, dtype=torch.bfloat16)[:, :, None]
+    attn._need_cache("paged", -1, 3, 8, 8 * 64, 1, 64, head)

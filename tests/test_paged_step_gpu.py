@@ -594,3 +594,26 @@ def test_time_of_a_spoilt_call(dev, hq, hkv, d, requests, window, at):
     spoilt = time_of(st.attend, 3)
     print(f"[paged] {requests[:2]} {1e3 * clean:.0f} us, with a NaN {1e3 * spoilt:.0f}", flush=True)
     assert spoilt < 30 * clean
+
+
+def test_binding_refuses_caches_of_other_layouts(dev):
+    """A transposed cache, or one whose pages lie elsewhere than the call says:
+    refused by both calls that take one, nothing written."""
+    st = Step(dev, [(40, 1), (90, 3)], 8, 2, 128, 16)
+    st.make_plan()
+    swapped = st.k.transpose(1, 2).contiguous()
+    apart = torch.zeros(st.pages, 2, 16, 2, 128, dtype=torch.bfloat16, device=dev)[:, 0]
+    rope = torch.zeros(99, 64, 2, device=dev)
+    index = torch.zeros(st.rows, dtype=torch.int32, device=dev)
+    new = st.q_d[:, :2].contiguous()
+    w = torch.ones(128, dtype=torch.bfloat16, device=dev)
+    for bad in (swapped, swapped.transpose(1, 2), apart):
+        for k, v in ((bad, st.v), (st.k, bad)):
+            with pytest.raises(attn.ToyInferError):
+                attn.paged_attention_bf16(st.q_d, k, v, st.o, st.table, st.plan, st.batch, st.rows,
+                                          st.pages, st.ps, st.stride, st.blocks, 0, 0, 8, 2, 128, st.ws)
+            with pytest.raises(attn.ToyInferError):
+                attn.paged_qkv_prologue_bf16(st.q_d, new, new, w, w, rope, 99, index, index, st.rows,
+                                             1e-6, st.q_d, k, v, st.pages, st.ps, st.stride, 8, 2, 128)
+    H.sync()
+    assert (st.o == 3.0).all() and (apart == 0).all()

@@ -524,15 +524,43 @@ def _need(fn: str, device: int, dtypes, *pairs) -> None:
             raise ToyInferError(fn, ERR_INVALID_ARGUMENT)
 
 
+def _dense_in_pages(t, num_pages: int, page_size: int, page_stride: int, num_kv_heads: int,
+                    head_dim: int) -> bool:
+    """Whether t's elements lie as pages of [page_size][num_kv_heads][head_dim]
+    do: in one piece up to a page, the next one page_stride on."""
+    inner = (page_size, num_kv_heads, head_dim)
+    page = page_size * num_kv_heads * head_dim
+    if t.dim() >= 3 and t.shape[-3:].numel() == page and t.shape[-3:] != inner:
+        return False  # [heads][rows], say
+    dense = 1
+    for size, stride in zip(reversed(t.shape), reversed(t.stride())):
+        if size == 1:
+            continue
+        if dense == page:
+            if num_pages == 1:
+                break
+            # (Or pages of K and V in turn.)
+            if stride != page_stride and not (stride == page and size * page == page_stride):
+                return False
+        elif stride != dense:
+            return False
+        dense = stride * size
+    return True
+
+
 def _need_cache(fn: str, device: int, num_pages: int, page_size: int, page_stride: int,
                 num_kv_heads: int, head_dim: int, *caches) -> None:
     """Caches may be views with pages further apart than a page is long; what
     they span from their first element has to lie in their storage."""
     bf16 = _types()[0]
-    span = (num_pages - 1) * page_stride + page_size * num_kv_heads * head_dim
+    row = num_kv_heads * head_dim
+    span = (num_pages - 1) * page_stride + page_size * row
+    strides = page_stride, row, head_dim, 1
     for t in caches:
         if (t.get_device() != device or t.dtype not in bf16
-                or t.untyped_storage().nbytes() // 2 - t.storage_offset() < span):
+                or t.untyped_storage().nbytes() // 2 - t.storage_offset() < span
+                or t.stride() != strides and not _dense_in_pages(
+                    t, num_pages, page_size, page_stride, num_kv_heads, head_dim)):
             raise ToyInferError(fn, ERR_INVALID_ARGUMENT)
 
 
