@@ -151,34 +151,28 @@ __global__ __launch_bounds__(kTabThreads) void paged_tables_kernel(PagedTablesAr
     }
 }
 
-// D / 16 lanes per row, lane c the eight pairs (8c + k, 8c + k + D/2); U rows
-// per lane group, so that a position's angles and the weights are read once
-// for U rows.  Each input row is read once and each output row written once, and
-// both bypass the caches' retention: 8192 tokens of 32 + 2 * 8 heads 40.2 -> 36.7 us
-// (5.5 TB/s, the rate of a large copy), 1371 tokens 7.0 -> 5.3.  One row per lane
-// group is launched: two and four gave up to 2 % on 8192 tokens and cost a small call
-// 0.3 and 1.1 us of 2.5.
-template <int D, int U>
+// D / 16 lanes per row, lane c the eight pairs (8c + k, 8c + k + D/2); a wave has
+// G consecutive rows of a token.  Each input row is read once and each output row
+// written once, and both bypass the caches' retention: 8192 tokens of 32 + 2 * 8 heads
+// 40.2 -> 36.6 us (5.5 TB/s, the rate of a large copy).  Two and four rows per lane
+// group, to read a position's angles and the weights once for them, gave up to 2 % on
+// 8192 tokens and cost a small call 0.3 and 1.1 us of 2.5.
+template <int D>
 __global__ __launch_bounds__(256) void paged_prologue_kernel(PagedPrologueArgs a, uint32_t parts) {
     constexpr int LPR = D / 16, G = 64 / LPR, HALF = D / 2;
     const uint32_t unit = blockIdx.x * 4 + (threadIdx.x >> 6);
     const uint32_t t = unit / parts, part = unit % parts;
     if (t >= a.num_tokens) return;
     const int lane = threadIdx.x & 63, c = lane % LPR;
-    const uint32_t j0 = part * (G * U) + lane / LPR;
-    const uint32_t rows = a.hq + 2 * a.hkv;
+    // Row j of the token: of q, then k, then v; past the last one: that.
+    const uint32_t rows = a.hq + 2 * a.hkv, row = part * G + lane / LPR, j = min(row, rows - 1);
+    const bool is_q = j < a.hq, is_k = !is_q && j < a.hq + a.hkv;
+    const uint32_t heads = is_q ? a.hq : a.hkv, head = j - (is_q ? 0 : is_k ? a.hq : a.hq + a.hkv);
     const uint32_t pos = min(a.positions[t], a.num_positions - 1);
     const uint32_t slot = a.slots[t];
-    uint4 xr[U], xi[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const uint32_t j = min(j0 + u * G, rows - 1);
-        const uint16_t* src = j < a.hq           ? a.q + ((uint64_t)t * a.hq + j) * D
-                              : j < a.hq + a.hkv ? a.k + ((uint64_t)t * a.hkv + (j - a.hq)) * D
-                                                 : a.v + ((uint64_t)t * a.hkv + (j - a.hq - a.hkv)) * D;
-        xr[u] = ldg16_nt(src + 8 * c);
-        xi[u] = ldg16_nt(src + 8 * c + HALF);
-    }
+    const uint64_t at = ((uint64_t)t * heads + head) * D;
+    const uint16_t* src = (is_q ? a.q : is_k ? a.k : a.v) + at;
+    uint4 xr = ldg16_nt(src + 8 * c), xi = ldg16_nt(src + 8 * c + HALF);
     const uint4 qwr = ldg16(a.q_weight + 8 * c), qwi = ldg16(a.q_weight + 8 * c + HALF);
     const uint4 kwr = ldg16(a.k_weight + 8 * c), kwi = ldg16(a.k_weight + 8 * c + HALF);
     float4 cs[4];
@@ -187,60 +181,50 @@ __global__ __launch_bounds__(256) void paged_prologue_kernel(PagedPrologueArgs a
     for (int k = 0; k < 4; ++k) cs[k] = rope[k];
     const uint64_t cache_row = (uint64_t)(slot >> a.page_shift) * a.page_stride +
                                (uint64_t)(slot & ((1u << a.page_shift) - 1)) * a.hkv * D;
+    if (is_q || is_k) {
+        float re[8], im[8], ss = 0.0f;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const uint32_t j = j0 + u * G;
-        if (j < a.hq + a.hkv) {
-            float re[8], im[8], ss = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                re[2 * k] = bf16_lo(word_of(xr[u], k));
-                re[2 * k + 1] = bf16_hi(word_of(xr[u], k));
-                im[2 * k] = bf16_lo(word_of(xi[u], k));
-                im[2 * k + 1] = bf16_hi(word_of(xi[u], k));
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) ss = fmaf(re[k], re[k], fmaf(im[k], im[k], ss));
-            // The LPR lanes of a row share a j and so take this branch together.
-            ss += dpp_f32<kDppXor1>(ss);
-            ss += dpp_f32<kDppXor2>(ss);
-            if constexpr (LPR == 8) ss += dpp_f32<kDppRowHalfMirror>(ss);
-            const float inv = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
-            const bool is_q = j < a.hq;
-            uint32_t wr[4], wi[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t gr = is_q ? word_of(qwr, k) : word_of(kwr, k);
-                const uint32_t gi = is_q ? word_of(qwi, k) : word_of(kwi, k);
-                const float r0 = re[2 * k] * inv * bf16_lo(gr), r1 = re[2 * k + 1] * inv * bf16_hi(gr);
-                const float i0 = im[2 * k] * inv * bf16_lo(gi), i1 = im[2 * k + 1] * inv * bf16_hi(gi);
-                // Rounded here only: the unfused sequence rounds the norm's
-                // result as well.
-                wr[k] = pack_bf16x2(cs[k].x * r0 - cs[k].y * i0, cs[k].z * r1 - cs[k].w * i1);
-                wi[k] = pack_bf16x2(cs[k].x * i0 + cs[k].y * r0, cs[k].z * i1 + cs[k].w * r1);
-            }
-            xr[u] = make_uint4(wr[0], wr[1], wr[2], wr[3]);
-            xi[u] = make_uint4(wi[0], wi[1], wi[2], wi[3]);
+        for (int k = 0; k < 4; ++k) {
+            re[2 * k] = bf16_lo(word_of(xr, k));
+            re[2 * k + 1] = bf16_hi(word_of(xr, k));
+            im[2 * k] = bf16_lo(word_of(xi, k));
+            im[2 * k + 1] = bf16_hi(word_of(xi, k));
         }
-        uint16_t* dst = nullptr;
-        if (j < a.hq)
-            dst = a.q_out + ((uint64_t)t * a.hq + j) * D;
-        else if (j < rows && slot < a.num_slots)
-            dst = j < a.hq + a.hkv ? a.k_cache + cache_row + (uint64_t)(j - a.hq) * D
-                                   : a.v_cache + cache_row + (uint64_t)(j - a.hq - a.hkv) * D;
-        if (dst) {
-            stg16_nt(dst + 8 * c, xr[u]);
-            stg16_nt(dst + 8 * c + HALF, xi[u]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) ss = fmaf(re[k], re[k], fmaf(im[k], im[k], ss));
+        // The LPR lanes of a row share a row and so take this branch together.
+        ss += dpp_f32<kDppXor1>(ss);
+        ss += dpp_f32<kDppXor2>(ss);
+        if constexpr (LPR == 8) ss += dpp_f32<kDppRowHalfMirror>(ss);
+        const float inv = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
+        uint32_t wr[4], wi[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t gr = is_q ? word_of(qwr, k) : word_of(kwr, k);
+            const uint32_t gi = is_q ? word_of(qwi, k) : word_of(kwi, k);
+            const float r0 = re[2 * k] * inv * bf16_lo(gr), r1 = re[2 * k + 1] * inv * bf16_hi(gr);
+            const float i0 = im[2 * k] * inv * bf16_lo(gi), i1 = im[2 * k + 1] * inv * bf16_hi(gi);
+            // Rounded here only: the unfused sequence rounds the norm's
+            // result as well.
+            wr[k] = pack_bf16x2(cs[k].x * r0 - cs[k].y * i0, cs[k].z * r1 - cs[k].w * i1);
+            wi[k] = pack_bf16x2(cs[k].x * i0 + cs[k].y * r0, cs[k].z * i1 + cs[k].w * r1);
         }
+        xr = make_uint4(wr[0], wr[1], wr[2], wr[3]);
+        xi = make_uint4(wi[0], wi[1], wi[2], wi[3]);
+    }
+    if (row < rows && (is_q || slot < a.num_slots)) {
+        uint16_t* dst = (is_q ? a.q_out : is_k ? a.k_cache : a.v_cache) + (is_q ? at : cache_row + (uint64_t)head * D);
+        stg16_nt(dst + 8 * c, xr);
+        stg16_nt(dst + 8 * c + HALF, xi);
     }
 }
 
-template <int D, int U>
+template <int D>
 hipError_t launch_prologue_t(const PagedPrologueArgs& a, hipStream_t st) {
     constexpr uint32_t G = 64 / (D / 16);
-    const uint32_t parts = (a.hq + 2 * a.hkv + G * U - 1) / (G * U);
+    const uint32_t parts = (a.hq + 2 * a.hkv + G - 1) / G;
     const uint64_t units = (uint64_t)a.num_tokens * parts;
-    hipLaunchKernelGGL((paged_prologue_kernel<D, U>), dim3((uint32_t)((units + 3) / 4)), dim3(256), 0, st, a, parts);
+    hipLaunchKernelGGL((paged_prologue_kernel<D>), dim3((uint32_t)((units + 3) / 4)), dim3(256), 0, st, a, parts);
     return hipGetLastError();
 }
 
@@ -255,7 +239,7 @@ hipError_t launch_paged_tables(const PagedTablesArgs& a, hipStream_t stream) {
 }
 
 hipError_t launch_paged_prologue(const PagedPrologueArgs& a, uint32_t d, hipStream_t stream) {
-    return d == 64 ? launch_prologue_t<64, 1>(a, stream) : launch_prologue_t<128, 1>(a, stream);
+    return d == 64 ? launch_prologue_t<64>(a, stream) : launch_prologue_t<128>(a, stream);
 }
 
 }  // namespace tiattn
