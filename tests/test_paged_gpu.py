@@ -495,3 +495,18 @@ def test_attention_graph_and_streams(dev):
         st.attend()
         H.sync()
         assert torch.equal(st.o.cpu().double(), got)
+
+
+def test_tables_idle_requests_are_not_refused(dev):
+    """Requests without new tokens, the padding of a batch, behind one whose rows
+    do not fit: one is refused."""
+    context, new = [0, 0, 0, 40, 7], [9, 9, 9, 0, 0]
+    out = [ints([0] * 24, dev) for _ in range(5)]
+    bt = ints(np.zeros((5, 8)), dev)
+    attn.paged_tables_u32(ints(context, dev), ints(new, dev), 5, ints(range(20), dev), 20,
+                          ints([20], dev), 8, bt, 8, 20, *out)
+    H.sync()
+    start, seq, pos, slots, status = (host(t) for t in out)
+    assert start[:6] == [0, 9, 18, 27, 27, 27] and seq[:5] == [9, 9, 0, 40, 7]
+    assert status[:2] == [16, 1]
+    assert pos[:20] == [*range(9), *range(9), 0, 1] and slots[18:20] == [0xFFFFFFFF] * 2

@@ -78,7 +78,8 @@ __global__ __launch_bounds__(kTabThreads) void paged_tables_kernel(PagedTablesAr
         tokens += sum_n;
         pages += sum_p;
         if (has) {
-            const bool ok = end <= a.max_blocks && st + n <= a.num_tokens &&
+            // (A request without new tokens has no rows that could pass num_tokens.)
+            const bool ok = end <= a.max_blocks && (n == 0 || st + n <= a.num_tokens) &&
                             (need == 0 || first + need <= num_free);
             s_start[b] = clamp32(st);
             s_first[b] = ok ? (uint32_t)(need ? first : 0) : kNoSlot;
