@@ -19,3 +19,14 @@ def test_dropin_header_program():
     assert res.returncode == 0, res.stdout[-3000:] + res.stderr[-2000:]
     assert "ALL PASS" in res.stdout
     assert res.stdout.count("[PASS]") >= 40
+
+
+def test_paged_header_program():
+    """The header's paged-cache calls: steps of a server, eager and captured."""
+    program = os.path.join(os.path.dirname(BIN), "paged_test")
+    assert os.path.exists(program), "tests/dropin/paged_test is missing: run __graft_entry__.build()"
+    res = subprocess.run([program], capture_output=True, text=True, timeout=120)
+    print(res.stdout, res.stderr, flush=True)
+    assert res.returncode == 0, res.stdout[-3000:] + res.stderr[-2000:]
+    assert "ALL PASS" in res.stdout
+    assert res.stdout.count("[PASS]") == 40
