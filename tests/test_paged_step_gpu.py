@@ -617,3 +617,29 @@ def test_binding_refuses_caches_of_other_layouts(dev):
                                              1e-6, st.q_d, k, v, st.pages, st.ps, st.stride, 8, 2, 128)
     H.sync()
     assert (st.o == 3.0).all() and (apart == 0).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (9000, 100)])
+def test_long_contexts_miss_no_tile(dev, window, sinks, d):
+    """Over tens of thousands of keys each weighs less than the elements' bound
+    can see; the RMS over a request's elements sees a tile.  Its limit: a
+    weight's rounding moves an element by at most 2^-8 w_j |v_j|, of random sign,
+    which over the keys is 2^-8 of the output's own RMS, and the output's
+    rounding is 2^-8 of it again: sqrt(2) 2^-8, below 2^-7.  64 of 33000 keys are
+    4 % of it, which the same limit finds in an oracle that leaves them out."""
+    st = Wide(dev, [(40001, 1), (20000, 33), (33000, 9)], 8, 2, d, 16, window, sinks, seed=d)
+    st.run()
+    rms = lambda x: x.square().mean().sqrt().item()
+    for b, (length, n) in enumerate(st.requests):
+        rows = slice(int(st.start[b]), int(st.start[b + 1]))
+        k, v = (x.to(dev) for x in st.kv[b])
+        o, _ = wide_attention(st.q_d[rows], k, v, window, sinks)
+        error = rms(st.o[rows].double() - o) / rms(o)
+        print(f"[paged] {length} keys, window {window}, D={d}: RMS {error:.5f}", flush=True)
+        assert error < 2.0 ** -7, b
+        gone = v.clone()
+        first = length - length % 64 - 4 * 64
+        gone[first:first + 64] = 0
+        without, _ = wide_attention(st.q_d[rows], k, gone, window, sinks)
+        assert rms(without - o) / rms(o) > 2.0 ** -7, b
