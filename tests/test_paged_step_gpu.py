@@ -554,15 +554,21 @@ def test_values_that_are_not_finite(dev, case):
         check_nan(st, at)
 
 
-def test_more_spoilt_blocks_than_marks(dev):
+@pytest.mark.parametrize("hq,d,requests", [
+    (32, 64, [(5000, 5000), (900, 1)]),
+    (64, 128, [(3300, 2300)]),
+])
+def test_more_spoilt_blocks_than_marks(dev, hq, d, requests):
     """NaN in one dim of every seventh token: more blocks of rows to compute again
-    than a call keeps apart."""
-    st = Wide(dev, [(5000, 5000), (900, 1)], 32, 32, 64, 16, seed=3)
-    at = [(0, j, 11, NAN) for j in range(3, 5000, 7)]
+    than a call keeps apart, some of them of units in pieces."""
+    st = Wide(dev, requests, hq, hq, d, 16, seed=3)
+    at = [(0, j, 11, NAN) for j in range(3, requests[0][0], 7)]
     put_nan(st, at)
     st.make_plan()
     st.attend()
     H.sync()
+    print(f"[paged] more than the marks: {hq}/{hq} D={d}: {shape_of(st)}", flush=True)
+    assert shape_of(st)[1]
     check_nan(st, at)
 
 
