@@ -1372,6 +1372,11 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedAttnArg
             plan_load<PagedSplitBlock>(a.plan, lay.split_blocks + (uint64_t)(i / (DBLK * hkv)) * sizeof(PagedSplitBlock));
         const uint64_t b0 = (uint64_t)kvh * paged_partial_blocks(hkv) + sb.first;
         const bool has = (uint32_t)(lane & 31) < sb.rows;
+        // The place of this lane's row in o, found while the loads below are on
+        // their way.
+        const uint32_t r = sb.row0 + (lane & 31), token = sb.token0 + r / group, h = kvh * group + r % group;
+        uint64_t at = ((uint64_t)token * a.head.hq + h) * D + 32 * db + 8 * wave + 4 * (lane >> 5);
+        asm volatile("" : "+v"(at));
         float M = -INFINITY, den = 0.0f;
         float4 acc[4];
 #pragma unroll
@@ -1430,12 +1435,9 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedAttnArg
         const float inv = tot == 0.0f ? 0.0f : 1.0f / tot;
         // (Marked blocks are written below only.)
         if (met && (all_marked || marked(marks, sb.req, sb.token0 + sb.row0 / group, sb.row0 % group, kvh))) continue;
-        if (has) {
-            const uint32_t r = sb.row0 + (lane & 31), token = sb.token0 + r / group, h = kvh * group + r % group;
-            uint16_t* o = a.o + ((uint64_t)token * a.head.hq + h) * D + 32 * db + 8 * wave + 4 * (lane >> 5);
-            *reinterpret_cast<uint2*>(o) =
+        if (has)
+            *reinterpret_cast<uint2*>(a.o + at) =
                 make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
-        }
     }
     if (!met) return;
     // The rows of the marked blocks, each block by its first mark.
