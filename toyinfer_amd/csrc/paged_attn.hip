@@ -30,9 +30,11 @@
 //   streaming, 32 requests of 2208..8193 keys (704 MB): 114 us, 6.2 TB/s of keys
 //     and values where a contiguous cache streams at 6.5; 64 KB of loads in flight per
 //     compute unit is what LDS leaves beside the merge;
-//   > 128 rows, a prompt of 8192: 511 to 522 us, 1.05 to 1.07 PFLOP/s; matrix cores busy for 49 %
-//     of the cycles, waves waiting for 29 %.  Lanes end up to 6 % from their mean; the
-//     contiguous prefill attention, without pages and lists, takes 480.
+//   > 128 rows, a prompt of 8192: 523 to 544 us from card to card, 1.01 to 1.05 PFLOP/s;
+//     matrix cores busy for 48 % of the cycles, waves waiting for 29 %.  Lanes end up to
+//     6 % from their mean; the contiguous prefill attention, without pages and lists,
+//     takes 480 to 494;
+//   streaming at head_dim 64, half the bytes in flight: 32 such requests 66 us, 5.3 TB/s.
 // What a SIMD's two waves do is in step, from barrier to barrier.  Two groups of
 // waves half a tile apart, so that one multiplies while the other takes
 // exponentials, took 577 us with one barrier per tile and 601 with two.
@@ -162,6 +164,8 @@ __device__ __forceinline__ void probabilities(f32x16_t (&st)[NB], RowState<D>& s
             for (int j = 0; j < 8; ++j)
                 e[j] = __builtin_amdgcn_exp2f(fmaf(st[tt / 2][8 * (tt & 1) + j], scale_log2, -mref));
             // P.V multiplies the bf16 probabilities, so the sum is taken of those.
+            // (Against 64 bits the output is then off by 0.0023 of its RMS, where
+            // its own rounding to bf16 alone is 0.0017.)
             const uint4 w = make_uint4(pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3]), pack_bf16x2(e[4], e[5]),
                                        pack_bf16x2(e[6], e[7]));
             pf[tt] = as_bf16x8(w);
