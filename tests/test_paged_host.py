@@ -183,3 +183,4 @@ def test_binding_takes_one_page_and_one_head():
         attn._need_cache("paged", -1, 2, 8, 8 * 4 * 64, 1, 64, wide[:, :, 1:2])
     head = torch.zeros(3, 8, 64, dtype=torch.bfloat16)[:, :, None]
     attn._need_cache("paged", -1, 3, 8, 8 * 64, 1, 64, head)
+    attn._need_cache("paged", -1, 1, 8, 8 * 2 * 64, 2, 64, one.view(1, 8, 128))  # heads and dims in one

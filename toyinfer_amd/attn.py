@@ -530,7 +530,8 @@ def _dense_in_pages(t, num_pages: int, page_size: int, page_stride: int, num_kv_
     do: in one piece up to a page, the next one page_stride on."""
     inner = (page_size, num_kv_heads, head_dim)
     page = page_size * num_kv_heads * head_dim
-    if t.dim() >= 3 and t.shape[-3:].numel() == page and t.shape[-3:] != inner:
+    last = tuple(t.shape[-3:])
+    if last != inner and sorted(last) == sorted(inner):
         return False  # [heads][rows], say
     dense = 1
     for size, stride in zip(reversed(t.shape), reversed(t.stride())):
