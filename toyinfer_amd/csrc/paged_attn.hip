@@ -1354,7 +1354,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_kernel(PagedAttnArg
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t met = scalar_load(a.flags), marks = min(met, kPagedMarks);
     const bool all_marked = met > kPagedMarks;
-    // Whether one of the first n marks is of this block, of the workgroup's row.
+    // Whether one of the first n marks names this block; the same answer to all threads.
     auto marked = [&](uint32_t n, uint32_t req, uint32_t token, uint32_t h, uint32_t kvh) {
         bool is = false;
         for (uint32_t i = threadIdx.x; i < n; i += kMergeThreads) {
