@@ -472,6 +472,64 @@ int toyinfer_paged_attention_bf16(const void* q, const void* k_cache, const void
                                   uint32_t heads_dim, void* workspace, size_t workspace_bytes,
                                   void* stream);
 
+/* The same cache in 8 bits.  A page is a record of bytes: its codes
+ * [Hkv][page_size][D], then its scales, fp32 [Hkv][page_size/16], one for each
+ * block of 16 rows and head; page_stride is in bytes, a multiple of 16 and at
+ * least toyinfer_paged_fp8_page_bytes (0 for sizes that are not supported).
+ * page_size is a power of two in 16..65536.  Codes are e4m3 (largest 448, 0x7f
+ * and 0xff NaN, no infinities), a scale is a power of two, 2^-100 .. 2^119, and a
+ * value code * scale, which bf16 holds exactly.  The caches need no
+ * initialisation.  Tables, plan and workspace are those above, a plan serves
+ * caches of either kind, and so do the limits ((num_pages - 1) * page_stride <=
+ * 2^47, page_stride < 2^41 here). */
+size_t toyinfer_paged_fp8_page_bytes(uint32_t page_size, uint32_t num_kv_heads, uint32_t head_dim);
+
+/* toyinfer_paged_qkv_prologue_bf16 into 8-bit caches; q_out stays bf16.  Of each
+ * block and head that it writes into, a call makes the scale the smallest with
+ * which the largest finite value that it writes there is at most 448 * scale, if
+ * it writes the block's first row; else that or, where it is larger, the block's
+ * scale of before, and if the scale grows the block's other rows are rounded to
+ * it.  Values are rounded once, to the nearest code, halves to even; finite ones
+ * above 448 * 2^119 become that, infinities NaN.  So rows are written in order:
+ * a block's later rows mean nothing once its first row is written again.
+ * Tokens whose slots lie in one block are neighbours in slot_mapping, with none
+ * between them that lies elsewhere or has no slot, and slots of one call distinct
+ * (of blocks where they are not, K's and V's bytes are unspecified). */
+int toyinfer_paged_qkv_prologue_fp8(const void* q, const void* k, const void* v,
+                                    const void* q_norm_weight, const void* k_norm_weight,
+                                    const float* rope_cos_sin, uint32_t num_positions,
+                                    const uint32_t* positions, const uint32_t* slot_mapping,
+                                    uint32_t num_tokens, float rms_norm_eps, void* q_out,
+                                    void* k_cache, void* v_cache, uint32_t num_pages,
+                                    uint32_t page_size, uint64_t page_stride,
+                                    uint32_t num_q_heads, uint32_t num_kv_heads,
+                                    uint32_t head_dim, void* stream);
+
+/* Rows of 8-bit caches as bf16, without rounding: k_out and v_out
+ * [num_tokens][Hkv][D].  Rows query_start[b] .. query_start[b+1] are the last
+ * query_start[b+1] - query_start[b] tokens of request b's seq_lens[b], as for the
+ * attention; with sums of seq_lens for query_start they are its whole context.
+ * Rows of tokens before position 0 are 0, rows past query_start[batch] are left
+ * as they are.  The arrays may hold anything, as for the attention.  k_out and
+ * v_out overlap nothing else. */
+int toyinfer_paged_kv_read_fp8(const void* k_cache, const void* v_cache,
+                               const uint32_t* block_tables, const uint32_t* query_start,
+                               const uint32_t* seq_lens, uint32_t batch, uint32_t num_tokens,
+                               void* k_out, void* v_out, uint32_t num_pages, uint32_t page_size,
+                               uint64_t page_stride, uint32_t max_blocks, uint32_t num_kv_heads,
+                               uint32_t head_dim, void* stream);
+
+/* toyinfer_paged_attention_bf16 over 8-bit caches: q and o are bf16, keys and
+ * values enter the products as they read back. */
+int toyinfer_paged_attention_fp8(const void* q, const void* k_cache, const void* v_cache, void* o,
+                                 const uint32_t* block_tables, const void* plan,
+                                 size_t plan_bytes, uint32_t batch, uint32_t num_tokens,
+                                 uint32_t num_pages, uint32_t page_size, uint64_t page_stride,
+                                 uint32_t max_blocks, uint32_t window, uint32_t sinks,
+                                 uint32_t num_q_heads, uint32_t num_kv_heads,
+                                 uint32_t heads_dim, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,635 @@
+"""The 8-bit paged cache on the GPU.
+
+V's codes and scales have to be the oracle's bit for bit: a value is bf16, its
+code the nearest.  K's scale and codes come from fp32 values that are off by at
+most 2^-16 of the rotation's products (the prologue's norm and rotation): the
+scale is the one of a largest value inside that error, a code off by half a step
+more, 2^-4 of the value or 2^-10 of the scale.  Reading back is exact.
+
+Keys and values enter the attention's products without a rounding of their own,
+so its bounds are those of the bf16 cache over the values that the codes stand
+for.
+"""
+import numpy as np
+import pytest
+import torch
+
+from tests import fp8_oracle as F8
+from tests import helpers as H
+from tests import paged_oracle as PO
+from tests.test_paged_gpu import BATCHES, HEADS, Step, host, ints
+from tests.test_paged_step_gpu import (EARLY, FORMS, SPOILT, Early, Wide, check_nan, check_rows,
+                                       shape_of, wide_attention)
+from toyinfer_amd import attn
+
+pytestmark = pytest.mark.gpu
+
+POSITIONS = 97
+
+
+def bf16(x):
+    return torch.from_numpy(np.asarray(x, np.float64)).to(torch.bfloat16)
+
+
+# ------------------------------------------------------------------- write
+
+class Writer:
+    """K and V caches on the GPU beside the oracle's, and calls that go to both."""
+
+    def __init__(self, dev, pages, ps, hq, hkv, d, seed=0, apart=0, interleaved=False):
+        self.dev, self.pages, self.ps, self.hq, self.hkv, self.d = dev, pages, ps, hq, hkv, d
+        self.rng = np.random.default_rng(seed)
+        page = F8.page_bytes(ps, hkv, d) + apart
+        self.k, self.v = (F8.Cache(pages, ps, hkv, d, page) for _ in range(2))
+        if interleaved:
+            both = torch.from_numpy(np.stack([self.k.raw, self.v.raw], 1)).to(dev)
+            self.k_d, self.v_d = both[:, 0], both[:, 1]
+        else:
+            self.k_d, self.v_d = (torch.from_numpy(c.raw.copy()).to(dev) for c in (self.k, self.v))
+        self.qw, self.kw = (bf16(self.rng.uniform(0.5, 1.5, d)) for _ in range(2))
+        self.rope = torch.from_numpy(self.rng.uniform(-1, 1, (POSITIONS, d // 2, 2))).float()
+
+    def rows(self, t, std=1.0):
+        return bf16(self.rng.standard_normal((t, self.hkv, self.d)) * std)
+
+    def launch(self, q, k, v, pos, slots, q_out, stream=None):
+        attn.paged_qkv_prologue_fp8(q, k, v, self.qw.to(self.dev), self.kw.to(self.dev),
+                                    self.rope.to(self.dev), POSITIONS, pos, slots, slots.numel(),
+                                    1e-6, q_out, self.k_d, self.v_d, self.pages, self.ps,
+                                    self.k_d.stride(0), self.hq, self.hkv, self.d, stream)
+
+    def write(self, slots, k=None, v=None):
+        """One call, checked against the oracle's."""
+        t, hkv, d = len(slots), self.hkv, self.d
+        slots = np.asarray(slots, np.uint32)
+        k = self.rows(t, 3.0) if k is None else k
+        v = self.rows(t) if v is None else v
+        q = bf16(self.rng.standard_normal((t, self.hq, d)) * 2)
+        pos = self.rng.integers(0, POSITIONS + 3, t)
+        q_out = torch.empty_like(q, device=self.dev)
+        self.launch(q.to(self.dev), k.to(self.dev), v.to(self.dev), ints(pos, self.dev),
+                    ints(slots, self.dev), q_out)
+        H.sync()
+        cs = self.rope.double().numpy()[np.minimum(pos, POSITIONS - 1)]
+        wide = np.abs(cs).sum(-1)
+
+        def turned(x, w):
+            x, w = x.double().numpy(), w.double().numpy()
+            y = np.abs(PO.rms_rope(x, w, np.stack([np.ones_like(wide), np.zeros_like(wide)], -1), 1e-6))
+            terms = np.tile((y[..., :d // 2] + y[..., d // 2:]) * wide[:, None], 2)
+            return PO.rms_rope(x, w, cs, 1e-6), 2.0 ** -16 * terms
+
+        exp, off = turned(q, self.qw)
+        got = q_out.cpu().double().numpy()
+        assert (np.abs(got - exp) <= 2.0 ** -8 * np.abs(exp) * 1.001 + off).all(), "q"
+        self.v.write(slots, v.double().numpy())
+        assert (self.v_d.cpu().numpy() == self.v.raw).all(), "V's bytes"
+        self.check_k(slots, *turned(k, self.kw))
+
+    def check_k(self, slots, x, off):
+        now = F8.Cache(self.pages, self.ps, self.hkv, self.d, self.k.raw.shape[1])
+        now.raw = self.k_d.cpu().numpy().copy()
+        by_block = {}
+        for t, s in enumerate(int(i) for i in slots):
+            if s < self.pages * self.ps:
+                by_block.setdefault(s // F8.BLOCK, []).append(t)
+        exponents = {}
+        for block, ts in by_block.items():
+            page, b = divmod(block, self.ps // F8.BLOCK)
+            opens = any(int(slots[t]) % F8.BLOCK == 0 for t in ts)
+            for h in range(self.hkv):
+                e = F8.POWERS[now.scale(page, h, b)]
+                lo = F8.exponent_for(max((np.abs(x[t, h]) - off[t, h]).max() for t in ts))
+                hi = F8.exponent_for(max((np.abs(x[t, h]) + off[t, h]).max() for t in ts))
+                old = self.k.scale(page, h, b)
+                if not opens and old in F8.POWERS:
+                    lo, hi = max(lo, F8.POWERS[old]), max(hi, F8.POWERS[old])
+                assert lo <= e <= hi, (block, h, lo, e, hi)
+                exponents[block, h] = e
+        live = [t for t, s in enumerate(slots) if s < self.pages * self.ps]
+        for t in live:
+            s = int(slots[t])
+            e = np.array([exponents[s // F8.BLOCK, h] for h in range(self.hkv)])[:, None]
+            half = np.maximum(2.0 ** -4 * (np.abs(x[t]) + off[t]), 2.0 ** (e - 10.0))
+            assert (np.abs(now.row(s) - x[t]) <= half + off[t]).all(), ("K", t)
+        # All other bytes: the oracle's, with these scales.
+        self.k.write(slots, x, exponents)
+        for t in live:
+            page, r = divmod(int(slots[t]), self.ps)
+            self.k.put_codes(page, r, now.codes()[page, :, r])
+        assert (now.raw == self.k.raw).all(), "K's other bytes"
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(16, 8, 128), (5, 1, 64), (12, 2, 64), (1, 1, 128), (6, 3, 128)])
+@pytest.mark.parametrize("t", [1, 7, 16, 17, 130])
+def test_write_prompt(dev, hq, hkv, d, t):
+    """Prompts that begin at each kind of place in a block, into pages in any
+    order, a row at the edge of a block and the last without a slot."""
+    print(f"[fp8] write {hq}/{hkv} D={d} t={t}", flush=True)
+    for first in (0, 3, 15):
+        w = Writer(dev, t // 16 + 5, 16, hq, hkv, d, seed=t + first)
+        pages = w.rng.permutation(w.pages)
+        at = first + np.arange(t)
+        slots = (pages[at // 16] * 16 + at % 16).astype(np.uint32)
+        if t > 20:
+            slots[32 - first], slots[t - 1] = 0xFFFFFFFF, w.pages * 16
+        if first:
+            w.write(pages[0] * 16 + np.arange(first))
+        w.write(slots)
+
+
+@pytest.mark.parametrize("ps", [16, 32, 256])
+@pytest.mark.parametrize("d", [64, 128])
+def test_write_steps(dev, ps, d):
+    """Decoded tokens of 40 requests, values that grow and shrink from step to
+    step: blocks grow, keep their scale and open, in pages further apart than
+    they are long, K's beside V's."""
+    w = Writer(dev, 40, ps, 4, 2, d, seed=ps, apart=48, interleaved=True)
+    first = w.rng.integers(0, ps - 12, 40)
+    w.write(np.concatenate([p * ps + f // 16 * 16 + np.arange(f % 16) for p, f in enumerate(first)]))
+    for step, std in enumerate((1.0, 8.0, 0.01, 300.0, 1e4, 1.0, 3e-5)):
+        slots = np.arange(40) * ps + first + step
+        w.write(slots, v=w.rows(40, std), k=w.rows(40, std))
+
+
+def test_write_drafted_tokens(dev):
+    """Several tokens per request, rewritten from the middle of a block on, runs
+    that cross the boundary of a wave's rows."""
+    w = Writer(dev, 12, 16, 2, 2, 128, seed=2)
+    w.write(np.concatenate([p * 16 + np.arange(9) for p in range(12)]))
+    for start, n in ((9, 4), (10, 5), (3, 2), (9, 7)):
+        w.write(np.concatenate([p * 16 + start + np.arange(n) for p in range(12)]), v=w.rows(12 * n, 2.0 ** n))
+    w.write(np.concatenate([p * 16 + np.arange(16) for p in (3, 1)]))  # opens again
+
+
+def test_write_rows_of_a_block_in_another_order(dev):
+    """Neighbouring rows of one block need not ascend, nor leave no gaps."""
+    w = Writer(dev, 4, 16, 2, 2, 64, seed=5)
+    w.write(np.arange(16) + 16)
+    w.write([31, 17, 25, 40, 33], v=w.rows(5, 50.0))
+    w.write(np.arange(16)[::-1] + 48)
+
+
+def test_write_values_at_the_edges(dev):
+    """NaN, infinities, zeros, the largest and the smallest bf16, values at the
+    borders of a scale and between two codes."""
+    w = Writer(dev, 3, 16, 1, 1, 64, seed=1)
+    v = np.zeros((12, 1, 64))
+    v[1] = 3.3e38 * (1 - 2 * (np.arange(64) % 2))
+    v[2, 0, :3] = np.inf, -np.inf, np.nan
+    v[3] = 2.0 ** -133
+    v[4], v[5, 0, 0], v[5, 0, 1:] = 448, 450, 2.0 ** -5 * np.arange(63)
+    v[6] = np.arange(64) * 7.0
+    w.write(np.arange(16, 17), v=bf16(v[:1]))          # zeros open a block
+    for i in range(1, 12):
+        w.write([16 + i], v=bf16(v[i:i + 1]))          # one after the other
+    w.write(np.arange(32, 36), v=bf16(v[3:7]))
+    w.write(np.arange(36, 40), v=bf16(v[8:12]))
+    w.write([0], v=bf16(v[2:3]))
+
+
+def test_write_many_tokens(dev):
+    w = Writer(dev, 80, 64, 8, 4, 128, seed=9)
+    pages = w.rng.permutation(80)
+    at = np.arange(4000) + 500
+    w.write((pages[at // 64] * 64 + at % 64).astype(np.uint32))
+
+
+def test_write_in_place_and_again(dev):
+    """q_out may be q, and a call gives the same bytes every time."""
+    w = Writer(dev, 9, 16, 4, 2, 128)
+    slots = np.arange(100) + 7
+    q = bf16(w.rng.standard_normal((100, 4, 128))).to(dev)
+    k, v, pos = w.rows(100).to(dev), w.rows(100).to(dev), ints(np.arange(100) % POSITIONS, dev)
+    res = []
+    for i in range(4):
+        w.k_d.fill_(255)
+        w.v_d.fill_(255)
+        mine = q.clone()
+        out = mine if i % 2 else torch.empty_like(q)
+        w.launch(mine, k, v, pos, ints(slots, dev), out)
+        res.append((out, w.k_d.clone(), w.v_d.clone()))
+    H.sync()
+    for r in res[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, res[0]))
+
+
+def test_write_same_slot_twice(dev):
+    """Tokens that share a slot spoil no other block."""
+    w = Writer(dev, 6, 16, 2, 2, 128, seed=3)
+    before = w.k_d.clone()
+    slots = np.concatenate([np.full(50, 20), [33, 33, 34], np.arange(48, 52)]).astype(np.uint32)
+    t = len(slots)
+    q = bf16(w.rng.standard_normal((t, 2, 128))).to(dev)
+    v = w.rows(t)
+    w.launch(q, w.rows(t).to(dev), v.to(dev), ints(np.arange(t), dev), ints(slots, dev), torch.empty_like(q))
+    H.sync()
+    for page in (0, 4, 5):
+        assert torch.equal(w.k_d[page], before[page])
+    w.v.write(np.arange(48, 52), v[-4:].double().numpy())
+    assert (w.v_d[3].cpu().numpy() == w.v.raw[3]).all()
+
+
+# -------------------------------------------------------------------- read
+
+def read_back(dev, k, v, table, start, lens, rows, ps, blocks, hkv, d, fill=5.0):
+    out = [torch.full((rows, hkv, d), fill, dtype=torch.bfloat16, device=dev) for _ in range(2)]
+    attn.paged_kv_read_fp8(k, v, table, ints(start, dev), ints(lens, dev), len(lens), rows, *out,
+                           k.shape[0], ps, k.stride(0), blocks, hkv, d)
+    H.sync()
+    return [x.cpu() for x in out]
+
+
+@pytest.mark.parametrize("hkv,d,ps", [(8, 128, 16), (1, 64, 16), (3, 64, 128), (5, 128, 32)])
+def test_read(dev, hkv, d, ps):
+    """Every code under scales of every size, contexts of any length, the last
+    tokens of others, more of them than there are, rows behind the last."""
+    rng = np.random.default_rng(ps + d)
+    lens, news = [1, 200, 17, 0, 64, 333, 5], [1, 30, 17, 0, 64, 333, 9]
+    need = [-(-x // ps) for x in lens]
+    pages, blocks = sum(need) + 1, max(need) + 1
+    caches = []
+    for _ in range(2):
+        c = F8.Cache(pages, ps, hkv, d)
+        c.raw[:] = rng.integers(0, 256, c.raw.shape)
+        for p in range(pages):
+            for h in range(hkv):
+                for b in range(ps // 16):
+                    c.put_scale(p, h, b, 2.0 ** rng.integers(F8.LOW, F8.HIGH + 1))
+        caches.append(c)
+    order, table, at = rng.permutation(pages), np.full((len(lens), blocks), 0xFFFFFFFF, np.uint32), 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[at:at + n]
+        at += n
+    start = np.concatenate([[0], np.cumsum(news)])
+    got = read_back(dev, *(torch.from_numpy(c.raw).to(dev) for c in caches), ints(table, dev), start,
+                    lens, int(start[-1]) + 4, ps, blocks, hkv, d)
+    for g, c in zip(got, caches):
+        g = g.double().numpy()
+        assert (g[start[-1]:] == 5).all()
+        for b, (length, n) in enumerate(zip(lens, news)):
+            for i in range(n):
+                j = length - n + i
+                row = g[start[b] + i]
+                if j < 0:
+                    assert (row == 0).all()
+                else:
+                    want = c.row(int(table[b, j // ps]) * ps + j % ps)
+                    assert np.array_equal(row, want, equal_nan=True), (b, j)
+
+
+@pytest.mark.parametrize("batch", [1, 2, 255, 4096])
+def test_read_batches(dev, batch):
+    rng = np.random.default_rng(batch)
+    lens = rng.integers(0, 5, batch)
+    w = Writer(dev, batch, 16, 1, 1, 64, seed=batch)
+    slots = np.concatenate([b * 16 + np.arange(n) for b, n in enumerate(lens)] + [np.zeros(0)]).astype(np.uint32)
+    slots = slots if len(slots) else np.array([0], np.uint32)
+    if len(slots) < 3000:
+        w.write(slots)
+    else:
+        k = w.rows(len(slots)).to(dev)
+        w.launch(torch.zeros(len(slots), 1, 64, dtype=torch.bfloat16, device=dev), k, k,
+                 ints(slots % 16, dev), ints(slots, dev),
+                 torch.empty(len(slots), 1, 64, dtype=torch.bfloat16, device=dev))
+        H.sync()
+        w.v.raw = w.v_d.cpu().numpy()
+    start = np.concatenate([[0], np.cumsum(lens)])
+    _, v = read_back(dev, w.k_d, w.v_d, ints(np.arange(batch)[:, None], dev), start, lens,
+                     int(start[-1]) + 1, 16, 1, 1, 64)
+    want = np.stack([w.v.row(b * 16 + i) for b, n in enumerate(lens) for i in range(n)] + [np.full((1, 64), 5.0)])
+    assert np.array_equal(v.double().numpy(), want)
+
+
+def test_read_arrays_of_any_content(dev):
+    """Lengths and pages that are none: no access outside the tensors."""
+    w = Writer(dev, 4, 16, 2, 2, 64)
+    w.write(np.arange(64))
+    for start, lens in (([0, 4000000000, 5, 33], [7, 8, 9]), ([9, 3, 30, 1], [4000000000] * 3),
+                        ([0, 36, 0, 36], [90, 90, 90]), ([50, 60, 70, 80], [1, 2, 3])):
+        read_back(dev, w.k_d, w.v_d, ints(np.full((3, 4), 0xFFFFFFFB), dev), start, lens, 36, 16, 4, 2, 64)
+
+
+# --------------------------------------------------------------- attention
+
+class In8Bits:
+    """A Step's requests in 8-bit caches whose unwritten rows, blocks and pages
+    are NaN; `kv` becomes what the codes stand for."""
+
+    apart = 0
+
+    def __init__(self, *args, interleaved=False, **kw):
+        super().__init__(*args, **kw)
+        hkv, d, ps = self.hkv, self.d, self.ps
+        n = F8.page_bytes(ps, hkv, d) + self.apart
+        both = torch.full((self.pages, 2, n), 255, dtype=torch.uint8)
+        codes = both[:, :, :hkv * ps * d].view(self.pages, 2, hkv, ps, d)
+        at = hkv * ps * d
+        scales = both[:, :, at:at + hkv * ps // 16 * 4].view(torch.float32).view(self.pages, 2, hkv, ps // 16)
+        table = self.table.cpu().numpy()
+        held = []
+        for b, kv in enumerate(self.kv):
+            new = []
+            for which, x in enumerate(kv):
+                rows = x.shape[0]
+                wide = torch.zeros(-(-rows // 16) * 16, hkv, d)
+                wide[:rows] = x.float() * torch.exp2(torch.arange(rows) % 5 - 2.0)[:, None, None]
+                blocks = wide.view(-1, 16, hkv, d)
+                most = blocks.abs().amax((1, 3))
+                m, e = torch.frexp(most)
+                s = torch.ldexp(torch.ones_like(most), e - 9 + (m > 0.875).int())
+                c = (blocks / s[:, None, :, None]).to(torch.float8_e4m3fn)
+                new.append((c.float() * s[:, None, :, None]).view(-1, hkv, d)[:rows].to(torch.bfloat16))
+                c = c.view(torch.uint8).view(-1, hkv, d)
+                for j in range(-(-rows // ps)):
+                    page, m = int(table[b, j]), min(ps, rows - j * ps)
+                    codes[page, which, :, :m] = c[j * ps:j * ps + m].transpose(0, 1)
+                    mb = -(-m // 16)
+                    scales[page, which, :, :mb] = s[j * ps // 16:j * ps // 16 + mb].t()
+            held.append(tuple(new))
+        self.kv = held
+        del self.k, self.v
+        if interleaved:
+            both = both.to(self.dev)
+            self.k, self.v = both[:, 0], both[:, 1]
+        else:
+            self.k, self.v = (both[:, i].contiguous().to(self.dev) for i in range(2))
+        self.stride = self.k.stride(0)
+
+    def attend(self, stream=None):
+        attn.paged_attention_fp8(self.q_d, self.k, self.v, self.o, self.table, self.plan,
+                                 self.batch, self.rows, self.pages, self.ps, self.stride,
+                                 self.blocks, self.window, self.sinks, self.hq, self.hkv, self.d,
+                                 self.ws, stream)
+
+    def put(self, which, b, j, dim, code):
+        """`code` at a key and dim of every head."""
+        cache = (self.k, self.v)[which]
+        at = torch.arange(self.hkv, device=self.dev) * self.ps * self.d + j % self.ps * self.d + dim
+        cache[int(self.table[b, j // self.ps]), at] = code
+
+
+class Step8(In8Bits, Step):
+    pass
+
+
+class Wide8(In8Bits, Wide):
+    pass
+
+
+class Early8(In8Bits, Early):
+    pass
+
+
+@pytest.mark.parametrize("hq,hkv,d", HEADS)
+@pytest.mark.parametrize("name", BATCHES)
+def test_attention(dev, name, hq, hkv, d):
+    print(f"[fp8] attention {name} {hq}/{hkv} D={d}", flush=True)
+    Step8(dev, BATCHES[name], hq, hkv, d, 16, seed=hq + d).run()
+
+
+@pytest.mark.parametrize("ps", [16, 32, 64, 128, 512])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_page_sizes(dev, ps, d):
+    Step8(dev, [(700, 1), (130, 130), (333, 40), (64, 2), (1, 1)], 8, 2, d, ps, seed=ps,
+          interleaved=True).run()
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (7, 4), (64, 0), (100, 70), (300, 4),
+                                          (5000, 3)])
+@pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (6, 2, 64)])
+def test_attention_window(dev, window, sinks, hq, hkv, d):
+    print(f"[fp8] window {window} sinks {sinks} {hq}/{hkv}", flush=True)
+    Step8(dev, [(900, 1), (150, 150), (500, 60), (64, 3), (1, 1)], hq, hkv, d, 32, window, sinks,
+          seed=window).run()
+
+
+@pytest.mark.parametrize("case", range(len(FORMS)))
+def test_each_form(dev, case):
+    """Units of every size, whole and in pieces (the plan and so the forms are
+    those of the bf16 cache)."""
+    hq, hkv, d, requests = FORMS[case]
+    st = Wide8(dev, requests, hq, hkv, d, 16, seed=case)
+    st.make_plan()
+    H.sync()
+    print(f"[fp8] {hq}/{hkv} D={d} {requests[:3]}: {shape_of(st)}", flush=True)
+    st.run()
+
+
+@pytest.mark.parametrize("hq,hkv,d,requests", [
+    (64, 1, 128, [(700, 3), (90, 90)]),
+    (71, 1, 64, [(500, 2), (40, 40)]),
+    (9, 3, 128, [(3000, 1), (260, 130)]),
+    (260, 260, 64, [(200, 1), (70, 20)]),
+    (25, 5, 128, [(2042, 373)]),
+    (8, 8, 128, [(6000, 200)]),
+])
+def test_head_layouts(dev, hq, hkv, d, requests):
+    print(f"[fp8] heads {hq}/{hkv} D={d}", flush=True)
+    Wide8(dev, requests, hq, hkv, d, 16, seed=hq).run()
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (9000, 100)])
+@pytest.mark.parametrize("ps", [16, 64, 256])
+def test_long_contexts(dev, ps, window, sinks):
+    print(f"[fp8] long, page size {ps} window {window}", flush=True)
+    Wide8(dev, [(40001, 1), (20000, 100), (33000, 9)], 8, 2, 128, ps, window, sinks, seed=ps).run()
+
+
+def test_many_requests(dev):
+    rng = np.random.default_rng(4)
+    Wide8(dev, [(int(x), 1) for x in rng.integers(1, 700, 1000)], 16, 4, 128, 16, seed=4).run()
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (37, 2), (1 << 31, 5)])
+@pytest.mark.parametrize("case", range(len(EARLY)))
+def test_rows_on_both_sides_of_position_0(dev, case, window, sinks):
+    hq, hkv, d, requests = EARLY[case]
+    print(f"[fp8] before 0: {hq}/{hkv} D={d} {requests[:4]} window {window}", flush=True)
+    Early8(dev, requests, hq, hkv, d, 16, window, sinks, seed=case).run()
+
+
+@pytest.mark.parametrize("case", range(len(SPOILT)))
+def test_codes_that_are_nan(dev, case):
+    """A NaN in V reaches the dims of the rows that see it, and no others; one in
+    K the rows that see it."""
+    hq, hkv, d, requests, window, sinks, at = SPOILT[case]
+    st = Wide8(dev, requests, hq, hkv, d, 16, window, sinks, seed=case)
+    st.make_plan()
+    H.sync()
+    print(f"[fp8] NaN: {hq}/{hkv} D={d} {requests[:3]}: {shape_of(st)}", flush=True)
+    st.run()
+    for i, (b, j, dim, _) in enumerate(at):
+        st.put(1, b, j, dim, 127 + 128 * (i % 2))
+    for _ in range(2):
+        st.o.fill_(3.0)
+        st.attend()
+        H.sync()
+        check_nan(st, at)
+    b, j, dim, _ = at[0]
+    st.put(0, b, j, dim, 255)
+    st.attend()
+    H.sync()
+    length, n = requests[b]
+    seen = torch.from_numpy(PO.visible(n, length, window, sinks))[:, j]
+    got = st.o[int(st.start[b]):int(st.start[b + 1])].cpu()
+    assert torch.isnan(got[seen]).all()
+    other = (dim + 1) % d  # (no NaN of V in it, or in rows that see it only)
+    if all(x[2] != other for x in at):
+        assert torch.isfinite(got[~seen][..., other]).all()
+
+
+@pytest.mark.parametrize("hq,d,requests", [(32, 64, [(5000, 5000), (900, 1)])])
+def test_more_spoilt_blocks_than_marks(dev, hq, d, requests):
+    st = Wide8(dev, requests, hq, hq, d, 16, seed=3)
+    at = [(0, j, 11, None) for j in range(3, requests[0][0], 7)]
+    for b, j, dim, _ in at:
+        st.put(1, b, j, dim, 127)
+    st.make_plan()
+    st.attend()
+    H.sync()
+    assert shape_of(st)[1]
+    check_nan(st, at)
+
+
+def test_hidden_scales_that_are_none(dev):
+    """Scales of blocks that no row sees, behind a window and past the last key,
+    may hold anything."""
+    for requests, window in (([(700, 1), (300, 40)], 100), ([(330, 330)], 64), ([(129, 1), (65, 3)], 0)):
+        for d in (64, 128):
+            st = Step8(dev, requests, 8, 2, d, 64, window, 0, seed=d)
+            at = 2 * 64 * d
+            scales = st.v[:, at:at + 32].view(torch.float32).view(-1, 2, 4)
+            for b, (length, n) in enumerate(requests):
+                low = max(0, length - n + 1 - window) if window else 0
+                for block in range(low // 16):
+                    scales[int(st.table[b, block // 4]), :, block % 4] = (float("inf"), float("nan"))[block % 2]
+            st.run()
+
+
+def test_attention_other_plan(dev):
+    st = Step8(dev, [(40, 1), (90, 3)], 8, 2, 128, 16)
+    attn.paged_attention_plan(st.query_start, st.seq_lens, st.batch, st.rows, st.ps, st.blocks, 5,
+                              0, st.hq, st.hkv, st.d, st.plan)
+    st.attend()
+    H.sync()
+    assert torch.isnan(st.o).all()
+
+
+def test_attention_arrays_of_any_content(dev):
+    st = Step8(dev, [(40, 1), (90, 30), (64, 2)], 8, 2, 128, 16)
+    good = st.query_start.clone(), st.seq_lens.clone(), st.table.clone()
+    for qs, lens in (([0, 4000000000, 5, 33], [7, 8, 9]), ([9, 3, 30, 1], [4000000000] * 3),
+                     ([0, 36, 0, 36], [90, 90, 90])):
+        st.query_start.copy_(ints(qs, dev))
+        st.seq_lens.copy_(ints(lens, dev))
+        st.table.fill_(-5)
+        st.make_plan()
+        st.attend()
+        H.sync()
+    for t, x in zip((st.query_start, st.seq_lens, st.table), good):
+        t.copy_(x)
+    st.o.fill_(3.0)
+    st.run()
+
+
+def test_attention_large_scores(dev):
+    for seed in range(3):
+        Step8(dev, [(300, 1), (200, 200), (1500, 20)], 8, 2, 128, 16, std=60.0, seed=seed).run()
+
+
+def test_no_new_tokens(dev):
+    st = Step8(dev, [(40, 0), (0, 0), (300, 0)], 8, 2, 128, 16)
+    st.run()
+    assert (st.o == 3.0).all() and not st.ws[:4 * (st.hkv + 2)].any()
+
+
+def test_attention_repeats_bit_for_bit(dev):
+    st = Step8(dev, [(3000, 1), (500, 200), (900, 30)], 16, 8, 128, 16)
+    st.run()
+    first = st.o.clone()
+    for _ in range(3):
+        st.o.fill_(3.0)
+        st.make_plan()
+        st.attend()
+        assert torch.equal(st.o, first)
+
+
+def test_long_contexts_miss_no_tile(dev):
+    """As over the bf16 cache: the RMS over a request's elements sees a tile that
+    the elements' bound cannot."""
+    rms = lambda x: x.square().mean().sqrt().item()
+    for d in (64, 128):
+        st = Wide8(dev, [(40001, 1), (20000, 33), (33000, 9)], 8, 2, d, 16, 0, 0, seed=d)
+        st.run()
+        for b, (length, n) in enumerate(st.requests):
+            rows = slice(int(st.start[b]), int(st.start[b + 1]))
+            k, v = (x.to(dev) for x in st.kv[b])
+            o, _ = wide_attention(st.q_d[rows], k, v, 0, 0)
+            error = rms(st.o[rows].double() - o) / rms(o)
+            print(f"[fp8] {length} keys, D={d}: RMS {error:.5f}", flush=True)
+            assert error < 2.0 ** -7, b
+
+
+def test_equals_the_bf16_cache(dev):
+    """Units of more than 32 rows run the same products over the same operands:
+    bit for bit what the bf16 cache of the values gives."""
+    for hq, hkv, d, requests, window in ((32, 8, 128, [(700, 300), (512, 512)], 0),
+                                         (8, 2, 64, [(900, 100), (64, 64), (1300, 777)], 200)):
+        st = Step8(dev, requests, hq, hkv, d, 64, window, 4 if window else 0, seed=7)
+        st.run()
+        pages = torch.zeros(2, st.pages, 64, hkv, d, dtype=torch.bfloat16)
+        table = st.table.cpu().numpy()
+        for b, kv in enumerate(st.kv):
+            for which, x in enumerate(kv):
+                for j in range(0, x.shape[0], 64):
+                    part = x[j:j + 64]
+                    pages[which, int(table[b, j // 64]), :part.shape[0]] = part
+        o = torch.full_like(st.o, 3.0)
+        k, v = (p.contiguous().to(dev) for p in pages)
+        attn.paged_attention_bf16(st.q_d, k, v, o, st.table, st.plan, st.batch, st.rows, st.pages, 64,
+                                  64 * hkv * d, st.blocks, st.window, st.sinks, hq, hkv, d, st.ws)
+        H.sync()
+        assert torch.equal(o, st.o)
+
+
+def test_pages_past_4_gib(dev):
+    """Byte offsets beyond 32 bits in the write's slots, the read's and the
+    attention's pages."""
+    hq, hkv, d, ps = 8, 4, 128, 64
+    page = attn.paged_fp8_page_bytes(ps, hkv, d)
+    pages = (2 ** 32 + 2 ** 28) // page
+    kc, vc = (torch.empty(pages, page, dtype=torch.uint8, device=dev) for _ in range(2))
+    length, new = 300, 40
+    table = [pages - 1, 3, pages - 7, pages // 2 + 1, pages - 3]
+    g = torch.Generator().manual_seed(1)
+    def bf(*shape):
+        return torch.randn(shape, generator=g).to(torch.bfloat16).to(dev)
+    q, k, v = bf(length, hq, d), bf(length, hkv, d), bf(length, hkv, d)
+    one = torch.ones(d, dtype=torch.bfloat16, device=dev)
+    rope = torch.zeros(length, d // 2, 2, device=dev)
+    rope[..., 0] = 1.0
+    slots = [table[j // ps] * ps + j % ps for j in range(length)]
+    q_out = torch.empty_like(q)
+    print("[fp8] write past 4 GiB", flush=True)
+    attn.paged_qkv_prologue_fp8(q, k, v, one, one, rope, length, ints(range(length), dev),
+                                ints(slots, dev), length, 1e-6, q_out, kc, vc, pages, ps, page, hq,
+                                hkv, d)
+    H.sync()
+    rows_k, rows_v = (x.to(dev) for x in read_back(dev, kc, vc, ints([table], dev), [0, length], [length],
+                                                   length, ps, 5, hkv, d))
+    small = F8.Cache(5, ps, hkv, d)
+    small.write(np.arange(length), v.cpu().double().numpy())
+    assert np.array_equal(rows_v.cpu().double().numpy(), np.stack([small.row(j) for j in range(length)]))
+    qn = q_out[length - new:].contiguous()
+    for n in (new, 1):
+        o = torch.empty_like(qn[:n])
+        plan = attn.paged_attention_plan_buffer(1, n, hq, hkv, d, dev)
+        ws = attn.paged_attention_workspace(hq, hkv, d, dev)
+        print("[fp8] attention past 4 GiB", flush=True)
+        attn.paged_attention_plan(ints([0, n], dev), ints([length], dev), 1, n, ps, 5, 0, 0, hq, hkv,
+                                  d, plan)
+        attn.paged_attention_fp8(qn[new - n:].contiguous(), kc, vc, o, ints(table, dev), plan, 1, n,
+                                 pages, ps, page, 5, 0, 0, hq, hkv, d, ws)
+        H.sync()
+        check_rows(o, qn[new - n:], rows_k, rows_v, 0, 0, "past 4 GiB")

@@ -89,6 +89,15 @@ SIGNATURES = {
     "toyinfer_paged_attention_bf16": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _u32, _u32, _u32,
                                              _u32, _u64, _u32, _u32, _u32, _u32, _u32, _u32, _vp,
                                              _sz, _vp]),
+    "toyinfer_paged_fp8_page_bytes": (_sz, [_u32, _u32, _u32]),
+    "toyinfer_paged_qkv_prologue_fp8": (
+        _i32, [_vp, _vp, _vp, _vp, _vp, _vp, _u32, _vp, _vp, _u32, _f32, _vp, _vp, _vp, _u32, _u32,
+               _u64, _u32, _u32, _u32, _vp]),
+    "toyinfer_paged_kv_read_fp8": (_i32, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _vp, _vp, _u32, _u32,
+                                          _u64, _u32, _u32, _u32, _vp]),
+    "toyinfer_paged_attention_fp8": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _u32, _u32, _u32,
+                                            _u32, _u64, _u32, _u32, _u32, _u32, _u32, _u32, _vp,
+                                            _sz, _vp]),
     "toyinfer_decode_qkv_prologue_bf16": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _f32,
                                                  _vp, _vp, _vp, _u32, _u32, _u32, _vp]),
 }
@@ -668,6 +677,102 @@ def paged_attention_bf16(q, k_cache, v_cache, o, block_tables, plan, batch: int,
     _need_cache(fn, device, num_pages, page_size, page_stride, num_kv_heads, heads_dim, k_cache,
                 v_cache)
     _check(fn, LIB.toyinfer_paged_attention_bf16(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), block_tables.data_ptr(), plan.data_ptr(),
+        plan.numel() * plan.element_size(), batch, num_tokens, num_pages, page_size, page_stride,
+        max_blocks, window, sinks, num_q_heads, num_kv_heads, heads_dim, workspace.data_ptr(),
+        workspace.numel() * workspace.element_size(), _stream(stream)))
+
+
+def paged_fp8_page_bytes(page_size: int, num_kv_heads: int, head_dim: int) -> int:
+    """Bytes of a page of an 8-bit cache: codes [heads][rows][dims], then scales
+    [heads][rows / 16] in fp32."""
+    return int(LIB.toyinfer_paged_fp8_page_bytes(page_size, num_kv_heads, head_dim))
+
+
+def paged_fp8_cache(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, device):
+    """An uninitialised 8-bit cache, uint8 [num_pages][bytes of a page]."""
+    import torch
+
+    page = paged_fp8_page_bytes(page_size, num_kv_heads, head_dim)
+    if page == 0:
+        raise ToyInferError("paged_fp8_cache", ERR_INVALID_ARGUMENT)
+    return torch.empty(num_pages, page, dtype=torch.uint8, device=device)
+
+
+def _need_cache_fp8(fn: str, device: int, num_pages: int, page_size: int, page_stride: int,
+                    num_kv_heads: int, head_dim: int, *caches) -> None:
+    """uint8 [pages][bytes], a page in one piece and page_stride bytes from the next."""
+    import torch
+
+    page = paged_fp8_page_bytes(page_size, num_kv_heads, head_dim)
+    for t in caches:
+        if (t.get_device() != device or t.dtype != torch.uint8 or t.dim() != 2
+                or t.shape[0] < num_pages or t.shape[1] < page or t.stride(1) != 1
+                or t.stride(0) != page_stride and num_pages > 1):
+            raise ToyInferError(fn, ERR_INVALID_ARGUMENT)
+
+
+def paged_qkv_prologue_fp8(q, k, v, q_norm_weight, k_norm_weight, rope_cos_sin,
+                           num_positions: int, positions, slot_mapping, num_tokens: int,
+                           rms_norm_eps: float, q_out, k_cache, v_cache, num_pages: int,
+                           page_size: int, page_stride: int, num_q_heads: int, num_kv_heads: int,
+                           head_dim: int, stream=None) -> None:
+    """paged_qkv_prologue_bf16 into 8-bit caches, with a scale for each block of 16
+    rows and head; page_stride in bytes."""
+    fn = "paged_qkv_prologue_fp8"
+    row = num_tokens * head_dim
+    bf16, u32, f32 = _types()
+    device = _on_device(fn, q)
+    _need(fn, device, bf16, (q, row * num_q_heads), (k, row * num_kv_heads), (v, row * num_kv_heads),
+          (q_norm_weight, head_dim), (k_norm_weight, head_dim), (q_out, row * num_q_heads))
+    _need(fn, device, f32, (rope_cos_sin, num_positions * head_dim))
+    _need(fn, device, u32, (positions, num_tokens), (slot_mapping, num_tokens))
+    _need_cache_fp8(fn, device, num_pages, page_size, page_stride, num_kv_heads, head_dim, k_cache,
+                    v_cache)
+    _check(fn, LIB.toyinfer_paged_qkv_prologue_fp8(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), rope_cos_sin.data_ptr(),
+        num_positions, positions.data_ptr(), slot_mapping.data_ptr(), num_tokens, rms_norm_eps, q_out.data_ptr(),
+        k_cache.data_ptr(), v_cache.data_ptr(), num_pages, page_size, page_stride, num_q_heads, num_kv_heads,
+        head_dim, _stream(stream)))
+
+
+def paged_kv_read_fp8(k_cache, v_cache, block_tables, query_start, seq_lens, batch: int,
+                      num_tokens: int, k_out, v_out, num_pages: int, page_size: int,
+                      page_stride: int, max_blocks: int, num_kv_heads: int, head_dim: int,
+                      stream=None) -> None:
+    """The last query_start[b+1] - query_start[b] tokens of each request's
+    seq_lens[b] out of 8-bit caches, as bf16 [num_tokens][heads][dims], exactly."""
+    fn = "paged_kv_read_fp8"
+    rows = num_tokens * num_kv_heads * head_dim
+    bf16, u32, _ = _types()
+    device = _on_device(fn, k_cache)
+    _need(fn, device, bf16, (k_out, rows), (v_out, rows))
+    _need(fn, device, u32, (block_tables, batch * max_blocks), (query_start, batch + 1), (seq_lens, batch))
+    _need_cache_fp8(fn, device, num_pages, page_size, page_stride, num_kv_heads, head_dim, k_cache,
+                    v_cache)
+    _check(fn, LIB.toyinfer_paged_kv_read_fp8(
+        k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), query_start.data_ptr(), seq_lens.data_ptr(),
+        batch, num_tokens, k_out.data_ptr(), v_out.data_ptr(), num_pages, page_size, page_stride, max_blocks,
+        num_kv_heads, head_dim, _stream(stream)))
+
+
+def paged_attention_fp8(q, k_cache, v_cache, o, block_tables, plan, batch: int, num_tokens: int,
+                        num_pages: int, page_size: int, page_stride: int, max_blocks: int,
+                        window: int, sinks: int, num_q_heads: int, num_kv_heads: int,
+                        heads_dim: int, workspace, stream=None) -> None:
+    """paged_attention_bf16 over 8-bit caches (q and o bf16, page_stride in bytes);
+    the plan and the workspace are the same."""
+    fn = "paged_attention_fp8"
+    rows = num_tokens * num_q_heads * heads_dim
+    bf16, u32, _ = _types()
+    device = _on_device(fn, q)
+    _need(fn, device, bf16, (q, rows), (o, rows))
+    _need(fn, device, u32, (block_tables, batch * max_blocks))
+    _need(fn, device, (plan.dtype,), (plan, 1))
+    _need(fn, device, (workspace.dtype,), (workspace, 1))
+    _need_cache_fp8(fn, device, num_pages, page_size, page_stride, num_kv_heads, heads_dim, k_cache,
+                    v_cache)
+    _check(fn, LIB.toyinfer_paged_attention_fp8(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), block_tables.data_ptr(), plan.data_ptr(),
         plan.numel() * plan.element_size(), batch, num_tokens, num_pages, page_size, page_stride,
         max_blocks, window, sinks, num_q_heads, num_kv_heads, heads_dim, workspace.data_ptr(),

@@ -781,7 +781,19 @@ static int check_paging(uint32_t page_size, uint32_t max_blocks) {
     return (uint64_t)max_blocks * page_size < (1ull << 31) ? TOYINFER_OK : TOYINFER_ERR_UNSUPPORTED;
 }
 
-// The caches' arguments; *bytes receives what each spans.
+// Pages of one cache may lie between pages of the other, not on them; *bytes
+// receives what each spans.  (All in bytes.)
+static int check_pages_apart(const void* k_cache, const void* v_cache, uint32_t num_pages, uint64_t stride,
+                             uint64_t page, uint64_t* bytes) {
+    *bytes = (num_pages - 1) * stride + page;
+    const uintptr_t a = (uintptr_t)k_cache, b = (uintptr_t)v_cache;
+    const uint64_t apart = (a < b ? b - a : a - b) % stride;
+    if (overlap(k_cache, *bytes, v_cache, *bytes) && (apart < page || stride - apart < page))
+        return TOYINFER_ERR_INVALID_ARGUMENT;
+    return TOYINFER_OK;
+}
+
+// The caches' arguments.
 static int check_caches(const void* k_cache, const void* v_cache, uint32_t num_pages, uint32_t page_size,
                         uint64_t page_stride, uint32_t hkv, uint32_t d, uint64_t* bytes) {
     if (int st = check_paging(page_size, 1)) return st;
@@ -792,13 +804,21 @@ static int check_caches(const void* k_cache, const void* v_cache, uint32_t num_p
     if ((uint64_t)num_pages * page_size >= (1ull << 32) || page_stride >= (1ull << 40) ||
         num_pages - 1 > (1ull << 46) / page_stride)  // more than 2^47 bytes: no memory holds it
         return TOYINFER_ERR_UNSUPPORTED;
-    *bytes = 2 * ((num_pages - 1) * page_stride + page);
-    // Pages of one cache may lie between pages of the other, not on them.
-    const uintptr_t a = (uintptr_t)k_cache, b = (uintptr_t)v_cache;
-    const uint64_t apart = (a < b ? b - a : a - b) % (2 * page_stride);
-    if (overlap(k_cache, *bytes, v_cache, *bytes) && (apart < 2 * page || 2 * page_stride - apart < 2 * page))
-        return TOYINFER_ERR_INVALID_ARGUMENT;
-    return TOYINFER_OK;
+    return check_pages_apart(k_cache, v_cache, num_pages, 2 * page_stride, 2 * page, bytes);
+}
+
+// The same of 8-bit caches; page_stride in bytes.
+static int check_caches_fp8(const void* k_cache, const void* v_cache, uint32_t num_pages, uint32_t page_size,
+                            uint64_t page_stride, uint32_t hkv, uint32_t d, uint64_t* bytes) {
+    if (int st = check_paging(page_size, 1)) return st;
+    if (!k_cache || !v_cache || num_pages == 0 || page_size < kFp8Block) return TOYINFER_ERR_INVALID_ARGUMENT;
+    if (!aligned(k_cache, 16) || !aligned(v_cache, 16)) return TOYINFER_ERR_INVALID_ARGUMENT;
+    const uint64_t page = fp8_page_bytes(page_size, hkv, d);
+    if (page_stride < page || page_stride % 16 != 0) return TOYINFER_ERR_INVALID_ARGUMENT;
+    if ((uint64_t)num_pages * page_size >= (1ull << 32) || page_stride >= (1ull << 41) ||
+        num_pages - 1 > (1ull << 47) / page_stride)
+        return TOYINFER_ERR_UNSUPPORTED;
+    return check_pages_apart(k_cache, v_cache, num_pages, page_stride, page, bytes);
 }
 
 int toyinfer_paged_tables_u32(const uint32_t* context_lens, const uint32_t* new_lens,
@@ -836,6 +856,28 @@ int toyinfer_paged_tables_u32(const uint32_t* context_lens, const uint32_t* new_
     return from_hip(launch_paged_tables(a, as_stream(stream)));
 }
 
+// The prologues' rows and what they may overlap; `cache`: the bytes that each cache spans.
+static int check_prologue(const void* q, const void* k, const void* v, const void* q_norm_weight,
+                          const void* k_norm_weight, const float* rope_cos_sin, uint32_t num_positions,
+                          const uint32_t* positions, const uint32_t* slot_mapping, uint32_t num_tokens, void* q_out,
+                          void* k_cache, void* v_cache, uint64_t cache, uint32_t num_q_heads, uint32_t num_kv_heads,
+                          uint32_t head_dim) {
+    const uint64_t row = 2ull * num_tokens * head_dim;
+    const void* const p[] = {q, k, v, q_norm_weight, k_norm_weight, rope_cos_sin, positions, slot_mapping, q_out,
+                             k_cache, v_cache};
+    const uint64_t bytes[] = {row * num_q_heads, row * num_kv_heads, row * num_kv_heads, 2ull * head_dim,
+                              2ull * head_dim, 4ull * num_positions * head_dim, 4ull * num_tokens,
+                              4ull * num_tokens, row * num_q_heads, cache, cache};
+    for (int i = 0; i < 9; ++i)
+        if (!p[i] || !aligned(p[i], i == 6 || i == 7 ? 4 : 16)) return TOYINFER_ERR_INVALID_ARGUMENT;
+    for (int i = 8; i < 11; ++i)
+        for (int j = 0; j < (i == 8 ? 8 : 9); ++j)  // (the caches against each other: check_caches)
+            if (!(i == 8 && j == 0 && q_out == q) && overlap(p[i], bytes[i], p[j], bytes[j]))
+                return TOYINFER_ERR_INVALID_ARGUMENT;
+    if ((uint64_t)num_tokens * (num_q_heads + 2ull * num_kv_heads) >= (1ull << 31)) return TOYINFER_ERR_UNSUPPORTED;
+    return TOYINFER_OK;
+}
+
 int toyinfer_paged_qkv_prologue_bf16(const void* q, const void* k, const void* v,
                                      const void* q_norm_weight, const void* k_norm_weight,
                                      const float* rope_cos_sin, uint32_t num_positions,
@@ -850,19 +892,10 @@ int toyinfer_paged_qkv_prologue_bf16(const void* q, const void* k, const void* v
     uint64_t cache = 0;
     if (int st = check_caches(k_cache, v_cache, num_pages, page_size, page_stride, num_kv_heads, head_dim, &cache))
         return st;
-    const uint64_t row = 2ull * num_tokens * head_dim;
-    const void* const p[] = {q, k, v, q_norm_weight, k_norm_weight, rope_cos_sin, positions, slot_mapping, q_out,
-                             k_cache, v_cache};
-    const uint64_t bytes[] = {row * num_q_heads, row * num_kv_heads, row * num_kv_heads, 2ull * head_dim,
-                              2ull * head_dim, 4ull * num_positions * head_dim, 4ull * num_tokens,
-                              4ull * num_tokens, row * num_q_heads, cache, cache};
-    for (int i = 0; i < 9; ++i)
-        if (!p[i] || !aligned(p[i], i == 6 || i == 7 ? 4 : 16)) return TOYINFER_ERR_INVALID_ARGUMENT;
-    for (int i = 8; i < 11; ++i)
-        for (int j = 0; j < (i == 8 ? 8 : 9); ++j)  // (the caches against each other: check_caches)
-            if (!(i == 8 && j == 0 && q_out == q) && overlap(p[i], bytes[i], p[j], bytes[j]))
-                return TOYINFER_ERR_INVALID_ARGUMENT;
-    if ((uint64_t)num_tokens * (num_q_heads + 2ull * num_kv_heads) >= (1ull << 31)) return TOYINFER_ERR_UNSUPPORTED;
+    if (int st = check_prologue(q, k, v, q_norm_weight, k_norm_weight, rope_cos_sin, num_positions, positions,
+                                slot_mapping, num_tokens, q_out, k_cache, v_cache, cache, num_q_heads, num_kv_heads,
+                                head_dim))
+        return st;
     PagedPrologueArgs a;
     a.q = static_cast<const uint16_t*>(q);
     a.k = static_cast<const uint16_t*>(k);
@@ -952,6 +985,42 @@ int toyinfer_paged_attention_plan(const uint32_t* query_start, const uint32_t* s
     return from_hip(launch_paged_plan(a, as_stream(stream)));
 }
 
+// The attentions' arguments beside the caches, of which each spans `cache` bytes.
+static int attention_args(const void* q, const void* k_cache, const void* v_cache, uint64_t cache, void* o,
+                          const uint32_t* block_tables, const void* plan, size_t plan_bytes, uint32_t batch,
+                          uint32_t num_tokens, uint32_t num_pages, uint32_t page_size, uint64_t page_bytes,
+                          uint32_t max_blocks, uint32_t window, uint32_t sinks, uint32_t num_q_heads,
+                          uint32_t num_kv_heads, uint32_t heads_dim, void* workspace, size_t workspace_bytes,
+                          PagedAttnArgs* a) {
+    if (!q || !o || !block_tables || !plan || !workspace) return TOYINFER_ERR_INVALID_ARGUMENT;
+    if (!aligned(q, 16) || !aligned(o, 16) || !aligned(block_tables, 4) || !aligned(plan, 256) ||
+        !aligned(workspace, 256))
+        return TOYINFER_ERR_INVALID_ARGUMENT;
+    const size_t plan_need = paged_plan_layout(batch, num_tokens, num_q_heads, num_kv_heads).bytes;
+    const size_t ws_need = toyinfer_paged_attention_workspace_bytes(num_q_heads, num_kv_heads, heads_dim);
+    if (plan_bytes < plan_need || workspace_bytes < ws_need) return TOYINFER_ERR_WORKSPACE;
+    const uint64_t rows = 2ull * num_tokens * num_q_heads * heads_dim;
+    const void* const p[] = {q, k_cache, v_cache, block_tables, plan, o, workspace};
+    const uint64_t bytes[] = {rows, cache, cache, 4ull * batch * max_blocks, plan_need, rows, ws_need};
+    if (!distinct(p, bytes, 5, 7)) return TOYINFER_ERR_INVALID_ARGUMENT;
+    a->q = static_cast<const uint16_t*>(q);
+    a->k_cache = k_cache;
+    a->v_cache = v_cache;
+    a->o = static_cast<uint16_t*>(o);
+    a->block_tables = block_tables;
+    a->plan = plan;
+    a->head = plan_header(batch, num_tokens, page_size, max_blocks, window, sinks, num_q_heads, num_kv_heads, heads_dim);
+    a->num_pages = num_pages;
+    a->page_bytes = page_bytes;
+    a->tickets = static_cast<uint32_t*>(workspace);
+    a->flags = a->tickets + num_kv_heads;
+    a->marks = reinterpret_cast<PagedMark*>(static_cast<char*>(workspace) + kPagedCounterBytes);
+    char* const part = static_cast<char*>(workspace) + kPagedPartials;
+    a->part_o = reinterpret_cast<float*>(part);
+    a->part_ml = reinterpret_cast<float2*>(part + paged_part_o_bytes(num_kv_heads, heads_dim));
+    return TOYINFER_OK;
+}
+
 int toyinfer_paged_attention_bf16(const void* q, const void* k_cache, const void* v_cache, void* o,
                                   const uint32_t* block_tables, const void* plan,
                                   size_t plan_bytes, uint32_t batch, uint32_t num_tokens,
@@ -965,34 +1034,114 @@ int toyinfer_paged_attention_bf16(const void* q, const void* k_cache, const void
     uint64_t cache = 0;
     if (int st = check_caches(k_cache, v_cache, num_pages, page_size, page_stride, num_kv_heads, heads_dim, &cache))
         return st;
-    if (!q || !o || !block_tables || !plan || !workspace) return TOYINFER_ERR_INVALID_ARGUMENT;
-    if (!aligned(q, 16) || !aligned(o, 16) || !aligned(block_tables, 4) || !aligned(plan, 256) ||
-        !aligned(workspace, 256))
-        return TOYINFER_ERR_INVALID_ARGUMENT;
-    const size_t plan_need = paged_plan_layout(batch, num_tokens, num_q_heads, num_kv_heads).bytes;
-    const size_t ws_need = toyinfer_paged_attention_workspace_bytes(num_q_heads, num_kv_heads, heads_dim);
-    if (plan_bytes < plan_need || workspace_bytes < ws_need) return TOYINFER_ERR_WORKSPACE;
-    const uint64_t rows = 2ull * num_tokens * num_q_heads * heads_dim;
-    const void* const p[] = {q, k_cache, v_cache, block_tables, plan, o, workspace};
-    const uint64_t bytes[] = {rows, cache, cache, 4ull * batch * max_blocks, plan_need, rows, ws_need};
-    if (!distinct(p, bytes, 5, 7)) return TOYINFER_ERR_INVALID_ARGUMENT;
     PagedAttnArgs a;
-    a.q = static_cast<const uint16_t*>(q);
-    a.k_cache = static_cast<const uint16_t*>(k_cache);
-    a.v_cache = static_cast<const uint16_t*>(v_cache);
-    a.o = static_cast<uint16_t*>(o);
-    a.block_tables = block_tables;
-    a.plan = plan;
-    a.head = plan_header(batch, num_tokens, page_size, max_blocks, window, sinks, num_q_heads, num_kv_heads, heads_dim);
-    a.num_pages = num_pages;
-    a.page_stride = page_stride;
-    a.tickets = static_cast<uint32_t*>(workspace);
-    a.flags = a.tickets + num_kv_heads;
-    a.marks = reinterpret_cast<PagedMark*>(static_cast<char*>(workspace) + kPagedCounterBytes);
-    char* const part = static_cast<char*>(workspace) + kPagedPartials;
-    a.part_o = reinterpret_cast<float*>(part);
-    a.part_ml = reinterpret_cast<float2*>(part + paged_part_o_bytes(num_kv_heads, heads_dim));
+    if (int st = attention_args(q, k_cache, v_cache, cache, o, block_tables, plan, plan_bytes, batch, num_tokens,
+                                num_pages, page_size, 2 * page_stride, max_blocks, window, sinks, num_q_heads,
+                                num_kv_heads, heads_dim, workspace, workspace_bytes, &a))
+        return st;
     return from_hip(launch_paged_attention(a, as_stream(stream)));
+}
+
+// -------------------------------------------------------- paged cache, 8 bits
+
+size_t toyinfer_paged_fp8_page_bytes(uint32_t page_size, uint32_t num_kv_heads, uint32_t head_dim) {
+    if (check_paging(page_size, 1) || page_size < kFp8Block || check_heads(num_kv_heads, num_kv_heads, head_dim)) return 0;
+    return fp8_page_bytes(page_size, num_kv_heads, head_dim);
+}
+
+int toyinfer_paged_qkv_prologue_fp8(const void* q, const void* k, const void* v,
+                                    const void* q_norm_weight, const void* k_norm_weight,
+                                    const float* rope_cos_sin, uint32_t num_positions,
+                                    const uint32_t* positions, const uint32_t* slot_mapping,
+                                    uint32_t num_tokens, float rms_norm_eps, void* q_out,
+                                    void* k_cache, void* v_cache, uint32_t num_pages,
+                                    uint32_t page_size, uint64_t page_stride,
+                                    uint32_t num_q_heads, uint32_t num_kv_heads,
+                                    uint32_t head_dim, void* stream) {
+    if (int st = check_heads(num_q_heads, num_kv_heads, head_dim)) return st;
+    if (num_tokens == 0 || num_positions == 0) return TOYINFER_ERR_INVALID_ARGUMENT;
+    uint64_t cache = 0;
+    if (int st = check_caches_fp8(k_cache, v_cache, num_pages, page_size, page_stride, num_kv_heads, head_dim, &cache))
+        return st;
+    if (int st = check_prologue(q, k, v, q_norm_weight, k_norm_weight, rope_cos_sin, num_positions, positions,
+                                slot_mapping, num_tokens, q_out, k_cache, v_cache, cache, num_q_heads, num_kv_heads,
+                                head_dim))
+        return st;
+    PagedPrologueFp8Args a;
+    a.q = static_cast<const uint16_t*>(q);
+    a.k = static_cast<const uint16_t*>(k);
+    a.v = static_cast<const uint16_t*>(v);
+    a.q_weight = static_cast<const uint16_t*>(q_norm_weight);
+    a.k_weight = static_cast<const uint16_t*>(k_norm_weight);
+    a.rope = rope_cos_sin;
+    a.num_positions = num_positions;
+    a.positions = positions;
+    a.slots = slot_mapping;
+    a.num_tokens = num_tokens;
+    a.eps = rms_norm_eps;
+    a.q_out = static_cast<uint16_t*>(q_out);
+    a.k_cache = static_cast<uint8_t*>(k_cache);
+    a.v_cache = static_cast<uint8_t*>(v_cache);
+    a.num_slots = num_pages * page_size;
+    a.page_shift = 31 - __builtin_clz(page_size);
+    a.page_bytes = page_stride;
+    a.hq = num_q_heads;
+    a.hkv = num_kv_heads;
+    return from_hip(launch_paged_prologue_fp8(a, head_dim, as_stream(stream)));
+}
+
+int toyinfer_paged_kv_read_fp8(const void* k_cache, const void* v_cache, const uint32_t* block_tables,
+                               const uint32_t* query_start, const uint32_t* seq_lens, uint32_t batch,
+                               uint32_t num_tokens, void* k_out, void* v_out, uint32_t num_pages,
+                               uint32_t page_size, uint64_t page_stride, uint32_t max_blocks,
+                               uint32_t num_kv_heads, uint32_t head_dim, void* stream) {
+    if (int st = check_paged_step(batch, num_tokens, num_kv_heads, num_kv_heads, head_dim)) return st;
+    if (int st = check_paging(page_size, max_blocks)) return st;
+    uint64_t cache = 0;
+    if (int st = check_caches_fp8(k_cache, v_cache, num_pages, page_size, page_stride, num_kv_heads, head_dim, &cache))
+        return st;
+    const uint64_t rows = 2ull * num_tokens * num_kv_heads * head_dim;
+    const void* const p[] = {block_tables, query_start, seq_lens, k_cache, v_cache, k_out, v_out};
+    const uint64_t bytes[] = {4ull * batch * max_blocks, 4 * (batch + 1ull), 4ull * batch, cache, cache, rows, rows};
+    for (int i = 0; i < 7; ++i)
+        if (!p[i] || !aligned(p[i], i < 3 ? 4 : 16)) return TOYINFER_ERR_INVALID_ARGUMENT;
+    if (!distinct(p, bytes, 5, 7)) return TOYINFER_ERR_INVALID_ARGUMENT;
+    PagedReadFp8Args a;
+    a.k_cache = static_cast<const uint8_t*>(k_cache);
+    a.v_cache = static_cast<const uint8_t*>(v_cache);
+    a.block_tables = block_tables;
+    a.query_start = query_start;
+    a.seq_lens = seq_lens;
+    a.batch = batch;
+    a.num_tokens = num_tokens;
+    a.k_out = static_cast<uint16_t*>(k_out);
+    a.v_out = static_cast<uint16_t*>(v_out);
+    a.num_pages = num_pages;
+    a.page_shift = 31 - __builtin_clz(page_size);
+    a.page_bytes = page_stride;
+    a.max_blocks = max_blocks;
+    a.hkv = num_kv_heads;
+    return from_hip(launch_paged_read_fp8(a, head_dim, as_stream(stream)));
+}
+
+int toyinfer_paged_attention_fp8(const void* q, const void* k_cache, const void* v_cache, void* o,
+                                 const uint32_t* block_tables, const void* plan, size_t plan_bytes,
+                                 uint32_t batch, uint32_t num_tokens, uint32_t num_pages,
+                                 uint32_t page_size, uint64_t page_stride, uint32_t max_blocks,
+                                 uint32_t window, uint32_t sinks, uint32_t num_q_heads,
+                                 uint32_t num_kv_heads, uint32_t heads_dim, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+    if (int st = check_paged_step(batch, num_tokens, num_q_heads, num_kv_heads, heads_dim)) return st;
+    if (int st = check_paging(page_size, max_blocks)) return st;
+    uint64_t cache = 0;
+    if (int st = check_caches_fp8(k_cache, v_cache, num_pages, page_size, page_stride, num_kv_heads, heads_dim, &cache))
+        return st;
+    PagedAttnArgs a;
+    if (int st = attention_args(q, k_cache, v_cache, cache, o, block_tables, plan, plan_bytes, batch, num_tokens,
+                                num_pages, page_size, page_stride, max_blocks, window, sinks, num_q_heads,
+                                num_kv_heads, heads_dim, workspace, workspace_bytes, &a))
+        return st;
+    return from_hip(launch_paged_attention_fp8(a, as_stream(stream)));
 }
 
 }  // extern "C"

@@ -11,6 +11,17 @@ namespace tiattn {
 constexpr uint32_t kPagedMaxBatch = 4096;
 constexpr uint32_t kNoSlot = 0xffffffffu;
 
+// The 8-bit cache: a page is its codes [Hkv][page_size][D], one byte each, then
+// the scales [Hkv][page_size / kFp8Block] in fp32.  (By head, so that a head's
+// rows of a page lie in one piece and a row of 64 dims shares its line with its
+// neighbours, not with other heads.)
+constexpr uint32_t kFp8Block = 16;
+constexpr int kFp8Low = -100, kFp8High = 119;  // exponents of the scales
+inline __host__ __device__ uint64_t fp8_page_bytes(uint32_t page_size, uint32_t hkv, uint32_t d) {
+    const uint64_t blocks = (uint64_t)hkv * (page_size / kFp8Block);
+    return (blocks * (kFp8Block * d + sizeof(float)) + 15) / 16 * 16;
+}
+
 // ------------------------------------------------------------------ tables
 struct PagedTablesArgs {
     const uint32_t* context_lens;
@@ -53,6 +64,45 @@ struct PagedPrologueArgs {
     uint32_t hq, hkv;
 };
 hipError_t launch_paged_prologue(const PagedPrologueArgs& a, uint32_t d, hipStream_t stream);
+
+struct PagedPrologueFp8Args {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    const uint16_t* q_weight;
+    const uint16_t* k_weight;
+    const float* rope;
+    uint32_t num_positions;
+    const uint32_t* positions;
+    const uint32_t* slots;
+    uint32_t num_tokens;
+    float eps;
+    uint16_t* q_out;
+    uint8_t* k_cache;
+    uint8_t* v_cache;
+    uint32_t num_slots;
+    uint32_t page_shift;
+    uint64_t page_bytes;  // from one page to the next
+    uint32_t hq, hkv;
+};
+hipError_t launch_paged_prologue_fp8(const PagedPrologueFp8Args& a, uint32_t d, hipStream_t stream);
+
+// -------------------------------------------------------------------- read
+struct PagedReadFp8Args {
+    const uint8_t* k_cache;
+    const uint8_t* v_cache;
+    const uint32_t* block_tables;
+    const uint32_t* query_start;
+    const uint32_t* seq_lens;
+    uint32_t batch, num_tokens;
+    uint16_t* k_out;
+    uint16_t* v_out;
+    uint32_t num_pages;
+    uint32_t page_shift;
+    uint64_t page_bytes;
+    uint32_t max_blocks, hkv;
+};
+hipError_t launch_paged_read_fp8(const PagedReadFp8Args& a, uint32_t d, hipStream_t stream);
 
 // --------------------------------------------------------------- attention
 //
@@ -161,14 +211,14 @@ hipError_t launch_paged_plan(const PagedPlanArgs& a, hipStream_t stream);
 
 struct PagedAttnArgs {
     const uint16_t* q;
-    const uint16_t* k_cache;
-    const uint16_t* v_cache;
+    const void* k_cache;
+    const void* v_cache;
     uint16_t* o;
     const uint32_t* block_tables;
     const void* plan;
     PagedPlanHeader head;  // what the plan has to have been made for
     uint32_t num_pages;
-    uint64_t page_stride;  // elements
+    uint64_t page_bytes;   // from one page to the next
     uint32_t* tickets;     // [KV head], zero between calls
     uint32_t* flags;       // [2], zero between calls: marks; workgroups of the merge that are done
     PagedMark* marks;      // [kPagedMarks]
@@ -176,5 +226,6 @@ struct PagedAttnArgs {
     float2* part_ml;       // [KV head][block][32 rows]: reference (log2), sum
 };
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream);
+hipError_t launch_paged_attention_fp8(const PagedAttnArgs& a, hipStream_t stream);
 
 }  // namespace tiattn

@@ -19,6 +19,7 @@
 
 #include "common.hpp"
 #include "paged.hpp"
+#include "paged_rows.hpp"
 
 namespace tiattn {
 namespace {
@@ -183,35 +184,10 @@ __global__ __launch_bounds__(256) void paged_prologue_kernel(PagedPrologueArgs a
     const uint64_t cache_row = (uint64_t)(slot >> a.page_shift) * a.page_stride +
                                (uint64_t)(slot & ((1u << a.page_shift) - 1)) * a.hkv * D;
     if (is_q || is_k) {
-        float re[8], im[8], ss = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            re[2 * k] = bf16_lo(word_of(xr, k));
-            re[2 * k + 1] = bf16_hi(word_of(xr, k));
-            im[2 * k] = bf16_lo(word_of(xi, k));
-            im[2 * k + 1] = bf16_hi(word_of(xi, k));
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) ss = fmaf(re[k], re[k], fmaf(im[k], im[k], ss));
-        // The LPR lanes of a row share a row and so take this branch together.
-        ss += dpp_f32<kDppXor1>(ss);
-        ss += dpp_f32<kDppXor2>(ss);
-        if constexpr (LPR == 8) ss += dpp_f32<kDppRowHalfMirror>(ss);
-        const float inv = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
-        uint32_t wr[4], wi[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint32_t gr = is_q ? word_of(qwr, k) : word_of(kwr, k);
-            const uint32_t gi = is_q ? word_of(qwi, k) : word_of(kwi, k);
-            const float r0 = re[2 * k] * inv * bf16_lo(gr), r1 = re[2 * k + 1] * inv * bf16_hi(gr);
-            const float i0 = im[2 * k] * inv * bf16_lo(gi), i1 = im[2 * k + 1] * inv * bf16_hi(gi);
-            // Rounded here only: the unfused sequence rounds the norm's
-            // result as well.
-            wr[k] = pack_bf16x2(cs[k].x * r0 - cs[k].y * i0, cs[k].z * r1 - cs[k].w * i1);
-            wi[k] = pack_bf16x2(cs[k].x * i0 + cs[k].y * r0, cs[k].z * i1 + cs[k].w * r1);
-        }
-        xr = make_uint4(wr[0], wr[1], wr[2], wr[3]);
-        xi = make_uint4(wi[0], wi[1], wi[2], wi[3]);
+        float re[8], im[8];
+        norm_rope_f32<D>(xr, xi, is_q ? qwr : kwr, is_q ? qwi : kwi, cs, a.eps, re, im);
+        xr = pack_bf16x8(re);
+        xi = pack_bf16x8(im);
     }
     if (row < rows && (is_q || slot < a.num_slots)) {
         uint16_t* dst = (is_q ? a.q_out : is_k ? a.k_cache : a.v_cache) + (is_q ? at : cache_row + (uint64_t)head * D);
