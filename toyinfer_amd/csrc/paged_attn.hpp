@@ -73,6 +73,14 @@ __device__ __forceinline__ int pk_swz(int row) { return row & (D / 8 - 1); }
 template <int D>
 __device__ __forceinline__ int pv_swz(int row) { return D == 128 ? 4 * (row & 3) : 2 * (row & 3); }
 
+// Of 8-bit rows: 16-byte chunks, for K's 16-byte operand reads and V's transposing
+// ones, which take eight rows {0-3, 8-11} or {4-7, 12-15} at a chunk and its
+// neighbour.  Four (two) rows fill the banks once (64 dims: 64 bytes).
+template <int D>
+__device__ __forceinline__ int p8_swz(int row) {
+    return D == 128 ? (row & 2) | (row >> 1 & 4) | (row >> 2 & 1) : (row >> 2 & 2) | (row >> 2 & 1);
+}
+
 template <int D>
 struct PaShape {
     static constexpr int KSTEPS = D / 16;
@@ -250,6 +258,19 @@ __device__ __forceinline__ bool any_nonfinite(const uint16_t* vb, int lane) {
         bad |= nonfinite_halves(v.x) | nonfinite_halves(v.y) | nonfinite_halves(v.z) | nonfinite_halves(v.w);
     }
     return __any(bad != 0);
+}
+
+// Whether 64 rows of codes from vb on hold NaN.
+template <int D>
+__device__ __forceinline__ bool any_nan_code(const uint8_t* vb, int lane) {
+    uint32_t bad = 0;
+#pragma unroll 1
+    for (int i = 0; i < D / 16; ++i) {
+        const uint4 v = *reinterpret_cast<const uint4*>(vb + 1024 * i + 16 * lane);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bad |= (word_of(v, j) & 0x7f7f7f7fu) + 0x01010101u;
+    }
+    return __any((bad & 0x80808080u) != 0);
 }
 
 template <int D, int NB>
@@ -840,6 +861,99 @@ __device__ __forceinline__ void read_v(uint4 (&v)[2][2], uint32_t at) {
                                    r[4 * db + 2 * tt + 1].y);
 }
 
+// The same of 64 keys in 8 bits: K's k[nb][j] holds the codes of dims 32 j + 16 kg
+// on, of key 32 nb + the lane's; V's v[tt][db] eight keys of 16 tt on at one dim.
+__device__ __forceinline__ void read_k8(uint4 (&k)[2][4], uint2& bases, uint32_t at, uint32_t bases_at) {
+    typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+    typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+    u4_t r[8];
+    u2_t e;
+    asm volatile(
+        "ds_read_b64 %8, %13\n\t"
+        "ds_read_b128 %0, %9\n\t"
+        "ds_read_b128 %1, %10\n\t"
+        "ds_read_b128 %2, %11\n\t"
+        "ds_read_b128 %3, %12\n\t"
+        "ds_read_b128 %4, %9 offset:4096\n\t"
+        "ds_read_b128 %5, %10 offset:4096\n\t"
+        "ds_read_b128 %6, %11 offset:4096\n\t"
+        "ds_read_b128 %7, %12 offset:4096\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]),
+          "=&v"(e)
+        : "v"(at), "v"(at ^ 32), "v"(at ^ 64), "v"(at ^ 96), "v"(bases_at)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) k[i / 4][i % 4] = make_uint4(r[i].x, r[i].y, r[i].z, r[i].w);
+    bases = make_uint2(e.x, e.y);
+}
+__device__ __forceinline__ void read_k8(uint4 (&k)[2][2], uint2& bases, uint32_t at, uint32_t bases_at) {
+    typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+    typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+    u4_t r[4];
+    u2_t e;
+    asm volatile(
+        "ds_read_b64 %4, %7\n\t"
+        "ds_read_b128 %0, %5\n\t"
+        "ds_read_b128 %1, %6\n\t"
+        "ds_read_b128 %2, %5 offset:2048\n\t"
+        "ds_read_b128 %3, %6 offset:2048\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(e)
+        : "v"(at), "v"(at ^ 32), "v"(bases_at)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k[i / 2][i % 2] = make_uint4(r[i].x, r[i].y, r[i].z, r[i].w);
+    bases = make_uint2(e.x, e.y);
+}
+__device__ __forceinline__ void read_v8(uint2 (&v)[4][4], uint32_t at) {
+    typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+    u2_t r[16];  // [db][tt]
+    asm volatile(
+        "ds_read_b64_tr_b8 %0, %16\n\t"
+        "ds_read_b64_tr_b8 %1, %16 offset:2048\n\t"
+        "ds_read_b64_tr_b8 %2, %16 offset:4096\n\t"
+        "ds_read_b64_tr_b8 %3, %16 offset:6144\n\t"
+        "ds_read_b64_tr_b8 %4, %17\n\t"
+        "ds_read_b64_tr_b8 %5, %17 offset:2048\n\t"
+        "ds_read_b64_tr_b8 %6, %17 offset:4096\n\t"
+        "ds_read_b64_tr_b8 %7, %17 offset:6144\n\t"
+        "ds_read_b64_tr_b8 %8, %18\n\t"
+        "ds_read_b64_tr_b8 %9, %18 offset:2048\n\t"
+        "ds_read_b64_tr_b8 %10, %18 offset:4096\n\t"
+        "ds_read_b64_tr_b8 %11, %18 offset:6144\n\t"
+        "ds_read_b64_tr_b8 %12, %19\n\t"
+        "ds_read_b64_tr_b8 %13, %19 offset:2048\n\t"
+        "ds_read_b64_tr_b8 %14, %19 offset:4096\n\t"
+        "ds_read_b64_tr_b8 %15, %19 offset:6144\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]),
+          "=&v"(r[8]), "=&v"(r[9]), "=&v"(r[10]), "=&v"(r[11]), "=&v"(r[12]), "=&v"(r[13]), "=&v"(r[14]), "=&v"(r[15])
+        : "v"(at), "v"(at ^ 32), "v"(at ^ 64), "v"(at ^ 96)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i % 4][i / 4] = make_uint2(r[i].x, r[i].y);
+}
+__device__ __forceinline__ void read_v8(uint2 (&v)[4][2], uint32_t at) {
+    typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+    u2_t r[8];
+    asm volatile(
+        "ds_read_b64_tr_b8 %0, %8\n\t"
+        "ds_read_b64_tr_b8 %1, %8 offset:1024\n\t"
+        "ds_read_b64_tr_b8 %2, %8 offset:2048\n\t"
+        "ds_read_b64_tr_b8 %3, %8 offset:3072\n\t"
+        "ds_read_b64_tr_b8 %4, %9\n\t"
+        "ds_read_b64_tr_b8 %5, %9 offset:1024\n\t"
+        "ds_read_b64_tr_b8 %6, %9 offset:2048\n\t"
+        "ds_read_b64_tr_b8 %7, %9 offset:3072\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+        : "v"(at), "v"(at ^ 32)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i % 4][i / 4] = make_uint2(r[i].x, r[i].y);
+}
+
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
     return (uint32_t)(size_t)(const __attribute__((address_space(3))) void*)p;
 }
@@ -884,7 +998,7 @@ __device__ __forceinline__ void stage(const PagedAttnArgs& a, ItemView& v, Paged
     v.head = it.row0 - ahead * v.group;
     v.pos = it.pos0 + (int32_t)ahead;
     uint32_t kind = kSegShared;
-    if (BITS == 16 && it.rows <= 32) {
+    if (it.rows <= 32) {
         kind = kSegStream;
         const uint32_t per_shift = 6 - v.src.entry_shift;
         it.tile_begin = from;
@@ -956,8 +1070,8 @@ __device__ __forceinline__ void advance(const PagedAttnArgs& a, ItemView& v, con
     if (lane == 0) seg->kind = kSegNone;
 }
 
-// Up to 32 rows: wave w < kStreams streams the 32-key halves w, w + kStreams,
-// ... of a segment's tiles, and on into the next segment, which wave kStreams
+// Up to 32 rows: wave w < kStreams streams the steps w, w + kStreams, ... of a
+// segment, 32-key halves of its tiles (16 bits) or whole tiles (8 bits), and on into the next segment, which wave kStreams
 // stages meanwhile: a wave's first loads of it go out behind its last ones of
 // this, and are in flight while the streams merge.  (Staged by all waves after
 // the merge, a new item cost 20 us of its workgroup under load: its ticket, the
@@ -969,12 +1083,17 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
                                                 uint2* s_tab, uint16_t* s_q, float2 (*s_ml)[32], float scale_log2,
                                                 RowView rv) {
     using P = PaShape<D>;
-    constexpr int NL = P::HALF_LOADS, NF = P::NF, NT = 2;  // non-temporal: the keys are read once
+    constexpr int NL = BITS == 16 ? P::HALF_LOADS : D / 16;  // loads of a step's K or V
+    constexpr int NF = P::NF, NT = 2;                        // non-temporal: the keys are read once
+    constexpr uint32_t SPT = BITS == 16 ? 2 : 1;             // steps per tile
+    constexpr int RI = BITS == 16 ? P::RI : 1024 / D;        // rows per load
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ql = lane & 31, kg = lane >> 5;
-    const uint32_t per_shift = 6 - v.src.entry_shift, half = wave & 1;
+    const uint32_t per_shift = 6 - v.src.entry_shift, half = BITS == 16 ? wave & 1 : 0;
     uint16_t* const sk = s_a + (wave % kStreams) * 32 * D;
     uint16_t* const sv = s_b + (wave % kStreams) * 32 * D;
+    // The lane's entry of a tile's.  (8 bits: that of its row, lane.)
+    const uint32_t my_entry = BITS == 16 ? lane & ((1u << per_shift) - 1) : lane >> v.src.entry_shift;
     // The merge lies behind the streams' tiles: stream k's 32 rows in fragment
     // order at merge_at(k).
     const uint32_t merge_a = lds_address(s_a + P::BUF / 2), merge_b = lds_address(s_b + P::BUF / 2);
@@ -983,52 +1102,69 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
         return (k < 2 ? merge_a : merge_b) + (k & 1) * NF * 1024 + 16 * lane;
     };
 
-    const int lr = lane / P::CPR, phys = lane % P::CPR;
-    constexpr int SWZ = D / 8 / P::RI;  // instructions after which K's swizzle repeats
+    constexpr int SWZ = BITS == 16 ? D / 8 / P::RI : 16 / RI;  // loads after which K's swizzle repeats
+    const int lr = BITS == 16 ? lane / P::CPR : lane / (D / 16);
     uint32_t koff[SWZ];
+    [[maybe_unused]] uint32_t voff[8 / P::RI];
+    uint32_t k_at, v_at;
+    if constexpr (BITS == 16) {
+        const int phys = lane % P::CPR;
 #pragma unroll
-    for (int j = 0; j < SWZ; ++j)
-        koff[j] = ((P::RI * j & 7) + lr) * v.src.row_bytes + 16 * (phys ^ pk_swz<D>(P::RI * j + lr));
-    uint32_t voff[8 / P::RI];
+        for (int j = 0; j < SWZ; ++j)
+            koff[j] = ((RI * j & 7) + lr) * v.src.row_bytes + 16 * (phys ^ pk_swz<D>(RI * j + lr));
 #pragma unroll
-    for (int j = 0; j < 8 / P::RI; ++j) voff[j] = (P::RI * j + lr) * v.src.row_bytes + 16 * (phys ^ pv_swz<D>(lr));
-    int v_off[P::DBLK];
-    {
+        for (int j = 0; j < 8 / RI; ++j) voff[j] = (RI * j + lr) * v.src.row_bytes + 16 * (phys ^ pv_swz<D>(lr));
         const int s16 = lane & 15, g16 = lane >> 4, vrow = 4 * kg + (s16 >> 2);
+        k_at = lds_address(sk + ql * D + 8 * (kg ^ pk_swz<D>(ql)));
+        v_at = lds_address(sv + vrow * D + 8 * ((2 * (g16 & 1) + ((s16 & 3) >> 1)) ^ pv_swz<D>(vrow)) + 4 * (s16 & 1));
+    } else {
+        const int phys = lane % (D / 16);
 #pragma unroll
-        for (int db = 0; db < P::DBLK; ++db)
-            v_off[db] = vrow * D + 8 * ((4 * db + 2 * (g16 & 1) + ((s16 & 3) >> 1)) ^ pv_swz<D>(vrow)) + 4 * (s16 & 1);
+        for (int j = 0; j < SWZ; ++j) koff[j] = (RI * j + lr) * D + 16 * (phys ^ p8_swz<D>(RI * j + lr));
+        const int s16 = lane & 15, g16 = lane >> 4, vrow = 4 * kg + (s16 >> 1 & 3) + (s16 & 8);
+        k_at = lds_address(reinterpret_cast<const uint8_t*>(sk) + ql * D + 16 * (kg ^ p8_swz<D>(ql)));
+        v_at = lds_address(reinterpret_cast<const uint8_t*>(sv) + vrow * D + 16 * ((g16 & 1) ^ p8_swz<D>(vrow)) + 8 * (s16 & 1));
     }
-    const uint32_t k_at = lds_address(sk + ql * D + 8 * (kg ^ pk_swz<D>(ql))), v_at = lds_address(sv + v_off[0]);
-    // This wave's halves lie in one half of their tiles.
-    auto fill_k = [&](const char* from, uint2 bases) __attribute__((always_inline)) {
+    // K or V of a step, one after the other into its place.  Rows of one page lie
+    // together: eight (16 bits, a wave's halves lie in one half of their tiles) or
+    // the 16 of a block.
+    auto fill = [&](const char* from, uint2 bases, uint16_t* to, const uint32_t* off, int period)
+                    __attribute__((always_inline)) {
+        constexpr int GROUP = BITS == 16 ? 8 : kFp8Block;
+        constexpr int ROWS = BITS == 16 ? 32 : 64;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {  // eight rows: one page
-            const uint32_t r = 32 * half + 8 * g;
-            const __amdgpu_buffer_rsrc_t rows = rows_at(from + base_of(bases, r >> v.src.entry_shift) +
-                                                        (r & ((1u << v.src.entry_shift) - 1)) * v.src.row_bytes);
+        for (int g = 0; g < ROWS / GROUP; ++g) {
+            const uint32_t r = 32 * half + GROUP * g;
+            const __amdgpu_buffer_rsrc_t rows =
+                rows_at(from + base_of(bases, BITS == 16 ? r >> v.src.entry_shift : r) +
+                        (r & ((1u << v.src.entry_shift) - 1)) * v.src.row_bytes);
 #pragma unroll
-            for (int i = 0; i < 8 / P::RI; ++i)
-                load_lds16<NT>(rows, koff[(g * (8 / P::RI) + i) % SWZ], sk + D * (8 * g + P::RI * i));
+            for (int i = 0; i < GROUP / RI; ++i) {
+                const int n = g * (GROUP / RI) + i;
+                load_lds16<NT>(rows, off[n % period], to + 512 * n);
+            }
         }
     };
-    auto fill_v = [&](const char* from, uint2 bases) __attribute__((always_inline)) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const uint32_t r = 32 * half + 8 * g;
-            const __amdgpu_buffer_rsrc_t rows = rows_at(from + base_of(bases, r >> v.src.entry_shift) +
-                                                        (r & ((1u << v.src.entry_shift) - 1)) * v.src.row_bytes);
-#pragma unroll
-            for (int i = 0; i < 8 / P::RI; ++i) load_lds16<NT>(rows, voff[i], sv + D * (8 * g + P::RI * i));
-        }
+    // (16 bits: V's swizzle repeats after eight rows; 8 bits: V's is K's.)
+    const uint32_t* const v_offsets = BITS == 16 ? voff : koff;
+    constexpr int V_PERIOD = BITS == 16 ? 8 / P::RI : SWZ;
+    // 8 bits: the scale of the block that row `lane` of the tile at key0 lies in.
+    [[maybe_unused]] auto scale_of = [&](const char* from, uint64_t scales, uint2 bases, uint32_t key0)
+                                         __attribute__((always_inline)) {
+        const uint32_t in_entry = (1u << v.src.entry_shift) - 1;
+        const uint32_t row = key0 & ((1u << v.src.page_shift) - 1) & ~in_entry;  // of the entry's first key
+        const uint64_t base = (uint64_t)bases.y << 32 | bases.x;
+        return *reinterpret_cast<const float*>(from + (base - (uint64_t)row * D + scales) +
+                                               (row + (lane & in_entry)) / kFp8Block * sizeof(float));
     };
-    // Entry of half h of a segment that begins at tile c0.
+    // Entry of step h of a segment that begins at tile c0.
     auto entry_of = [&](uint32_t at, uint32_t h, uint32_t c0) __attribute__((always_inline)) {
-        return s_tab + at * kSegEntries + (((h >> 1) - c0) << per_shift) + (lane & ((1u << per_shift) - 1));
+        return s_tab + at * kSegEntries + ((h / SPT - c0) << per_shift) + my_entry;
     };
-    // Of a segment: the halves that hold a key which is seen end here.
+    // Of a segment: the steps that hold a key which is seen end here.
     auto end_of = [&](const PagedItem& it) __attribute__((always_inline)) {
-        if (it.tile_end <= it.tile_begin) return 2 * it.tile_begin;
+        if (it.tile_end <= it.tile_begin) return SPT * it.tile_begin;
+        if (BITS == 8) return it.tile_end;
         KeySource k = v.src;
         k.low_tile = it.low_tile;
         k.sink_tiles = it.sink_tiles;
@@ -1107,6 +1243,7 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
     RowState<D> s;
     bf16x8_t qf[P::KSTEPS];
     bool armed = false;  // this wave's first loads of the segment are out
+    [[maybe_unused]] float k_scale = 0.0f, v_scale = 0.0f;  // of the step to come
     while (true) {
         const Segment seg = segment(slot);
         if (seg.kind != kSegStream) return slot;
@@ -1117,89 +1254,177 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
         rv.pos = v.pos + (int32_t)tokens_on(v, row);
         rv.span(v.pos, v.pos + (int32_t)__builtin_amdgcn_readfirstlane(tokens_on(v, last_row)));
         const uint32_t c0 = seg.it.tile_begin, end = end_of(seg.it);
-        uint32_t h = 2 * c0 + wave;
+        uint32_t h = SPT * c0 + wave;
         const uint32_t n = h < end ? (end - h + kStreams - 1) / kStreams : 0;
         if (!armed && n) {
             const uint2 bases = *entry_of(slot, h, c0);
-            fill_k(v.src.k, bases);
-            fill_v(v.src.v, bases);
+            if constexpr (BITS == 8) {
+                k_scale = scale_of(v.src.k, v.src.scales, bases, v.src.key0(h));
+                v_scale = scale_of(v.src.v, v.src.scales, bases, v.src.key0(h));
+                asm volatile("" ::: "memory");  // (the waits count on their order)
+            }
+            fill(v.src.k, bases, sk, koff, SWZ);
+            fill(v.src.v, bases, sv, v_offsets, V_PERIOD);
         }
         if (seg.opens) {
             const uint16_t* const q = s_q + slot * 32 * D + row * D;
 #pragma unroll
             for (int ks = 0; ks < P::KSTEPS; ++ks)
-                qf[ks] = as_bf16x8(*reinterpret_cast<const uint4*>(q + 8 * ((2 * ks + kg) ^ pk_swz<D>(row))));
+                // (8 bits: k-steps 2 j and 2 j + 1 take the halves of K's 16-byte reads.)
+                qf[ks] = as_bf16x8(*reinterpret_cast<const uint4*>(
+                    q + 8 * ((BITS == 16 ? 2 * ks + kg : 4 * (ks / 2) + 2 * kg + (ks & 1)) ^ pk_swz<D>(row))));
             clear(s);
         }
         // The next segment is known from this iteration on.
         const uint32_t meet = n > 2 ? 2 : n ? n - 1 : 0;
         const char *next_k = nullptr, *next_v = nullptr;
         uint32_t next_c0 = 0;
+        [[maybe_unused]] uint32_t next_key0 = 0;
+        [[maybe_unused]] uint64_t next_scales = 0;
         auto look_ahead = [&]() __attribute__((always_inline)) {
             lds_ops_barrier();
             const Segment nx = segment(slot ^ 1);
             if (nx.kind != kSegStream) return;
             next_c0 = nx.it.tile_begin;
-            next_has = 2 * next_c0 + wave < end_of(nx.it);
+            next_has = SPT * next_c0 + wave < end_of(nx.it);
+            if constexpr (BITS == 8) {
+                ItemView w = v;
+                point_at<BITS>(w, a, nx);
+                next_key0 = w.src.key0(next_c0 + wave);
+                next_scales = w.src.scales;
+            }
             next_k = head_rows<BITS>(a.k_cache, a, nx.kvh);
             next_v = head_rows<BITS>(a.v_cache, a, nx.kvh);
         };
         if (n == 0) {
             look_ahead();
             if (next_has) {
-                const uint2 bases = *entry_of(slot ^ 1, 2 * next_c0 + wave, next_c0);
-                fill_k(next_k, bases);
-                fill_v(next_v, bases);
+                const uint2 bases = *entry_of(slot ^ 1, SPT * next_c0 + wave, next_c0);
+                if constexpr (BITS == 8) {
+                    k_scale = scale_of(next_k, next_scales, bases, next_key0);
+                    v_scale = scale_of(next_v, next_scales, bases, next_key0);
+                    asm volatile("" ::: "memory");  // (the waits count on their order)
+                }
+                fill(next_k, bases, sk, koff, SWZ);
+                fill(next_v, bases, sv, v_offsets, V_PERIOD);
             }
         }
         for (uint32_t i = 0; i < n; ++i, h += kStreams) {
             if (i == meet) look_ahead();
-            const uint32_t k0 = v.src.key0(h >> 1) + 32 * half;
+            const uint32_t k0 = v.src.key0(h / SPT) + 32 * half;
             const bool inside = i + 1 < n, more = inside || next_has;
             const char* const from_k = inside ? v.src.k : next_k;
             const char* const from_v = inside ? v.src.v : next_v;
             const uint2* const entry = inside     ? entry_of(slot, h + kStreams, c0)
-                                       : next_has ? entry_of(slot ^ 1, 2 * next_c0 + wave, next_c0)
+                                       : next_has ? entry_of(slot ^ 1, SPT * next_c0 + wave, next_c0)
                                                   : entry_of(slot, h, c0);
-            // K has landed (V, requested after it, may not have): its operands
-            // to registers, then the next K into its place.
-            __builtin_amdgcn_s_waitcnt(wait_vmcnt(NL));
-            uint4 ka[P::KSTEPS];
-            uint2 bases;
-            read_k(ka, bases, k_at, lds_address(entry));
-            if (more) fill_k(from_k, bases);
-            f32x16_t st[1];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) st[0][j] = 0.0f;
-#pragma unroll
-            for (int ks = 0; ks < P::KSTEPS; ++ks) st[0] = mfma32x32x16(as_bf16x8(ka[ks]), qf[ks], st[0]);
-            const uint32_t k1 = k0 + 31;
-            const bool hidden = rv.some_hidden(k0, k1);
-            if (hidden) hide<D, 1>(st, rv, k0, kg);
-            bf16x8_t pf[2];
-            probabilities<D, 1>(st, s, pf, scale_log2);
-            // V likewise: of what is in flight only the next K came after it.
-            if (more)
+            if constexpr (BITS == 16) {
+                // K has landed (V, requested after it, may not have): its operands
+                // to registers, then the next K into its place.
                 __builtin_amdgcn_s_waitcnt(wait_vmcnt(NL));
-            else
-                __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
-            if (hidden) {
-                asm volatile("" ::: "memory");
-#pragma unroll
-                for (int j = 0; j < NL; ++j)
-                    if (k0 + P::RI * j + lr >= v.src.key_end)
-                        *reinterpret_cast<uint4*>(sv + 512 * j + 8 * lane) = make_uint4(0, 0, 0, 0);
-                __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
-                if (rv.some_hidden(k0, min(k1, v.src.key_end - 1)) && any_nonfinite<D, 1>(sv, lane)) s_seg[slot].spoilt = 1;
+                uint4 ka[P::KSTEPS];
+                uint2 bases;
+                read_k(ka, bases, k_at, lds_address(entry));
+                if (more) fill(from_k, bases, sk, koff, SWZ);
+                f32x16_t st[1];
+    #pragma unroll
+                for (int j = 0; j < 16; ++j) st[0][j] = 0.0f;
+    #pragma unroll
+                for (int ks = 0; ks < P::KSTEPS; ++ks) st[0] = mfma32x32x16(as_bf16x8(ka[ks]), qf[ks], st[0]);
+                const uint32_t k1 = k0 + 31;
+                const bool hidden = rv.some_hidden(k0, k1);
+                if (hidden) hide<D, 1>(st, rv, k0, kg);
+                bf16x8_t pf[2];
+                probabilities<D, 1>(st, s, pf, scale_log2);
+                // V likewise: of what is in flight only the next K came after it.
+                if (more)
+                    __builtin_amdgcn_s_waitcnt(wait_vmcnt(NL));
+                else
+                    __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+                if (hidden) {
+                    asm volatile("" ::: "memory");
+    #pragma unroll
+                    for (int j = 0; j < NL; ++j)
+                        if (k0 + P::RI * j + lr >= v.src.key_end)
+                            *reinterpret_cast<uint4*>(sv + 512 * j + 8 * lane) = make_uint4(0, 0, 0, 0);
+                    __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+                    if (rv.some_hidden(k0, min(k1, v.src.key_end - 1)) && any_nonfinite<D, 1>(sv, lane)) s_seg[slot].spoilt = 1;
+                }
+                uint4 va[2][P::DBLK];
+                read_v(va, v_at);
+                if (more) fill(from_v, bases, sv, v_offsets, V_PERIOD);
+    #pragma unroll
+                for (int tt = 0; tt < 2; ++tt)
+    #pragma unroll
+                    for (int db = 0; db < P::DBLK; ++db)
+                        s.o[db] = mfma32x32x16(as_bf16x8(va[tt][db]), pf[tt], s.o[db]);
+            } else {
+                // As above, with the step's scales ahead of its K.
+                constexpr int J = D / 32;
+                __builtin_amdgcn_s_waitcnt(wait_vmcnt(NL));
+                const uint32_t ks_bits = __float_as_uint(k_scale), vs_bits = __float_as_uint(v_scale);
+                uint4 ka[2][J];
+                uint2 bases;
+                read_k8(ka, bases, k_at, lds_address(entry));
+                if (more) {
+                    const uint32_t key0 = inside ? v.src.key0(h + kStreams) : next_key0;
+                    const uint64_t scales = inside ? v.src.scales : next_scales;
+                    k_scale = scale_of(from_k, scales, bases, key0);
+                    v_scale = scale_of(from_v, scales, bases, key0);
+                    asm volatile("" ::: "memory");  // (the waits count on their order)
+                    fill(from_k, bases, sk, koff, SWZ);
+                }
+                // Lanes hold their row's block: those of rows 0 to 31 and 32 to 63.
+                const auto kn = __builtin_amdgcn_permlane32_swap(ks_bits, ks_bits, false, false);
+                f32x16_t st[2];
+    #pragma unroll
+                for (int nb = 0; nb < 2; ++nb) {
+                    const float scale = __uint_as_float(kn[nb]);
+    #pragma unroll
+                    for (int j = 0; j < 16; ++j) st[nb][j] = 0.0f;
+    #pragma unroll
+                    for (int j = 0; j < J; ++j) {
+                        const uint4 x = ka[nb][j];
+                        st[nb] = mfma32x32x16(as_bf16x8(fp8x8_to_bf16(make_uint2(x.x, x.y), scale)), qf[2 * j], st[nb]);
+                        st[nb] = mfma32x32x16(as_bf16x8(fp8x8_to_bf16(make_uint2(x.z, x.w), scale)), qf[2 * j + 1], st[nb]);
+                    }
+                }
+                const uint32_t k1 = k0 + 63;
+                const bool hidden = rv.some_hidden(k0, k1);
+                if (hidden) hide<D, 2>(st, rv, k0, kg);
+                bf16x8_t pf[4];
+                probabilities<D, 2>(st, s, pf, scale_log2);
+                // Of what is in flight only the next scales and K came after V.
+                if (more)
+                    __builtin_amdgcn_s_waitcnt(wait_vmcnt(NL + 2));
+                else
+                    __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+                uint32_t vs = vs_bits;
+                if (hidden) {
+                    asm volatile("" ::: "memory");
+                    uint8_t* const codes = reinterpret_cast<uint8_t*>(sv);
+    #pragma unroll
+                    for (int j = 0; j < NL; ++j)
+                        if (k0 + RI * j + lr >= v.src.key_end)
+                            *reinterpret_cast<uint4*>(codes + 1024 * j + 16 * lane) = make_uint4(0, 0, 0, 0);
+                    __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+                    // (A block past the last key has any scale.)
+                    if (k0 + (lane & ~(kFp8Block - 1)) >= v.src.key_end) vs = 0x3f800000u;
+                    if (rv.some_hidden(k0, min(k1, v.src.key_end - 1)) &&
+                        (__any((vs & 0x7f800000u) == 0x7f800000u) || any_nan_code<D>(codes, lane)))
+                        s_seg[slot].spoilt = 1;
+                }
+                uint2 va[4][P::DBLK];
+                read_v8(va, v_at);
+                if (more) fill(from_v, bases, sv, v_offsets, V_PERIOD);
+    #pragma unroll
+                for (int tt = 0; tt < 4; ++tt) {
+                    const float scale = __uint_as_float(__builtin_amdgcn_readlane(vs, 16 * tt));
+    #pragma unroll
+                    for (int db = 0; db < P::DBLK; ++db)
+                        s.o[db] = mfma32x32x16(as_bf16x8(fp8x8_to_bf16(va[tt][db], scale)), pf[tt], s.o[db]);
+                }
             }
-            uint4 va[2][P::DBLK];
-            read_v(va, v_at);
-            if (more) fill_v(from_v, bases);
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                for (int db = 0; db < P::DBLK; ++db)
-                    s.o[db] = mfma32x32x16(as_bf16x8(va[tt][db]), pf[tt], s.o[db]);
         }
         if (closes) {
             const float l = xor32_sum(s.l);
