@@ -683,6 +683,7 @@ def paged_attention_bf16(q, k_cache, v_cache, o, block_tables, plan, batch: int,
         workspace.numel() * workspace.element_size(), _stream(stream)))
 
 
+@functools.lru_cache(maxsize=None)
 def paged_fp8_page_bytes(page_size: int, num_kv_heads: int, head_dim: int) -> int:
     """Bytes of a page of an 8-bit cache: codes [heads][rows][dims], then scales
     [heads][rows / 16] in fp32."""
@@ -699,16 +700,24 @@ def paged_fp8_cache(num_pages: int, page_size: int, num_kv_heads: int, head_dim:
     return torch.empty(num_pages, page, dtype=torch.uint8, device=device)
 
 
+@functools.lru_cache(maxsize=None)
+def _byte_type():
+    import torch
+
+    return torch.uint8
+
+
 def _need_cache_fp8(fn: str, device: int, num_pages: int, page_size: int, page_stride: int,
                     num_kv_heads: int, head_dim: int, *caches) -> None:
     """uint8 [pages][bytes], a page in one piece and page_stride bytes from the next."""
-    import torch
-
-    page = paged_fp8_page_bytes(page_size, num_kv_heads, head_dim)
+    uint8 = _byte_type()
+    page, stride = paged_fp8_page_bytes(page_size, num_kv_heads, head_dim), (page_stride, 1)
     for t in caches:
-        if (t.get_device() != device or t.dtype != torch.uint8 or t.dim() != 2
-                or t.shape[0] < num_pages or t.shape[1] < page or t.stride(1) != 1
-                or t.stride(0) != page_stride and num_pages > 1):
+        if t.get_device() != device or t.dtype is not uint8 or t.dim() != 2:
+            raise ToyInferError(fn, ERR_INVALID_ARGUMENT)
+        rows, width = t.shape
+        if (rows < num_pages or width < page
+                or t.stride() != stride and (num_pages > 1 or t.stride(1) != 1)):
             raise ToyInferError(fn, ERR_INVALID_ARGUMENT)
 
 

@@ -75,9 +75,14 @@ __device__ __forceinline__ int pv_swz(int row) { return D == 128 ? 4 * (row & 3)
 
 // Of 8-bit rows: 16-byte chunks, for K's 16-byte operand reads and V's transposing
 // ones, which take eight rows {0-3, 8-11} or {4-7, 12-15} at a chunk and its
-// neighbour.  Four (two) rows fill the banks once (64 dims: 64 bytes).
-template <int D>
+// neighbour, or (NARROW) {0-3, 16-19} + 4 i at one chunk.  Two rows fill the banks
+// once (64 dims: four).
+template <int D, bool NARROW>
 __device__ __forceinline__ int p8_swz(int row) {
+    if (NARROW) {
+        const int high = (row >> 3 ^ row >> 4) & 1;
+        return D == 128 ? (row >> 1 & 3) | high << 2 : (row >> 2 & 1) | high << 1;
+    }
     return D == 128 ? (row & 2) | (row >> 1 & 4) | (row >> 2 & 1) : (row >> 2 & 2) | (row >> 2 & 1);
 }
 
@@ -216,6 +221,82 @@ __device__ __forceinline__ void probabilities(f32x16_t (&st)[NB], RowState<D>& s
     s.l += ts;
 }
 
+// Up to 16 rows on v_mfma_f32_16x16x32_bf16: a lane has row lane & 15 and the keys
+// 4 (lane / 16) + i of each 16.
+template <int D>
+struct NarrowState {
+    f32x4_t o[D / 16];
+    float m, l;  // as RowState's, l this lane's quarter
+};
+template <int D>
+__device__ __forceinline__ void clear(NarrowState<D>& s) {
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s.o[db][i] = 0.0f;
+    s.m = 0.0f;
+    s.l = 0.0f;
+}
+__device__ __forceinline__ float quarters_sum(float x) { return xor32_sum(xor16_sum(x)); }
+
+template <int D>
+__device__ __forceinline__ void probabilities(f32x4_t (&st)[4], NarrowState<D>& s, bf16x8_t (&pf)[2], float scale_log2) {
+    auto probs = [&](float mref) __attribute__((always_inline)) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            float e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                e[j] = __builtin_amdgcn_exp2f(fmaf(st[2 * t + j / 4][j % 4], scale_log2, -mref));
+            const uint4 w = make_uint4(pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3]), pack_bf16x2(e[4], e[5]),
+                                       pack_bf16x2(e[6], e[7]));
+            pf[t] = as_bf16x8(w);
+            sum = sum_bf16x8(w, sum);
+        }
+        return sum;
+    };
+    float ts = probs(s.m);
+    const float mass = quarters_sum(s.l + ts);
+    if (__any(!(ts <= kPaMassMax) || !(mass >= kPaMassMin))) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, st[kb][i]);
+        const float mt = xor32_max(xor16_max(mx)) * scale_log2;
+        const bool first = quarters_sum(s.l) == 0.0f;
+        if (first && mt > -INFINITY) s.m = mt;
+        const bool need = !first && mt > s.m + kPaRescale;
+        if (__any(need)) {
+            float alpha = 1.0f;
+            if (need) {
+                alpha = __builtin_amdgcn_exp2f(s.m - mt);
+                s.m = mt;
+            }
+            s.l *= alpha;
+#pragma unroll
+            for (int db = 0; db < D / 16; ++db) s.o[db] *= alpha;
+        }
+        ts = probs(s.m);
+    }
+    s.l += ts;
+}
+
+__device__ __forceinline__ void hide(f32x4_t (&st)[4], const RowView& rv, uint32_t k0, int kg) {
+    asm volatile("; hidden keys");  // (keeps the branch, as below)
+    const int32_t ago = rv.pos - (int32_t)k0 - 4 * kg;
+    const int32_t sinks = min((int32_t)min(rv.sinks, 0x7fffffffu), rv.pos + 1) - (int32_t)k0 - 4 * kg;
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int32_t c = 16 * kb + i;
+            const float x = c < sinks ? st[kb][i] : -INFINITY;
+            st[kb][i] = (uint32_t)(ago - c) < rv.window ? st[kb][i] : x;
+        }
+}
+
 // Minus infinity over the scores of keys that this lane's row does not see.
 template <int D, int NB>
 __device__ __forceinline__ void hide(f32x16_t (&st)[NB], const RowView& rv, uint32_t k0, int kg) {
@@ -258,19 +339,6 @@ __device__ __forceinline__ bool any_nonfinite(const uint16_t* vb, int lane) {
         bad |= nonfinite_halves(v.x) | nonfinite_halves(v.y) | nonfinite_halves(v.z) | nonfinite_halves(v.w);
     }
     return __any(bad != 0);
-}
-
-// Whether 64 rows of codes from vb on hold NaN.
-template <int D>
-__device__ __forceinline__ bool any_nan_code(const uint8_t* vb, int lane) {
-    uint32_t bad = 0;
-#pragma unroll 1
-    for (int i = 0; i < D / 16; ++i) {
-        const uint4 v = *reinterpret_cast<const uint4*>(vb + 1024 * i + 16 * lane);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) bad |= (word_of(v, j) & 0x7f7f7f7fu) + 0x01010101u;
-    }
-    return __any((bad & 0x80808080u) != 0);
 }
 
 template <int D, int NB>
@@ -954,6 +1022,163 @@ __device__ __forceinline__ void read_v8(uint2 (&v)[4][2], uint32_t at) {
     for (int i = 0; i < 8; ++i) v[i % 4][i / 4] = make_uint2(r[i].x, r[i].y);
 }
 
+// 16 bytes of LDS, and 16 zeros into it, likewise.
+__device__ __forceinline__ uint4 lds_read16(uint32_t at) {
+    typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+    u4_t r;
+    asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(r) : "v"(at) : "memory");
+    return make_uint4(r.x, r.y, r.z, r.w);
+}
+__device__ __forceinline__ void lds_zero16(uint32_t at) {
+    const f32x4_t z = {0.0f, 0.0f, 0.0f, 0.0f};
+    asm volatile("ds_write_b128 %0, %1" ::"v"(at), "v"(z) : "memory");
+}
+// Whether the 64 rows of codes hold NaN, of which a lane's first 16 are at `at`.
+template <int D>
+__device__ __forceinline__ bool any_nan_code(uint32_t at) {
+    uint32_t bad = 0;
+#pragma unroll 1
+    for (int i = 0; i < D / 16; ++i) {
+        const uint4 v = lds_read16(at + 1024 * i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bad |= (word_of(v, j) & 0x7f7f7f7fu) + 0x01010101u;
+    }
+    return __any((bad & 0x80808080u) != 0);
+}
+// Queries of the lane's row, k-step ks's at `at` ^ (its chunk of the first's).
+template <int KSTEPS>
+__device__ __forceinline__ void read_q(bf16x8_t (&q)[KSTEPS], const uint32_t (&at)[KSTEPS]) {
+    typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+    u4_t r[KSTEPS];
+    if constexpr (KSTEPS == 8)
+        asm volatile(
+            "ds_read_b128 %0, %8\n\t"
+            "ds_read_b128 %1, %9\n\t"
+            "ds_read_b128 %2, %10\n\t"
+            "ds_read_b128 %3, %11\n\t"
+            "ds_read_b128 %4, %12\n\t"
+            "ds_read_b128 %5, %13\n\t"
+            "ds_read_b128 %6, %14\n\t"
+            "ds_read_b128 %7, %15\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+            : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[4]), "v"(at[5]), "v"(at[6]), "v"(at[7])
+            : "memory");
+    else if constexpr (KSTEPS == 4)
+        asm volatile(
+            "ds_read_b128 %0, %4\n\t"
+            "ds_read_b128 %1, %5\n\t"
+            "ds_read_b128 %2, %6\n\t"
+            "ds_read_b128 %3, %7\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+            : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3])
+            : "memory");
+    else
+        asm volatile(
+            "ds_read_b128 %0, %2\n\t"
+            "ds_read_b128 %1, %3\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(r[0]), "=&v"(r[1])
+            : "v"(at[0]), "v"(at[1])
+            : "memory");
+#pragma unroll
+    for (int i = 0; i < KSTEPS; ++i) q[i] = __builtin_bit_cast(bf16x8_t, r[i]);
+}
+
+// Of up to 16 rows: k[kb][j] the codes of dims 64 j + 16 kg on, of key 16 kb + the
+// lane's; v[t][db] keys 32 t + 4 kg on and 16 further, four each, at one dim.
+__device__ __forceinline__ void read_k8(uint4 (&k)[4][2], uint2& bases, uint32_t at, uint32_t bases_at) {
+    typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+    typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+    u4_t r[8];
+    u2_t e;
+    asm volatile(
+        "ds_read_b64 %8, %11\n\t"
+        "ds_read_b128 %0, %9\n\t"
+        "ds_read_b128 %1, %10\n\t"
+        "ds_read_b128 %2, %10 offset:2048\n\t"
+        "ds_read_b128 %3, %9 offset:2048\n\t"
+        "ds_read_b128 %4, %9 offset:4096\n\t"
+        "ds_read_b128 %5, %10 offset:4096\n\t"
+        "ds_read_b128 %6, %10 offset:6144\n\t"
+        "ds_read_b128 %7, %9 offset:6144\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]),
+          "=&v"(e)
+        : "v"(at), "v"(at ^ 64), "v"(bases_at)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) k[i / 2][i % 2] = make_uint4(r[i].x, r[i].y, r[i].z, r[i].w);
+    bases = make_uint2(e.x, e.y);
+}
+__device__ __forceinline__ void read_k8(uint4 (&k)[4][1], uint2& bases, uint32_t at, uint32_t bases_at) {
+    typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+    typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+    u4_t r[4];
+    u2_t e;
+    asm volatile(
+        "ds_read_b64 %4, %7\n\t"
+        "ds_read_b128 %0, %5\n\t"
+        "ds_read_b128 %1, %6 offset:1024\n\t"
+        "ds_read_b128 %2, %5 offset:2048\n\t"
+        "ds_read_b128 %3, %6 offset:3072\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(e)
+        : "v"(at), "v"(at ^ 32), "v"(bases_at)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k[i][0] = make_uint4(r[i].x, r[i].y, r[i].z, r[i].w);
+    bases = make_uint2(e.x, e.y);
+}
+__device__ __forceinline__ void read_v8(uint2 (&v)[2][8], uint32_t at) {
+    typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+    u2_t r[16];  // [db][t]
+    asm volatile(
+        "ds_read_b64_tr_b8 %0, %16\n\t"
+        "ds_read_b64_tr_b8 %1, %16 offset:4096\n\t"
+        "ds_read_b64_tr_b8 %2, %17\n\t"
+        "ds_read_b64_tr_b8 %3, %17 offset:4096\n\t"
+        "ds_read_b64_tr_b8 %4, %18\n\t"
+        "ds_read_b64_tr_b8 %5, %18 offset:4096\n\t"
+        "ds_read_b64_tr_b8 %6, %19\n\t"
+        "ds_read_b64_tr_b8 %7, %19 offset:4096\n\t"
+        "ds_read_b64_tr_b8 %8, %20\n\t"
+        "ds_read_b64_tr_b8 %9, %20 offset:4096\n\t"
+        "ds_read_b64_tr_b8 %10, %21\n\t"
+        "ds_read_b64_tr_b8 %11, %21 offset:4096\n\t"
+        "ds_read_b64_tr_b8 %12, %22\n\t"
+        "ds_read_b64_tr_b8 %13, %22 offset:4096\n\t"
+        "ds_read_b64_tr_b8 %14, %23\n\t"
+        "ds_read_b64_tr_b8 %15, %23 offset:4096\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]),
+          "=&v"(r[8]), "=&v"(r[9]), "=&v"(r[10]), "=&v"(r[11]), "=&v"(r[12]), "=&v"(r[13]), "=&v"(r[14]), "=&v"(r[15])
+        : "v"(at), "v"(at ^ 16), "v"(at ^ 32), "v"(at ^ 48), "v"(at ^ 64), "v"(at ^ 80), "v"(at ^ 96), "v"(at ^ 112)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i % 2][i / 2] = make_uint2(r[i].x, r[i].y);
+}
+__device__ __forceinline__ void read_v8(uint2 (&v)[2][4], uint32_t at) {
+    typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+    u2_t r[8];
+    asm volatile(
+        "ds_read_b64_tr_b8 %0, %8\n\t"
+        "ds_read_b64_tr_b8 %1, %8 offset:2048\n\t"
+        "ds_read_b64_tr_b8 %2, %9\n\t"
+        "ds_read_b64_tr_b8 %3, %9 offset:2048\n\t"
+        "ds_read_b64_tr_b8 %4, %10\n\t"
+        "ds_read_b64_tr_b8 %5, %10 offset:2048\n\t"
+        "ds_read_b64_tr_b8 %6, %11\n\t"
+        "ds_read_b64_tr_b8 %7, %11 offset:2048\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
+        : "v"(at), "v"(at ^ 16), "v"(at ^ 32), "v"(at ^ 48)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i % 2][i / 2] = make_uint2(r[i].x, r[i].y);
+}
+
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
     return (uint32_t)(size_t)(const __attribute__((address_space(3))) void*)p;
 }
@@ -983,7 +1208,26 @@ struct PlanHead {
     }
 };
 
-enum : uint32_t { kSegNone = 0, kSegStream = 1, kSegShared = 2 };
+// A streaming wave's state and scores, by the rows that its products hold.
+template <int D, int ROWS>
+struct StreamState {
+    typedef RowState<D> T;
+    typedef f32x16_t Scores;
+};
+template <int D>
+struct StreamState<D, 16> {
+    typedef NarrowState<D> T;
+    typedef f32x4_t Scores;
+};
+__device__ __forceinline__ f32x16_t products(bf16x8_t a, bf16x8_t b, f32x16_t c) { return mfma32x32x16(a, b, c); }
+__device__ __forceinline__ f32x4_t products(bf16x8_t a, bf16x8_t b, f32x4_t c) { return mfma16x16x32(a, b, c); }
+
+enum : uint32_t { kSegNone = 0, kSegStream = 1, kSegShared = 2, kSegNarrow = 3 };
+// A streamed segment's kind: up to 16 rows in 8 bits have a form of their own.
+template <int BITS>
+__device__ __forceinline__ uint32_t stream_kind(uint32_t rows) {
+    return BITS == 8 && rows <= 16 ? kSegNarrow : kSegStream;
+}
 
 // By one wave: `it` of KV head `kvh` from tile `from` on as a segment, with the
 // table and the query rows of a streamed one.
@@ -999,7 +1243,7 @@ __device__ __forceinline__ void stage(const PagedAttnArgs& a, ItemView& v, Paged
     v.pos = it.pos0 + (int32_t)ahead;
     uint32_t kind = kSegShared;
     if (it.rows <= 32) {
-        kind = kSegStream;
+        kind = stream_kind<BITS>(it.rows);
         const uint32_t per_shift = 6 - v.src.entry_shift;
         it.tile_begin = from;
         it.tile_end = min(item_end, from + (kSegEntries >> per_shift));
@@ -1077,18 +1321,20 @@ __device__ __forceinline__ void advance(const PagedAttnArgs& a, ItemView& v, con
 // the merge, a new item cost 20 us of its workgroup under load: its ticket, the
 // item, the table and the first keys are fetched one after the other.)
 // Runs segments from `slot` on; returns the slot of one that is not streamed.
-template <int D, int BITS>
+template <int D, int BITS, int ROWS>
 __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView v, const PlanHead& head,
                                                 uint32_t slot, Segment* s_seg, uint16_t* s_a, uint16_t* s_b,
                                                 uint2* s_tab, uint16_t* s_q, float2 (*s_ml)[32], float scale_log2,
                                                 RowView rv) {
     using P = PaShape<D>;
+    constexpr bool NARROW = ROWS == 16;
+    constexpr uint32_t KIND = NARROW ? kSegNarrow : kSegStream;
     constexpr int NL = BITS == 16 ? P::HALF_LOADS : D / 16;  // loads of a step's K or V
     constexpr int NF = P::NF, NT = 2;                        // non-temporal: the keys are read once
     constexpr uint32_t SPT = BITS == 16 ? 2 : 1;             // steps per tile
     constexpr int RI = BITS == 16 ? P::RI : 1024 / D;        // rows per load
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int ql = lane & 31, kg = lane >> 5;
+    const int ql = lane & (ROWS - 1), kg = lane / ROWS;
     const uint32_t per_shift = 6 - v.src.entry_shift, half = BITS == 16 ? wave & 1 : 0;
     uint16_t* const sk = s_a + (wave % kStreams) * 32 * D;
     uint16_t* const sv = s_b + (wave % kStreams) * 32 * D;
@@ -1102,7 +1348,7 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
         return (k < 2 ? merge_a : merge_b) + (k & 1) * NF * 1024 + 16 * lane;
     };
 
-    constexpr int SWZ = BITS == 16 ? D / 8 / P::RI : 16 / RI;  // loads after which K's swizzle repeats
+    constexpr int SWZ = BITS == 16 ? D / 8 / P::RI : (NARROW ? 32 : 16) / RI;  // loads after which K's swizzle repeats
     const int lr = BITS == 16 ? lane / P::CPR : lane / (D / 16);
     uint32_t koff[SWZ];
     [[maybe_unused]] uint32_t voff[8 / P::RI];
@@ -1120,10 +1366,13 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
     } else {
         const int phys = lane % (D / 16);
 #pragma unroll
-        for (int j = 0; j < SWZ; ++j) koff[j] = (RI * j + lr) * D + 16 * (phys ^ p8_swz<D>(RI * j + lr));
-        const int s16 = lane & 15, g16 = lane >> 4, vrow = 4 * kg + (s16 >> 1 & 3) + (s16 & 8);
-        k_at = lds_address(reinterpret_cast<const uint8_t*>(sk) + ql * D + 16 * (kg ^ p8_swz<D>(ql)));
-        v_at = lds_address(reinterpret_cast<const uint8_t*>(sv) + vrow * D + 16 * ((g16 & 1) ^ p8_swz<D>(vrow)) + 8 * (s16 & 1));
+        for (int j = 0; j < SWZ; ++j)
+            koff[j] = ((RI * j + lr) & (kFp8Block - 1)) * D + 16 * (phys ^ p8_swz<D, NARROW>(RI * j + lr));
+        const int s16 = lane & 15, g16 = NARROW ? 0 : lane >> 4 & 1;
+        const int vrow = 4 * kg + (s16 >> 1 & 3) + (NARROW ? 2 : 1) * (s16 & 8);
+        k_at = lds_address(reinterpret_cast<const uint8_t*>(sk) + ql * D + 16 * (kg ^ p8_swz<D, NARROW>(ql)));
+        v_at = lds_address(reinterpret_cast<const uint8_t*>(sv) + vrow * D + 16 * (g16 ^ p8_swz<D, NARROW>(vrow)) +
+                           8 * (s16 & 1));
     }
     // K or V of a step, one after the other into its place.  Rows of one page lie
     // together: eight (16 bits, a wave's halves lie in one half of their tiles) or
@@ -1131,9 +1380,9 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
     auto fill = [&](const char* from, uint2 bases, uint16_t* to, const uint32_t* off, int period)
                     __attribute__((always_inline)) {
         constexpr int GROUP = BITS == 16 ? 8 : kFp8Block;
-        constexpr int ROWS = BITS == 16 ? 32 : 64;
+        constexpr int STEP = BITS == 16 ? 32 : 64;
 #pragma unroll
-        for (int g = 0; g < ROWS / GROUP; ++g) {
+        for (int g = 0; g < STEP / GROUP; ++g) {
             const uint32_t r = 32 * half + GROUP * g;
             const __amdgpu_buffer_rsrc_t rows =
                 rows_at(from + base_of(bases, BITS == 16 ? r >> v.src.entry_shift : r) +
@@ -1220,7 +1469,7 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
     if (wave >= kStreams) {
         while (true) {
             const Segment seg = segment(slot);
-            if (seg.kind != kSegStream) return slot;
+            if (seg.kind != KIND) return slot;
             point_at<BITS>(v, a, seg);
             const bool closes = seg.it.tile_end == seg.item_end;
             if (wave == kStreams) {
@@ -1240,13 +1489,17 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
             slot ^= 1;
         }
     }
-    RowState<D> s;
-    bf16x8_t qf[P::KSTEPS];
+    constexpr int KSTEPS = D / (512 / ROWS);
+    typename StreamState<D, ROWS>::T s;
+    bf16x8_t qf[KSTEPS];
+    // (What other forms have in flight into these registers' places, the compiler
+    // would wait for where a step first uses them: in every step, for its tiles too.)
+    if constexpr (BITS == 8) __builtin_amdgcn_s_waitcnt(kWaitVmLgkm0);
     bool armed = false;  // this wave's first loads of the segment are out
     [[maybe_unused]] float k_scale = 0.0f, v_scale = 0.0f;  // of the step to come
     while (true) {
         const Segment seg = segment(slot);
-        if (seg.kind != kSegStream) return slot;
+        if (seg.kind != KIND) return slot;
         point_at<BITS>(v, a, seg);
         const bool closes = seg.it.tile_end == seg.item_end;
         bool next_has = false;
@@ -1268,11 +1521,20 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
         }
         if (seg.opens) {
             const uint16_t* const q = s_q + slot * 32 * D + row * D;
+            if constexpr (BITS == 16) {
 #pragma unroll
-            for (int ks = 0; ks < P::KSTEPS; ++ks)
-                // (8 bits: k-steps 2 j and 2 j + 1 take the halves of K's 16-byte reads.)
-                qf[ks] = as_bf16x8(*reinterpret_cast<const uint4*>(
-                    q + 8 * ((BITS == 16 ? 2 * ks + kg : 4 * (ks / 2) + 2 * kg + (ks & 1)) ^ pk_swz<D>(row))));
+                for (int ks = 0; ks < KSTEPS; ++ks)
+                    qf[ks] = as_bf16x8(*reinterpret_cast<const uint4*>(q + 8 * ((2 * ks + kg) ^ pk_swz<D>(row))));
+            } else {
+                // K-steps 2 j and 2 j + 1 take the halves of K's 16-byte reads.  (In asm: of
+                // reads that the compiler knows it waits for the tiles in flight, and where
+                // the queries are first used, in every step.)
+                uint32_t q_at[KSTEPS];
+#pragma unroll
+                for (int ks = 0; ks < KSTEPS; ++ks)
+                    q_at[ks] = lds_address(q + 8 * ((128 / ROWS * (ks / 2) + 2 * kg + (ks & 1)) ^ pk_swz<D>(row)));
+                read_q(qf, q_at);
+            }
             clear(s);
         }
         // The next segment is known from this iteration on.
@@ -1284,7 +1546,7 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
         auto look_ahead = [&]() __attribute__((always_inline)) {
             lds_ops_barrier();
             const Segment nx = segment(slot ^ 1);
-            if (nx.kind != kSegStream) return;
+            if (nx.kind != KIND) return;
             next_c0 = nx.it.tile_begin;
             next_has = SPT * next_c0 + wave < end_of(nx.it);
             if constexpr (BITS == 8) {
@@ -1327,9 +1589,9 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
                 read_k(ka, bases, k_at, lds_address(entry));
                 if (more) fill(from_k, bases, sk, koff, SWZ);
                 f32x16_t st[1];
-    #pragma unroll
+#pragma unroll
                 for (int j = 0; j < 16; ++j) st[0][j] = 0.0f;
-    #pragma unroll
+#pragma unroll
                 for (int ks = 0; ks < P::KSTEPS; ++ks) st[0] = mfma32x32x16(as_bf16x8(ka[ks]), qf[ks], st[0]);
                 const uint32_t k1 = k0 + 31;
                 const bool hidden = rv.some_hidden(k0, k1);
@@ -1343,7 +1605,7 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
                     __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
                 if (hidden) {
                     asm volatile("" ::: "memory");
-    #pragma unroll
+#pragma unroll
                     for (int j = 0; j < NL; ++j)
                         if (k0 + P::RI * j + lr >= v.src.key_end)
                             *reinterpret_cast<uint4*>(sv + 512 * j + 8 * lane) = make_uint4(0, 0, 0, 0);
@@ -1353,17 +1615,17 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
                 uint4 va[2][P::DBLK];
                 read_v(va, v_at);
                 if (more) fill(from_v, bases, sv, v_offsets, V_PERIOD);
-    #pragma unroll
+#pragma unroll
                 for (int tt = 0; tt < 2; ++tt)
-    #pragma unroll
+#pragma unroll
                     for (int db = 0; db < P::DBLK; ++db)
                         s.o[db] = mfma32x32x16(as_bf16x8(va[tt][db]), pf[tt], s.o[db]);
             } else {
                 // As above, with the step's scales ahead of its K.
-                constexpr int J = D / 32;
+                constexpr int NB = 64 / ROWS;
                 __builtin_amdgcn_s_waitcnt(wait_vmcnt(NL));
                 const uint32_t ks_bits = __float_as_uint(k_scale), vs_bits = __float_as_uint(v_scale);
-                uint4 ka[2][J];
+                uint4 ka[NB][KSTEPS / 2];
                 uint2 bases;
                 read_k8(ka, bases, k_at, lds_address(entry));
                 if (more) {
@@ -1374,26 +1636,38 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
                     asm volatile("" ::: "memory");  // (the waits count on their order)
                     fill(from_k, bases, sk, koff, SWZ);
                 }
-                // Lanes hold their row's block: those of rows 0 to 31 and 32 to 63.
-                const auto kn = __builtin_amdgcn_permlane32_swap(ks_bits, ks_bits, false, false);
-                f32x16_t st[2];
-    #pragma unroll
-                for (int nb = 0; nb < 2; ++nb) {
-                    const float scale = __uint_as_float(kn[nb]);
-    #pragma unroll
-                    for (int j = 0; j < 16; ++j) st[nb][j] = 0.0f;
-    #pragma unroll
-                    for (int j = 0; j < J; ++j) {
-                        const uint4 x = ka[nb][j];
-                        st[nb] = mfma32x32x16(as_bf16x8(fp8x8_to_bf16(make_uint2(x.x, x.y), scale)), qf[2 * j], st[nb]);
-                        st[nb] = mfma32x32x16(as_bf16x8(fp8x8_to_bf16(make_uint2(x.z, x.w), scale)), qf[2 * j + 1], st[nb]);
-                    }
+                // Lanes hold their row's block.  An operand of 32 keys has two, a
+                // lane's key is in one of them; one of 16 keys is in one.
+                typename StreamState<D, ROWS>::Scores st[NB];
+                [[maybe_unused]] const auto kn = __builtin_amdgcn_permlane32_swap(ks_bits, ks_bits, false, false);
+                float scale[NB];
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    if constexpr (NARROW)
+                        scale[nb] = __uint_as_float(__builtin_amdgcn_readlane(ks_bits, 16 * nb));
+                    else
+                        scale[nb] = __uint_as_float(kn[nb]);
+#pragma unroll
+                    for (int j = 0; j < (int)(sizeof(st[0]) / 4); ++j) st[nb][j] = 0.0f;
                 }
+#pragma unroll
+                for (int ks = 0; ks < KSTEPS; ++ks)
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        const uint4 x = ka[nb][ks / 2];
+                        const uint2 codes = ks & 1 ? make_uint2(x.z, x.w) : make_uint2(x.x, x.y);
+                        st[nb] = products(as_bf16x8(fp8x8_to_bf16(codes, scale[nb])), qf[ks], st[nb]);
+                    }
                 const uint32_t k1 = k0 + 63;
                 const bool hidden = rv.some_hidden(k0, k1);
-                if (hidden) hide<D, 2>(st, rv, k0, kg);
-                bf16x8_t pf[4];
-                probabilities<D, 2>(st, s, pf, scale_log2);
+                bf16x8_t pf[NARROW ? 2 : 4];
+                if constexpr (NARROW) {
+                    if (hidden) hide(st, rv, k0, kg);
+                    probabilities<D>(st, s, pf, scale_log2);
+                } else {
+                    if (hidden) hide<D, 2>(st, rv, k0, kg);
+                    probabilities<D, 2>(st, s, pf, scale_log2);
+                }
                 // Of what is in flight only the next scales and K came after V.
                 if (more)
                     __builtin_amdgcn_s_waitcnt(wait_vmcnt(NL + 2));
@@ -1402,40 +1676,56 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
                 uint32_t vs = vs_bits;
                 if (hidden) {
                     asm volatile("" ::: "memory");
-                    uint8_t* const codes = reinterpret_cast<uint8_t*>(sv);
-    #pragma unroll
+                    const uint32_t codes = lds_address(sv) + 16 * lane;
+#pragma unroll
                     for (int j = 0; j < NL; ++j)
-                        if (k0 + RI * j + lr >= v.src.key_end)
-                            *reinterpret_cast<uint4*>(codes + 1024 * j + 16 * lane) = make_uint4(0, 0, 0, 0);
+                        if (k0 + RI * j + lr >= v.src.key_end) lds_zero16(codes + 1024 * j);
                     __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
                     // (A block past the last key has any scale.)
                     if (k0 + (lane & ~(kFp8Block - 1)) >= v.src.key_end) vs = 0x3f800000u;
                     if (rv.some_hidden(k0, min(k1, v.src.key_end - 1)) &&
-                        (__any((vs & 0x7f800000u) == 0x7f800000u) || any_nan_code<D>(codes, lane)))
+                        (__any((vs & 0x7f800000u) == 0x7f800000u) || any_nan_code<D>(codes)))
                         s_seg[slot].spoilt = 1;
                 }
-                uint2 va[4][P::DBLK];
+                constexpr int VT = NARROW ? 2 : 4, DB = D / ROWS;
+                uint2 va[VT][DB];
                 read_v8(va, v_at);
                 if (more) fill(from_v, bases, sv, v_offsets, V_PERIOD);
-    #pragma unroll
-                for (int tt = 0; tt < 4; ++tt) {
-                    const float scale = __uint_as_float(__builtin_amdgcn_readlane(vs, 16 * tt));
-    #pragma unroll
-                    for (int db = 0; db < P::DBLK; ++db)
-                        s.o[db] = mfma32x32x16(as_bf16x8(fp8x8_to_bf16(va[tt][db], scale)), pf[tt], s.o[db]);
-                }
+                float value_scale[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) value_scale[i] = __uint_as_float(__builtin_amdgcn_readlane(vs, 16 * i));
+#pragma unroll
+                for (int t = 0; t < VT; ++t)
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) {
+                        const uint2 x = va[t][db];
+                        const float lo = value_scale[NARROW ? 2 * t : t], hi = value_scale[NARROW ? 2 * t + 1 : t];
+                        const uint4 w = make_uint4(fp8x2_to_bf16<false>(x.x, lo), fp8x2_to_bf16<true>(x.x, lo),
+                                                   fp8x2_to_bf16<false>(x.y, hi), fp8x2_to_bf16<true>(x.y, hi));
+                        s.o[db] = products(as_bf16x8(w), pf[t], s.o[db]);
+                    }
             }
         }
         if (closes) {
-            const float l = xor32_sum(s.l);
-            const uint32_t to = merge_at(wave);
+            float l;
+            if constexpr (NARROW) {
+                // Into the places of a 32-row block's fragments; rows from 16 on are not there.
+                l = quarters_sum(s.l);
+                const uint32_t to = merge_at(wave) + 1024 * (kg >> 1) + 16 * (ql + 32 * (kg & 1) - lane);
 #pragma unroll
-            for (int f = 0; f < NF; ++f) {
-                const f32x4_t x = {s.o[f / 4][4 * (f % 4)], s.o[f / 4][4 * (f % 4) + 1], s.o[f / 4][4 * (f % 4) + 2],
-                                   s.o[f / 4][4 * (f % 4) + 3]};
-                asm volatile("ds_write_b128 %0, %1 offset:%2" ::"v"(to), "v"(x), "n"(f * 1024) : "memory");
+                for (int db = 0; db < D / 16; ++db)
+                    asm volatile("ds_write_b128 %0, %1 offset:%2" ::"v"(to), "v"(s.o[db]), "n"(db * 2048) : "memory");
+            } else {
+                l = xor32_sum(s.l);
+                const uint32_t to = merge_at(wave);
+#pragma unroll
+                for (int f = 0; f < NF; ++f) {
+                    const f32x4_t x = {s.o[f / 4][4 * (f % 4)], s.o[f / 4][4 * (f % 4) + 1],
+                                       s.o[f / 4][4 * (f % 4) + 2], s.o[f / 4][4 * (f % 4) + 3]};
+                    asm volatile("ds_write_b128 %0, %1 offset:%2" ::"v"(to), "v"(x), "n"(f * 1024) : "memory");
+                }
             }
-            if (lane < 32) s_ml[wave][lane] = make_float2(s.m, l);
+            if (lane < ROWS) s_ml[wave][lane] = make_float2(s.m, l);
         }
         lds_ops_barrier();
         if (closes) merge();
@@ -1484,8 +1774,14 @@ __global__ __launch_bounds__(kPaThreads, 1) void paged_attn_kernel(PagedAttnArgs
     __syncthreads();
     while (s_seg[slot].kind != kSegNone) {
         if (s_seg[slot].kind == kSegStream) {
-            slot = run_streams<D, BITS>(arguments(), v, head, slot, s_seg, s_a, s_b, s_tab, s_q, s_ml, scale_log2, rv);
+            slot = run_streams<D, BITS, 32>(arguments(), v, head, slot, s_seg, s_a, s_b, s_tab, s_q, s_ml, scale_log2, rv);
             continue;
+        }
+        if constexpr (BITS == 8) {
+            if (s_seg[slot].kind == kSegNarrow) {
+                slot = run_streams<D, 8, 16>(arguments(), v, head, slot, s_seg, s_a, s_b, s_tab, s_q, s_ml, scale_log2, rv);
+                continue;
+            }
         }
         Segment seg;
         {

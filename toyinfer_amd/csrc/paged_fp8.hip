@@ -24,7 +24,8 @@
 namespace tiattn {
 namespace {
 
-constexpr int kWindow = 16;  // token rows whose runs a wave takes
+constexpr int kWindow = 16;  // token rows whose runs a workgroup takes
+constexpr uint32_t kWriteWgs = 512;
 
 // The largest of a row's lanes' values, in each of them.
 template <int D>
@@ -35,171 +36,203 @@ __device__ __forceinline__ float row_max(float x) {
     return x;
 }
 
+// By one workgroup: heads [head0, head1) of K or V in a window's runs, PARTS heads
+// at a time, HALVES waves each, of which one has the first 64 / (D / 16) rows of a
+// group and the other the rest.  (Both in one wave took 157 registers and, at 8192
+// tokens, 4 us longer.)
 template <int D>
-__device__ __forceinline__ void write_blocks(const PagedPrologueFp8Args& a, uint32_t window, uint32_t part,
-                                             float* s_most, uint32_t* s_bit) {
-    constexpr int LPR = D / 16, RPP = 64 / LPR, PASSES = 32 / RPP, HALF = D / 2;
-    const int lane = threadIdx.x & 63, g = lane / LPR, c = lane % LPR;
-    const bool is_k = part < a.hkv;
-    const uint32_t head = is_k ? part : part - a.hkv;
+struct WriteShape {
+    static constexpr int LPR = D / 16, RPP = 64 / LPR, HALVES = kWindow / RPP, PARTS = 4 / HALVES;
+};
+struct WriteLds {
+    float most[2][4][32];
+    uint32_t bit[4][32];
+};
+template <int D>
+__device__ __forceinline__ void write_blocks(const PagedPrologueFp8Args& a, uint32_t window, bool is_k, uint32_t head0,
+                                             uint32_t head1, WriteLds& lds) {
+    typedef WriteShape<D> W;
+    constexpr int LPR = W::LPR, HALF = D / 2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane % LPR;
+    const int local = wave / W::HALVES, g = wave % W::HALVES * W::RPP + lane / LPR;
     // Lane i + 1 looks at row i of the 32 from the window's first on, lane 0 at
     // the one before.
     const int64_t look = (int64_t)window * kWindow + lane - 1;
-    const uint32_t slot_at = look >= 0 && look < a.num_tokens && lane <= 32 ? a.slots[look] : kNoSlot;
+    const bool looks = look >= 0 && look < a.num_tokens && lane <= 32;
+    const uint32_t slot_at = looks ? a.slots[look] : kNoSlot;
+    const uint32_t pos_at = looks && is_k ? min(a.positions[look], a.num_positions - 1) : 0;
     const bool live = slot_at < a.num_slots;
     const uint32_t block = live ? slot_at / kFp8Block : kNoSlot, before = __shfl_up(block, 1);
-    const uint32_t has = (uint32_t)(__ballot(live) >> 1);                         // rows with a slot
-    const uint32_t first = (uint32_t)(__ballot(live && block != before) >> 1);    // of a run
+    const uint32_t has = (uint32_t)(__ballot(live) >> 1);                       // rows with a slot
+    const uint32_t first = (uint32_t)(__ballot(live && block != before) >> 1);  // of a run
     const uint32_t own = first & ((1u << kWindow) - 1);
     if (!own) return;
-    const uint32_t past = (~has | first) & ~((1u << kWindow) - 1);
-    const int begin = __builtin_ctz(own), end = past ? __builtin_ctz(past) : 32;
+    const uint32_t edges = ~has | first, past = edges & ~((1u << kWindow) - 1);
+    const int end = past ? __builtin_ctz(past) : 32;
 
-    const uint16_t* const src = is_k ? a.k : a.v;
-    const uint16_t* const weight = is_k ? a.k_weight : nullptr;
     uint8_t* const cache = is_k ? a.k_cache : a.v_cache;
+    const uint32_t in_page = (1u << a.page_shift) - 1;
     uint4 wr = make_uint4(0, 0, 0, 0), wi = wr;
     if (is_k) {
-        wr = ldg16(weight + 8 * c);
-        wi = ldg16(weight + 8 * c + HALF);
+        wr = ldg16(a.k_weight + 8 * c);
+        wi = ldg16(a.k_weight + 8 * c + HALF);
     }
-    float re[PASSES][8], im[PASSES][8], old[PASSES];
-    uint32_t slot[PASSES];
-    bool mine[PASSES];
-    uint4 xr[PASSES], xi[PASSES];
-    const uint32_t in_page = (1u << a.page_shift) - 1;
-    auto page_at = [&](uint32_t s) __attribute__((always_inline)) {
-        return cache + (uint64_t)(s >> a.page_shift) * a.page_bytes;
-    };
-    auto scale_at = [&](uint32_t s) __attribute__((always_inline)) {
-        const uint64_t codes = (uint64_t)a.hkv * D << a.page_shift;
-        return reinterpret_cast<float*>(page_at(s) + codes) + (uint64_t)head * ((in_page + 1) / kFp8Block) +
-               (s & in_page) / kFp8Block;
-    };
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-        const int i = begin + RPP * p + g;
-        mine[p] = i < end && (has >> i & 1);
-        slot[p] = __shfl(slot_at, min(i, 31) + 1);
-        if (!mine[p]) continue;
-        const uint64_t row = (uint64_t)window * kWindow + i;
-        const uint16_t* const from = src + (row * a.hkv + head) * D;
-        xr[p] = ldg16_nt(from + 8 * c);
-        xi[p] = ldg16_nt(from + 8 * c + HALF);
-        old[p] = *scale_at(slot[p]);
-    }
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-        if (!mine[p]) continue;
-        const int i = begin + RPP * p + g;
-        if (is_k) {
-            const uint32_t pos = min(a.positions[(uint64_t)window * kWindow + i], a.num_positions - 1);
+    // Whole runs, up to 16 rows, at a time: a prompt's block, sixteen decoded tokens.
+    // (The same groups in all waves, whose heads differ only.)
+    for (int begin = __builtin_ctz(own), next; begin < end; begin = next) {
+        const uint64_t cuts = ((uint64_t)edges | 1ull << end) & ((2ull << min(begin + kWindow, end)) - (2ull << begin));
+        next = cuts ? 63 - __builtin_clzll(cuts) : min(begin + kWindow, end);
+        const int i = begin + g;
+        const bool mine = i < next && (has >> i & 1);
+        const uint32_t slot = __shfl(slot_at, min(i, 31) + 1), pos = __shfl(pos_at, min(i, 31) + 1);
+        const uint32_t row = slot & in_page, rows = in_page + 1;
+        uint8_t* const page = cache + (mine ? (uint64_t)(slot >> a.page_shift) * a.page_bytes : 0);
+        float* const scales = reinterpret_cast<float*>(page + (uint64_t)a.hkv * D * rows) + (mine ? row / kFp8Block : 0);
+        const uint16_t* const src = (is_k ? a.k : a.v) + (mine ? ((uint64_t)window * kWindow + i) * a.hkv * D + 8 * c : 0);
+        float4 cs[4];
+        if (is_k && mine) {
             const float4* const rope = reinterpret_cast<const float4*>(a.rope + (uint64_t)pos * D + 16 * c);
-            float4 cs[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) cs[k] = rope[k];
-            norm_rope_f32<D>(xr[p], xi[p], wr, wi, cs, a.eps, re[p], im[p]);
-        } else {
-            bf16x8_to_f32(xr[p], re[p]);
-            bf16x8_to_f32(xi[p], im[p]);
         }
-        float most = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float x = fabsf(re[p][k]), y = fabsf(im[p][k]);
-            most = fmaxf(most, x < INFINITY ? x : 0.0f);
-            most = fmaxf(most, y < INFINITY ? y : 0.0f);
-        }
-        most = row_max<D>(most);
-        if (c == 0) {
-            s_most[i] = most;
-            s_bit[i] = 1u << (slot[p] % kFp8Block);
-        }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-        if (!mine[p]) continue;
-        const int i = begin + RPP * p + g;
         // The row's run.
-        const int lead = 31 - __builtin_clz(first & (~0u >> (31 - i)));
-        const uint32_t after = i == 31 ? 0 : (~has | first) & (~0u << (i + 1));
-        const int stop = after ? __builtin_ctz(after) : 32;
-        float most = 0.0f;
+        const int lead = mine ? max(begin, 31 - __builtin_clz(first & (~0u >> (31 - i)))) : 0;
+        const uint32_t after = i >= 31 ? 0 : edges & (~0u << (i + 1));
+        const int stop = min(next, after ? __builtin_ctz(after) : 32);
         uint32_t written = 0;
-        for (int j = lead; j < stop; ++j) {
-            most = fmaxf(most, s_most[j]);
-            written |= s_bit[j];
+
+        uint4 xr, xi;
+        float old_next;
+        auto load = [&](uint32_t head) __attribute__((always_inline)) {
+            const uint64_t h = min(head, a.hkv - 1);
+            xr = ldg16_nt(src + h * D);
+            xi = ldg16_nt(src + h * D + HALF);
+            old_next = scales[h * (rows / kFp8Block)];
+        };
+        uint32_t head = head0 + local;
+        load(head);
+        for (int buf = 0; head - local < head1; head += W::PARTS, buf ^= 1) {
+            float re[8], im[8];
+            const float old = old_next;
+            if (is_k) {
+                norm_rope_f32<D>(xr, xi, wr, wi, cs, a.eps, re, im);
+            } else {
+                bf16x8_to_f32(xr, re);
+                bf16x8_to_f32(xi, im);
+            }
+            if (head - local + W::PARTS < head1) load(head + W::PARTS);
+            const bool active = mine && head < head1;
+            float most = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float x = fabsf(re[k]), y = fabsf(im[k]);
+                most = fmaxf(most, x < INFINITY ? x : 0.0f);
+                most = fmaxf(most, y < INFINITY ? y : 0.0f);
+            }
+            most = row_max<D>(most);
+            if (c == 0 && active) {
+                lds.most[buf][local][i] = most;
+                lds.bit[local][i] = 1u << (row % kFp8Block);
+            }
+            float was_scale = old;
+            asm volatile("" : "+v"(was_scale));  // (has arrived before another wave writes the block's scale)
+            __syncthreads();
+            if (!active) continue;
+            most = 0.0f;
+            written = 0;
+            for (int j = lead; j < stop; ++j) {
+                most = fmaxf(most, lds.most[buf][local][j]);
+                written |= lds.bit[local][j];
+            }
+            const bool opens = (written & 1) || !fp8_scale_valid(was_scale);
+            const int need = fp8_exponent_for(most), was = (int)(__float_as_uint(was_scale) >> 23) - 127;
+            const int e = opens ? need : max(need, was);
+            const float inv = fp8_scale(-e);
+            uint8_t* const codes = page + (uint64_t)head * rows * D;
+            uint8_t* const to = codes + row * D + 8 * c;
+            *reinterpret_cast<uint2*>(to) = make_uint2(fp8x4_of(re[0], re[1], re[2], re[3], inv),
+                                                       fp8x4_of(re[4], re[5], re[6], re[7], inv));
+            *reinterpret_cast<uint2*>(to + HALF) = make_uint2(fp8x4_of(im[0], im[1], im[2], im[3], inv),
+                                                              fp8x4_of(im[4], im[5], im[6], im[7], inv));
+            if (i != lead) continue;
+            if (c == 0) scales[(uint64_t)head * (rows / kFp8Block)] = fp8_scale(e);
+            if (opens || e == was) continue;
+            // The block's other rows under its larger scale.
+            for (uint32_t r = 0; r < kFp8Block; ++r) {
+                if (written >> r & 1) continue;
+                uint4* const at = reinterpret_cast<uint4*>(codes + ((row & ~(kFp8Block - 1)) + r) * D + 16 * c);
+                const uint4 w = *at;
+                auto again = [&](uint32_t x) __attribute__((always_inline)) {
+                    const uint32_t lo = fp8x2_to_bf16<false>(x, was_scale), hi = fp8x2_to_bf16<true>(x, was_scale);
+                    return fp8x4_of(bf16_lo(lo), bf16_hi(lo), bf16_lo(hi), bf16_hi(hi), inv);
+                };
+                *at = make_uint4(again(w.x), again(w.y), again(w.z), again(w.w));
+            }
         }
-        const bool opens = (written & 1) || !fp8_scale_valid(old[p]);
-        const int need = fp8_exponent_for(most), was = (int)(__float_as_uint(old[p]) >> 23) - 127;
-        const int e = opens ? need : max(need, was);
-        const float inv = fp8_scale(-e);
-        uint8_t* const block_rows = page_at(slot[p]) + ((((uint64_t)head << a.page_shift) + (slot[p] & in_page)) & ~(uint64_t)(kFp8Block - 1)) * D;
-        uint8_t* const to = block_rows + slot[p] % kFp8Block * D + 8 * c;
-        *reinterpret_cast<uint2*>(to) = make_uint2(fp8x4_of(re[p][0], re[p][1], re[p][2], re[p][3], inv),
-                                                   fp8x4_of(re[p][4], re[p][5], re[p][6], re[p][7], inv));
-        *reinterpret_cast<uint2*>(to + HALF) = make_uint2(fp8x4_of(im[p][0], im[p][1], im[p][2], im[p][3], inv),
-                                                          fp8x4_of(im[p][4], im[p][5], im[p][6], im[p][7], inv));
-        if (i != lead) continue;
-        if (c == 0) *scale_at(slot[p]) = fp8_scale(e);
-        if (opens || e == was) continue;
-        // The block's other rows under its larger scale.
-        for (uint32_t r = 0; r < kFp8Block; ++r) {
-            if (written >> r & 1) continue;
-            uint4* const at = reinterpret_cast<uint4*>(block_rows + r * D + 16 * c);
-            uint4 w = *at;
-            auto again = [&](uint32_t x) __attribute__((always_inline)) {
-                const uint32_t lo = fp8x2_to_bf16<false>(x, old[p]), hi = fp8x2_to_bf16<true>(x, old[p]);
-                return fp8x4_of(bf16_lo(lo), bf16_hi(lo), bf16_lo(hi), bf16_hi(hi), inv);
-            };
-            *at = make_uint4(again(w.x), again(w.y), again(w.z), again(w.w));
-        }
+        __syncthreads();  // (the next group's rows have other places, but its first head may be this one's buffer)
     }
 }
 
-template <int D>
-__global__ __launch_bounds__(256) void paged_prologue_fp8_kernel(PagedPrologueFp8Args a, uint32_t kv_wgs, uint32_t q_parts) {
+// Workgroups [0, kv_wgs) write K and V, the others Q, a wave R times 64 / (D / 16)
+// heads of a token.
+template <int D, int R>
+__global__ __launch_bounds__(256) void paged_prologue_fp8_kernel(PagedPrologueFp8Args a, uint32_t kv_wgs, uint32_t kv_parts,
+                                                                uint32_t kv_heads, uint32_t q_parts) {
     constexpr int LPR = D / 16, G = 64 / LPR, HALF = D / 2;
-    __shared__ float s_most[4][32];
-    __shared__ uint32_t s_bit[4][32];
-    const int wave = threadIdx.x >> 6;
+    __shared__ WriteLds lds;
     if (blockIdx.x < kv_wgs) {
-        const uint32_t unit = blockIdx.x * 4 + wave, window = unit / (2 * a.hkv);
-        if (window * (uint64_t)kWindow < a.num_tokens)
-            write_blocks<D>(a, window, unit % (2 * a.hkv), s_most[wave], s_bit[wave]);
+        const uint32_t part = blockIdx.x % (2 * kv_parts), head0 = part / 2 * kv_heads;
+        write_blocks<D>(a, blockIdx.x / (2 * kv_parts), part % 2 == 0, head0, min(head0 + kv_heads, a.hkv), lds);
         return;
     }
-    const uint32_t unit = (blockIdx.x - kv_wgs) * 4 + wave, t = unit / q_parts;
+    const uint32_t unit = (blockIdx.x - kv_wgs) * 4 + (threadIdx.x >> 6), t = unit / q_parts;
     if (t >= a.num_tokens) return;
     const int lane = threadIdx.x & 63, c = lane % LPR;
-    const uint32_t row = unit % q_parts * G + lane / LPR, head = min(row, a.hq - 1);
+    const uint32_t head0 = unit % q_parts * (G * R) + lane / LPR;
     const uint32_t pos = min(a.positions[t], a.num_positions - 1);
-    const uint64_t at = ((uint64_t)t * a.hq + head) * D + 8 * c;
-    const uint4 xr = ldg16_nt(a.q + at), xi = ldg16_nt(a.q + at + HALF);
+    const uint64_t at0 = (uint64_t)t * a.hq * D + 8 * c;
+    uint4 xr[R], xi[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const uint64_t at = at0 + (uint64_t)min(head0 + G * r, a.hq - 1) * D;
+        xr[r] = ldg16_nt(a.q + at);
+        xi[r] = ldg16_nt(a.q + at + HALF);
+    }
     const uint4 wr = ldg16(a.q_weight + 8 * c), wi = ldg16(a.q_weight + 8 * c + HALF);
     const float4* const rope = reinterpret_cast<const float4*>(a.rope + (uint64_t)pos * D + 16 * c);
     float4 cs[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) cs[k] = rope[k];
-    float re[8], im[8];
-    norm_rope_f32<D>(xr, xi, wr, wi, cs, a.eps, re, im);
-    if (row < a.hq) {
-        stg16_nt(a.q_out + at, pack_bf16x8(re));
-        stg16_nt(a.q_out + at + HALF, pack_bf16x8(im));
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float re[8], im[8];
+        norm_rope_f32<D>(xr[r], xi[r], wr, wi, cs, a.eps, re, im);
+        if (head0 + G * r < a.hq) {
+            uint16_t* const to = a.q_out + at0 + (uint64_t)(head0 + G * r) * D;
+            stg16_nt(to, pack_bf16x8(re));
+            stg16_nt(to + HALF, pack_bf16x8(im));
+        }
     }
 }
 
 template <int D>
 hipError_t launch_prologue_t(const PagedPrologueFp8Args& a, hipStream_t st) {
-    constexpr uint32_t G = 64 / (D / 16);
-    const uint32_t q_parts = (a.hq + G - 1) / G;
-    const uint64_t kv = ((uint64_t)a.num_tokens + kWindow - 1) / kWindow * 2 * a.hkv, q = (uint64_t)a.num_tokens * q_parts;
-    const uint32_t kv_wgs = (uint32_t)((kv + 3) / 4);
-    hipLaunchKernelGGL((paged_prologue_fp8_kernel<D>), dim3(kv_wgs + (uint32_t)((q + 3) / 4)), dim3(256), 0, st, a, kv_wgs,
-                       q_parts);
+    typedef WriteShape<D> W;
+    const uint32_t windows = (a.num_tokens + kWindow - 1) / kWindow;
+    // Heads that a workgroup takes one after the other, the next one's rows on their
+    // way; all at once while that leaves compute units without a workgroup.
+    uint32_t kv_heads = W::PARTS;
+    while (kv_heads < a.hkv && (uint64_t)windows * 2 * ((a.hkv + 2 * kv_heads - 1) / (2 * kv_heads)) >= kWriteWgs) kv_heads *= 2;
+    const uint32_t kv_parts = (a.hkv + kv_heads - 1) / kv_heads, kv_wgs = windows * 2 * kv_parts;
+    const bool many = (uint64_t)a.num_tokens * a.hq >= 1u << 16;
+    const uint32_t q_heads = (many ? 4 : 1) * 64 / (D / 16), q_parts = (a.hq + q_heads - 1) / q_heads;
+    const uint32_t q_wgs = (uint32_t)(((uint64_t)a.num_tokens * q_parts + 3) / 4);
+    if (many)
+        hipLaunchKernelGGL((paged_prologue_fp8_kernel<D, 4>), dim3(kv_wgs + q_wgs), dim3(256), 0, st, a, kv_wgs, kv_parts,
+                           kv_heads, q_parts);
+    else
+        hipLaunchKernelGGL((paged_prologue_fp8_kernel<D, 1>), dim3(kv_wgs + q_wgs), dim3(256), 0, st, a, kv_wgs, kv_parts,
+                           kv_heads, q_parts);
     return hipGetLastError();
 }
 
