@@ -638,6 +638,16 @@ __device__ __forceinline__ void finish(const PagedAttnArgs& a, const ItemView& v
 // its loads in flight.
 __device__ __forceinline__ void lds_ops_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// This lane, for a form of the kernel.  8 bits: hidden from the compiler, which else
+// computes every form's lane constants once ahead of all and keeps them in scratch
+// memory (an item's start then took 6000 cycles, 2000 without).
+template <int BITS>
+__device__ __forceinline__ int lane_of() {
+    int lane = threadIdx.x & 63;
+    if constexpr (BITS == 8) asm volatile("" : "+v"(lane));
+    return lane;
+}
+
 // A wave's rows of an 8-bit tile on their way from the cache to LDS: consecutive
 // bytes of it, BYTES per lane, with the scale of the block that they lie in.
 template <int BYTES>
@@ -679,7 +689,7 @@ __device__ __forceinline__ void run_shared(const PagedAttnArgs& a, const ItemVie
     using P = PaShape<D>;
     constexpr int KS = kPaWaves / RB, TILES = RB == 8 ? 1 : 2, NB = 2 * TILES / KS;
     constexpr int ROWS = 64 * TILES / kPaWaves, LOADS = ROWS / P::RI;  // per wave, step and tensor
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = lane_of<BITS>(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ql = lane & 31, kg = lane >> 5, rb = wave % RB, stream = wave / RB;
     const uint32_t per_shift = 6 - v.src.entry_shift, chunk = kTabEntries >> per_shift;
 
@@ -766,23 +776,6 @@ __device__ __forceinline__ void run_shared(const PagedAttnArgs& a, const ItemVie
         // rows of V past the last key seen.  The wait is explicit: the compiler's
         // tracking of loads that write LDS is not relied on.
         auto land = [&](uint32_t t, uint16_t* buf) __attribute__((always_inline)) {
-            if constexpr (BITS == 8) {
-                if (t + fill_tile < c1) {
-                    uint16_t* const to = buf + P::TILE * fill_tile;
-                    const uint32_t left = v.src.key_end - min(v.src.key_end, v.src.key0(t + fill_tile) + fill_row);
-#pragma unroll
-                    for (int i = 0; i < k_codes.CHUNKS; ++i) {
-                        const int r = k_codes.template row<D>(i, lane), c = k_codes.template chunk<D>(i, lane);
-                        const int tr = fill_row + r;
-                        *reinterpret_cast<uint4*>(to + D * tr + 8 * (c ^ pk_swz<D>(tr))) = k_codes.values(i);
-                        uint4 x = v_codes.values(i);
-                        if ((uint32_t)r >= left) x = make_uint4(0, 0, 0, 0);
-                        *reinterpret_cast<uint4*>(to + D * (64 + tr) + 8 * (c ^ pv_swz<D>(tr))) = x;
-                    }
-                }
-                __syncthreads();
-                return;
-            }
             __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
             const uint32_t k0 = v.src.key0(t + fill_tile) + fill_row;
             if (t + fill_tile < c1 && k0 + ROWS > v.src.key_end) {
@@ -794,6 +787,22 @@ __device__ __forceinline__ void run_shared(const PagedAttnArgs& a, const ItemVie
             }
             __syncthreads();
         };
+        // 8 bits: the codes that this wave holds of the step from tile t on, as bf16
+        // into buf, zeros over its rows of V past the last key seen.
+        [[maybe_unused]] auto expand = [&](uint32_t t, uint16_t* buf) __attribute__((always_inline)) {
+            if (TILES > 1 && t + fill_tile >= c1) return;
+            uint16_t* const to = buf + P::TILE * fill_tile;
+            const uint32_t left = v.src.key_end - min(v.src.key_end, v.src.key0(t + fill_tile) + fill_row);
+#pragma unroll
+            for (int i = 0; i < k_codes.CHUNKS; ++i) {
+                const int r = k_codes.template row<D>(i, lane), c = k_codes.template chunk<D>(i, lane);
+                const int tr = fill_row + r;
+                *reinterpret_cast<uint4*>(to + D * tr + 8 * (c ^ pk_swz<D>(tr))) = k_codes.values(i);
+                uint4 x = v_codes.values(i);
+                if ((uint32_t)r >= left) x = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(to + D * (64 + tr) + 8 * (c ^ pv_swz<D>(tr))) = x;
+            }
+        };
         lds_ops_barrier();  // the table's and the tiles' last readers are done
         fill(c0, base_in(a, v, own_key, own_page), s_a);
 #pragma unroll
@@ -803,21 +812,42 @@ __device__ __forceinline__ void run_shared(const PagedAttnArgs& a, const ItemVie
         }
         lds_ops_barrier();
         uint2 bases = bases_of(c0 + TILES);
-        land(c0, s_a);
+        if constexpr (BITS == 16) {
+            land(c0, s_a);
+        } else {
+            expand(c0, s_a);
+            if (c0 + TILES < c1) {
+                fill(c0 + TILES, bases, s_b);
+                bases = bases_of(c0 + 2 * TILES);
+            }
+            lds_ops_barrier();
+        }
         // The step from tile t out of `cur` while the next streams into `nxt`,
         // whose last readers passed the previous barrier.
         constexpr int KEYS = 32 * NB;
         const int my_tile = KEYS * stream / 64, my_row = KEYS * stream % 64;
         auto step = [&](uint32_t t, const uint16_t* cur, uint16_t* nxt) __attribute__((always_inline)) {
-            if (t + TILES < c1) {
-                fill(t + TILES, bases, nxt);
-                bases = bases_of(t + 2 * TILES);
+            if constexpr (BITS == 16) {
+                if (t + TILES < c1) {
+                    fill(t + TILES, bases, nxt);
+                    bases = bases_of(t + 2 * TILES);
+                }
+            } else if (t + TILES < c1) {
+                // (Loaded a step ago, so that nothing waits for it here.)
+                expand(t + TILES, nxt);
+                if (t + 2 * TILES < c1) {
+                    fill(t + 2 * TILES, bases, nxt);
+                    bases = bases_of(t + 3 * TILES);
+                }
             }
             const uint32_t k0 = v.src.key0(t + my_tile) + my_row;
             const uint16_t* const kb = cur + P::TILE * my_tile + D * my_row;
             if (live && (TILES == 1 || t + my_tile < c1) && !rv.none(k0, k0 + KEYS - 1))
                 tile<D, NB>(s, kb, kb + 64 * D, k_off, v_off, qf, rv, k0, v.src.key_end, scale_log2, lane, bad);
-            land(t + TILES, nxt);
+            if constexpr (BITS == 16)
+                land(t + TILES, nxt);
+            else
+                lds_ops_barrier();
         };
         for (uint32_t t = c0; t < c1; t += 2 * TILES) {
             step(t, s_a, s_b);
@@ -1333,7 +1363,7 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
     constexpr int NF = P::NF, NT = 2;                        // non-temporal: the keys are read once
     constexpr uint32_t SPT = BITS == 16 ? 2 : 1;             // steps per tile
     constexpr int RI = BITS == 16 ? P::RI : 1024 / D;        // rows per load
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = lane_of<BITS>(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ql = lane & (ROWS - 1), kg = lane / ROWS;
     const uint32_t per_shift = 6 - v.src.entry_shift, half = BITS == 16 ? wave & 1 : 0;
     uint16_t* const sk = s_a + (wave % kStreams) * 32 * D;
