@@ -440,4 +440,59 @@ inline void paged_attention_bf16(const bf16* q, const bf16* k_cache, const bf16*
                    "paged_attention_bf16");
 }
 
+// ----------------------------------------- many requests: paged cache in 8 bits
+
+// Bytes of a page, and the least page_stride (in bytes) of the calls below.
+inline size_t paged_fp8_page_bytes(uint32_t page_size, uint32_t num_kv_heads, uint32_t head_dim) {
+    return toyinfer_paged_fp8_page_bytes(page_size, num_kv_heads, head_dim);
+}
+
+// paged_qkv_prologue_bf16 into 8-bit caches.
+inline void paged_qkv_prologue_fp8(const bf16* q, const bf16* k, const bf16* v,
+                                   const bf16* q_norm_weight, const bf16* k_norm_weight,
+                                   const float* rope_cos_sin, uint32_t num_positions,
+                                   const uint32_t* positions, const uint32_t* slot_mapping,
+                                   uint32_t num_tokens, float rms_norm_eps, bf16* q_out,
+                                   uint8_t* k_cache, uint8_t* v_cache, uint32_t num_pages,
+                                   uint32_t page_size, uint64_t page_stride, uint32_t num_q_heads,
+                                   uint32_t num_kv_heads, uint32_t head_dim,
+                                   hipStream_t stream_d = nullptr) {
+    TOYINFER_CHECK(toyinfer_paged_qkv_prologue_fp8(
+                       q, k, v, q_norm_weight, k_norm_weight, rope_cos_sin, num_positions,
+                       positions, slot_mapping, num_tokens, rms_norm_eps, q_out, k_cache, v_cache,
+                       num_pages, page_size, page_stride, num_q_heads, num_kv_heads, head_dim,
+                       stream_d),
+                   "paged_qkv_prologue_fp8");
+}
+
+// The requests' last tokens out of 8-bit caches, as bf16.
+inline void paged_kv_read_fp8(const uint8_t* k_cache, const uint8_t* v_cache,
+                              const uint32_t* block_tables, const uint32_t* query_start,
+                              const uint32_t* seq_lens, uint32_t batch, uint32_t num_tokens,
+                              bf16* k_out, bf16* v_out, uint32_t num_pages, uint32_t page_size,
+                              uint64_t page_stride, uint32_t max_blocks, uint32_t num_kv_heads,
+                              uint32_t head_dim, hipStream_t stream_d = nullptr) {
+    TOYINFER_CHECK(toyinfer_paged_kv_read_fp8(k_cache, v_cache, block_tables, query_start, seq_lens,
+                                              batch, num_tokens, k_out, v_out, num_pages, page_size,
+                                              page_stride, max_blocks, num_kv_heads, head_dim,
+                                              stream_d),
+                   "paged_kv_read_fp8");
+}
+
+// paged_attention_bf16 over 8-bit caches; plan and workspace are the same.
+inline void paged_attention_fp8(const bf16* q, const uint8_t* k_cache, const uint8_t* v_cache,
+                                bf16* o, const uint32_t* block_tables, const void* plan,
+                                size_t plan_bytes, uint32_t batch, uint32_t num_tokens,
+                                uint32_t num_pages, uint32_t page_size, uint64_t page_stride,
+                                uint32_t max_blocks, uint32_t window, uint32_t sinks,
+                                uint32_t num_q_heads, uint32_t num_kv_heads, uint32_t heads_dim,
+                                void* workspace, size_t workspace_bytes,
+                                hipStream_t stream_d = nullptr) {
+    TOYINFER_CHECK(toyinfer_paged_attention_fp8(
+                       q, k_cache, v_cache, o, block_tables, plan, plan_bytes, batch, num_tokens,
+                       num_pages, page_size, page_stride, max_blocks, window, sinks, num_q_heads,
+                       num_kv_heads, heads_dim, workspace, workspace_bytes, stream_d),
+                   "paged_attention_fp8");
+}
+
 }  // namespace toyinfer

@@ -645,3 +645,279 @@ def test_pages_past_4_gib(dev):
                                  pages, ps, page, 5, 0, 0, hq, hkv, d, ws)
         H.sync()
         check_rows(o, qn[new - n:], rows_k, rows_v, 0, 0, "past 4 GiB")
+
+
+# ------------------------------------------------------- operators together
+
+class Server8:
+    """A tiny serving loop over the tables, the plan and the 8-bit operators:
+    requests with prompts of their own, taken in chunks, then decoded; random q, k,
+    v per step.  V's bytes are the oracle's after every step; what the caches hold
+    is read back, and the attention checked over that."""
+
+    def __init__(self, dev, prompts, hq, hkv, d, ps, window, sinks, rows, seed):
+        self.dev, self.hq, self.hkv, self.d, self.ps = dev, hq, hkv, d, ps
+        self.window, self.sinks, self.rows = window, sinks, rows
+        self.batch, self.blocks, self.pages = len(prompts), 48, 160
+        self.left, self.lens = list(prompts), [0] * len(prompts)
+        g = torch.Generator().manual_seed(seed)
+        self.bf = lambda *shape, std=1.0: (torch.randn(shape, generator=g) * std).to(torch.bfloat16).to(dev)
+        self.v_now = F8.Cache(self.pages, ps, hkv, d)
+        self.kc, self.vc = (torch.from_numpy(self.v_now.raw.copy()).to(dev) for _ in range(2))
+        self.qw, self.kw = self.bf(d), self.bf(d)
+        ang = torch.rand(700, d // 2, generator=g) * 6.28
+        self.rope = torch.stack([ang.cos(), ang.sin()], -1).float().to(dev)
+        order = np.random.default_rng(seed).permutation(self.pages)
+        self.free_d, self.num_free = ints(order, dev), ints([self.pages], dev)
+        self.table = ints(np.zeros((self.batch, self.blocks)), dev)
+        self.ctx, self.new = ints([0] * self.batch, dev), ints([0] * self.batch, dev)
+        self.query_start, self.all_start = (ints([0] * (self.batch + 1), dev) for _ in range(2))
+        self.seq_lens = ints([0] * self.batch, dev)
+        self.positions, self.slots = ints([0] * rows, dev), ints([0] * rows, dev)
+        self.status = ints([0, 0], dev)
+        self.q, self.k, self.v = self.bf(rows, hq, d), self.bf(rows, hkv, d), self.bf(rows, hkv, d)
+        self.q_out, self.o = torch.empty_like(self.q), torch.empty_like(self.q)
+        self.back = sum(prompts) + 20 * self.batch
+        self.k_out, self.v_out = (torch.empty(self.back, hkv, d, dtype=torch.bfloat16, device=dev) for _ in range(2))
+        self.plan = attn.paged_attention_plan_buffer(self.batch, rows, hq, hkv, d, dev)
+        self.ws = attn.paged_attention_workspace(hq, hkv, d, dev)
+        self.keys = [torch.zeros(0, hkv, d, dtype=torch.float64) for _ in prompts]
+
+    def launch(self, stream=None):
+        """The whole step, and whole contexts read back: nothing of it depends on a
+        length on the host."""
+        attn.paged_tables_u32(self.ctx, self.new, self.batch, self.free_d, self.pages,
+                              self.num_free, self.ps, self.table, self.blocks, self.rows,
+                              self.query_start, self.seq_lens, self.positions, self.slots,
+                              self.status, stream)
+        attn.paged_attention_plan(self.query_start, self.seq_lens, self.batch, self.rows, self.ps,
+                                  self.blocks, self.window, self.sinks, self.hq, self.hkv, self.d,
+                                  self.plan, stream)
+        attn.paged_qkv_prologue_fp8(self.q, self.k, self.v, self.qw, self.kw, self.rope, 700,
+                                    self.positions, self.slots, self.rows, 1e-6, self.q_out,
+                                    self.kc, self.vc, self.pages, self.ps, self.kc.stride(0),
+                                    self.hq, self.hkv, self.d, stream)
+        attn.paged_attention_fp8(self.q_out, self.kc, self.vc, self.o, self.table, self.plan,
+                                 self.batch, self.rows, self.pages, self.ps, self.kc.stride(0),
+                                 self.blocks, self.window, self.sinks, self.hq, self.hkv, self.d,
+                                 self.ws, stream)
+        attn.paged_kv_read_fp8(self.kc, self.vc, self.table, self.all_start, self.seq_lens,
+                               self.batch, self.back, self.k_out, self.v_out, self.pages, self.ps,
+                               self.kc.stride(0), self.blocks, self.hkv, self.d, stream)
+
+    def step(self, chunk, launch):
+        new = [min(chunk, x) if x else 1 for x in self.left]
+        self.left = [x - n if x else 0 for x, n in zip(self.left, new)]
+        self.ctx.copy_(ints(self.lens, self.dev))
+        self.new.copy_(ints(new, self.dev))
+        ends = [x + n for x, n in zip(self.lens, new)]
+        self.all_start.copy_(ints(np.concatenate([[0], np.cumsum(ends)]), self.dev))
+        std = float(2.0 ** np.random.default_rng(sum(ends)).integers(-3, 4))  # blocks grow now and then
+        for t in (self.q, self.k, self.v):
+            t.copy_(self.bf(*t.shape, std=std))
+        for t in (self.o, self.k_out, self.v_out):
+            t.fill_(3.0)
+        H.sync()
+        launch()
+        H.sync()
+        left, refused = host(self.status)
+        assert refused == 0
+        self.num_free.copy_(ints([left], self.dev))
+        slots = np.array(host(self.slots), np.int64)
+        self.v_now.write(slots, self.v.cpu().double().numpy())
+        assert (self.vc.cpu().numpy() == self.v_now.raw).all()
+        at = base = 0
+        for b, n in enumerate(new):
+            rows, before = slice(at, at + n), self.lens[b]
+            self.lens[b] += n
+            length, at = self.lens[b], at + n
+            cs = self.rope[before:length].double().cpu().numpy()
+            k = PO.rms_rope(self.k[rows].double().cpu().numpy(), self.kw.double().cpu().numpy(), cs, 1e-6)
+            self.keys[b] = torch.cat([self.keys[b], torch.from_numpy(k)])
+            got_k, got_v = (x[base:base + length] for x in (self.k_out, self.v_out))
+            base += length
+            # A block's scale may be set by its largest value, of any row and head dim:
+            # a code is off by at most 2^-4 of the value or 2^-9 (with rows rounded again
+            # below 2^-9 of all scales before it) of the largest / 224.
+            most = torch.cat([self.keys[b].abs(), torch.zeros(-length % 16, self.hkv, self.d)]).view(
+                -1, 16, self.hkv, self.d).amax((1, 3)).repeat_interleave(16, 0)[:length, :, None]
+            off = 2.0 ** -4 * self.keys[b].abs() * 1.01 + 2.0 ** -8 * most / 224
+            assert ((got_k.cpu().double() - self.keys[b]).abs() <= off).all(), b
+            check_rows(self.o[rows], self.q_out[rows], got_k, got_v, self.window, self.sinks, b)
+        assert (self.o[at:] == 3.0).all()
+        assert (self.k_out[base:] == 3.0).all() and (self.v_out[base:] == 3.0).all()
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (90, 4)])
+@pytest.mark.parametrize("hq,hkv,d", [(16, 8, 128), (6, 2, 64)])
+def test_serving_steps(dev, hq, hkv, d, window, sinks):
+    print(f"[fp8] serving {hq}/{hkv} D={d} window {window}", flush=True)
+    s = Server8(dev, [130, 1, 300, 17, 64], hq, hkv, d, 16, window, sinks, 270, seed=hq + window)
+    for _ in range(8):
+        s.step(64, s.launch)
+
+
+def test_serving_steps_captured(dev):
+    """The same as one captured graph, replayed step after step with eager work
+    between the replays."""
+    s = Server8(dev, [100, 33, 200], 16, 8, 128, 32, 0, 0, 140, seed=5)
+    s.step(40, s.launch)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=stream):
+        s.launch(stream)
+    other = Step8(dev, [(700, 1), (90, 33)], 8, 2, 128, 16, seed=1)
+    for _ in range(6):
+        s.step(40, graph.replay)
+        other.run()
+    s.step(40, s.launch)
+
+
+def test_caches_of_both_kinds_share_plan_and_workspace(dev):
+    """Layers with a bf16 cache and layers with an 8-bit one in one step: one plan,
+    one workspace, in turn."""
+    requests = [(3000, 1), (500, 120), (60, 3), (900, 20)]
+    wide, narrow = Step(dev, requests, 16, 8, 128, 16, seed=3), Step8(dev, requests, 16, 8, 128, 16, seed=3)
+    narrow.plan, narrow.ws = wide.plan, wide.ws
+    wide.make_plan()
+    for _ in range(3):
+        for st in (wide, narrow):
+            st.o.fill_(3.0)
+            st.attend()
+    H.sync()
+    wide.check()
+    narrow.check()
+    assert not wide.ws[:4 * (8 + 2)].any()
+
+
+def test_graphs_that_share_a_workspace(dev):
+    one = Step8(dev, [(700, 1), (300, 40), (900, 1)], 8, 2, 128, 16, seed=21)
+    two = Step8(dev, [(3000, 1), (64, 64), (100, 5)], 8, 2, 128, 16, 70, 4, seed=22)
+    two.ws = one.ws
+    stream, graphs = torch.cuda.Stream(), []
+    for st in (one, two):
+        st.run()
+        graph = torch.cuda.CUDAGraph()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(graph, stream=stream):
+            st.make_plan(stream)
+            st.attend(stream)
+        graphs.append(graph)
+    for _ in range(3):
+        for st, graph in zip((one, two), graphs):
+            st.o.fill_(3.0)
+            graph.replay()
+        H.sync()
+        one.check()
+        two.check()
+        one.attend()
+        two.attend()
+        H.sync()
+        one.check()
+        two.check()
+
+
+def test_one_plan_on_two_streams(dev):
+    st = Step8(dev, [(3000, 1), (500, 120), (60, 3)], 16, 8, 64, 16, seed=23)
+    st.run()
+    ws = attn.paged_attention_workspace(st.hq, st.hkv, st.d, dev)
+    mine, other, first = st.o, torch.full_like(st.o, 3.0), st.o.clone()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    mine.fill_(3.0)
+    H.sync()
+    for _ in range(5):
+        for stream, o, w in zip(streams, (mine, other), (st.ws, ws)):
+            st.o, st.ws, keep = o, w, st.ws
+            st.attend(stream)
+            st.ws = keep
+    H.sync()
+    assert torch.equal(mine, first) and torch.equal(other, first)
+
+
+@pytest.mark.parametrize("hq,hkv,d,requests", [
+    (20, 1, 128, [(700, 1), (300, 1), (64, 1), (65, 1)]),        # 20 rows
+    (32, 1, 64, [(9000, 1), (31, 1)]),                           # 32
+    (6, 2, 128, [(700, 7), (5000, 10), (100, 5), (64, 6)]),      # 21, 30, 15, 18
+    (17, 17, 64, [(900, 17), (500, 16), (700, 1), (300, 32)]),
+    (4, 1, 128, [(700, 4), (300, 5), (1, 1), (2, 2), (65, 3)]),  # 16 and 20 rows
+])
+@pytest.mark.parametrize("window", [0, 130])
+def test_streams_of_each_width(dev, hq, hkv, d, requests, window):
+    """Streams of up to 16 rows and of 17 to 32, one after the other in a lane's
+    list."""
+    Step8(dev, requests, hq, hkv, d, 16, window, 3 if window else 0, seed=hq).run()
+
+
+def test_decoded_tokens_keep_the_weights_precision(dev):
+    """Streams of up to 16 rows round a weight twice (a bf16 value and what it
+    leaves), so an element's RMS error is the output's own rounding: a step 2^-7 of
+    the power of two below the value, over sqrt(12), against values whose mantissas
+    spread over [1, 2): 2^-7 / sqrt(12 * 7 / 3) = 0.0015 of the RMS.  One part alone
+    would add a weight's rounding, as much again in another direction (0.0021); the
+    limit is 2^-9 = 0.00195."""
+    st = Wide8(dev, [(5000, 1), (9000, 2), (3000, 4)], 32, 8, 128, 16, seed=5)
+    st.run()
+    rms = lambda x: x.square().mean().sqrt().item()
+    for b in range(3):
+        rows = slice(int(st.start[b]), int(st.start[b + 1]))
+        k, v = (x.to(dev) for x in st.kv[b])
+        o, _ = wide_attention(st.q_d[rows], k, v, 0, 0)
+        assert rms(st.o[rows].double() - o) < 2.0 ** -9 * rms(o), b
+
+
+def test_binding_refuses_on_the_gpu(dev):
+    """Tensors of another type, size, layout or device: refused, nothing written."""
+    st = Step8(dev, [(40, 1), (90, 3)], 8, 2, 128, 16)
+    st.make_plan()
+    H.sync()
+    before = st.k.clone(), st.v.clone()
+
+    def attend(**kw):
+        a = dict(q=st.q_d, k=st.k, v=st.v, o=st.o, table=st.table, plan=st.plan, ws=st.ws)
+        a.update(kw)
+        attn.paged_attention_fp8(a["q"], a["k"], a["v"], a["o"], a["table"], a["plan"], st.batch,
+                                 st.rows, st.pages, st.ps, st.stride, st.blocks, 0, 0, st.hq,
+                                 st.hkv, st.d, a["ws"])
+
+    for kw in (dict(q=st.q_d.half()), dict(q=st.q_d[:-1]), dict(q=st.q_d.cpu()), dict(k=st.k[1:]),
+               dict(v=st.v.cpu()), dict(k=st.k.view(torch.int8)), dict(k=st.k.view(-1)),
+               dict(k=st.k.view(torch.bfloat16)), dict(o=st.o.float()),
+               dict(v=torch.cat([st.v, st.v], 1)[:, :st.v.shape[1]]), dict(table=st.table.long()),
+               dict(table=st.table[:1]), dict(plan=st.plan[:-256]), dict(ws=st.ws[:-16]), dict(o=st.q_d)):
+        with pytest.raises(attn.ToyInferError):
+            attend(**kw)
+
+    rows, new = st.rows, st.q_d[:, :2].contiguous()
+    w, rope = torch.ones(128, dtype=torch.bfloat16, device=dev), torch.zeros(99, 64, 2, device=dev)
+    index = torch.zeros(rows, dtype=torch.int32, device=dev)
+
+    def write(**kw):
+        a = dict(q=st.q_d, k=new, v=new, w=w, rope=rope, pos=index, slots=index, out=st.q_d, kc=st.k, vc=st.v)
+        a.update(kw)
+        attn.paged_qkv_prologue_fp8(a["q"], a["k"], a["v"], a["w"], a["w"], a["rope"], 99, a["pos"],
+                                    a["slots"], rows, 1e-6, a["out"], a["kc"], a["vc"], st.pages,
+                                    st.ps, st.stride, 8, 2, 128)
+
+    for kw in (dict(k=new[1:]), dict(v=new.float()), dict(w=w[1:]), dict(rope=rope[1:]), dict(pos=index.long()),
+               dict(slots=index[:1]), dict(kc=st.k[:, 16:]), dict(vc=st.k), dict(out=new), dict(kc=st.k.cpu())):
+        with pytest.raises(attn.ToyInferError):
+            write(**kw)
+
+    outs = [torch.full((43, 2, 128), 3.0, dtype=torch.bfloat16, device=dev) for _ in range(2)]
+
+    def read(**kw):
+        a = dict(k=st.k, v=st.v, table=st.table, start=st.query_start, lens=st.seq_lens, ko=outs[0], vo=outs[1])
+        a.update(kw)
+        attn.paged_kv_read_fp8(a["k"], a["v"], a["table"], a["start"], a["lens"], 2, 43, a["ko"], a["vo"],
+                               st.pages, st.ps, st.stride, st.blocks, 2, 128)
+
+    for kw in (dict(k=st.k[1:]), dict(table=st.table[:1]), dict(start=st.query_start[:2]), dict(lens=st.seq_lens.long()),
+               dict(ko=outs[0][1:]), dict(vo=outs[0]), dict(ko=outs[0].half()), dict(v=st.v.cpu())):
+        with pytest.raises(attn.ToyInferError):
+            read(**kw)
+    H.sync()
+    assert (st.o == 3.0).all() and all((x == 3.0).all() for x in outs)
+    assert torch.equal(st.k, before[0]) and torch.equal(st.v, before[1])
+    attend()
+    H.sync()
+    st.check()

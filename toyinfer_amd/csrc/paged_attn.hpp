@@ -239,22 +239,32 @@ __device__ __forceinline__ void clear(NarrowState<D>& s) {
 }
 __device__ __forceinline__ float quarters_sum(float x) { return xor32_sum(xor16_sum(x)); }
 
+// The probabilities come in two bf16 parts, pf[2 + t] what rounding leaves of pf[t]:
+// these streams wait for memory, not for products, and one part alone is what the
+// output is off by beside its own rounding (0.0023 of its RMS against 64 bits, with
+// both 0.0017).
 template <int D>
-__device__ __forceinline__ void probabilities(f32x4_t (&st)[4], NarrowState<D>& s, bf16x8_t (&pf)[2], float scale_log2) {
+__device__ __forceinline__ void probabilities(f32x4_t (&st)[4], NarrowState<D>& s, bf16x8_t (&pf)[4], float scale_log2) {
     auto probs = [&](float mref) __attribute__((always_inline)) {
-        float sum = 0.0f;
+        float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             float e[8];
+            uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 8; ++j) {
                 e[j] = __builtin_amdgcn_exp2f(fmaf(st[2 * t + j / 4][j % 4], scale_log2, -mref));
-            const uint4 w = make_uint4(pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3]), pack_bf16x2(e[4], e[5]),
-                                       pack_bf16x2(e[6], e[7]));
-            pf[t] = as_bf16x8(w);
-            sum = sum_bf16x8(w, sum);
+                sum[j & 1] += e[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                hi[j] = pack_bf16x2(e[2 * j], e[2 * j + 1]);
+                lo[j] = pack_bf16x2(e[2 * j] - bf16_lo(hi[j]), e[2 * j + 1] - bf16_hi(hi[j]));
+            }
+            pf[t] = as_bf16x8(make_uint4(hi[0], hi[1], hi[2], hi[3]));
+            pf[2 + t] = as_bf16x8(make_uint4(lo[0], lo[1], lo[2], lo[3]));
         }
-        return sum;
+        return sum[0] + sum[1];
     };
     float ts = probs(s.m);
     const float mass = quarters_sum(s.l + ts);
@@ -677,6 +687,15 @@ struct CodeRows {
     static __device__ __forceinline__ int row(int i, int lane) { return byte(i, lane) / D; }
     template <int D>
     static __device__ __forceinline__ int chunk(int i, int lane) { return byte(i, lane) % D / 8; }
+    // Zeros from row `left` on.  (With none left, the scale may be anything.)
+    template <int D>
+    __device__ __forceinline__ void cut(uint32_t left, int lane) {
+        asm volatile("; rows past the last key");  // keeps the branch around this
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i)
+            if ((uint32_t)row<D>(i, lane) >= left) codes[i] = make_uint2(0, 0);
+        if (!left) scale = 1.0f;
+    }
     __device__ __forceinline__ uint4 values(int i) const { return fp8x8_to_bf16(codes[i], scale); }
 };
 
@@ -704,7 +723,7 @@ __device__ __forceinline__ void run_shared(const PagedAttnArgs& a, const ItemVie
     [[maybe_unused]] uint32_t voff[8 / P::RI];
 #pragma unroll
     for (int j = 0; j < 8 / P::RI; ++j) voff[j] = (P::RI * j + lr) * v.src.row_bytes + 16 * (phys ^ pv_swz<D>(lr));
-    [[maybe_unused]] CodeRows<ROWS * D / 64> k_codes, v_codes;
+    [[maybe_unused]] CodeRows<ROWS * D / 64> k_codes{}, v_codes{};
     int k_off[P::KSTEPS], v_off[P::DBLK];
 #pragma unroll
     for (int ks = 0; ks < P::KSTEPS; ++ks) k_off[ks] = ql * D + 8 * ((2 * ks + kg) ^ pk_swz<D>(ql));
@@ -790,17 +809,14 @@ __device__ __forceinline__ void run_shared(const PagedAttnArgs& a, const ItemVie
         // 8 bits: the codes that this wave holds of the step from tile t on, as bf16
         // into buf, zeros over its rows of V past the last key seen.
         [[maybe_unused]] auto expand = [&](uint32_t t, uint16_t* buf) __attribute__((always_inline)) {
-            if (TILES > 1 && t + fill_tile >= c1) return;
             uint16_t* const to = buf + P::TILE * fill_tile;
             const uint32_t left = v.src.key_end - min(v.src.key_end, v.src.key0(t + fill_tile) + fill_row);
+            if (left < ROWS) v_codes.template cut<D>(left, lane);
 #pragma unroll
             for (int i = 0; i < k_codes.CHUNKS; ++i) {
-                const int r = k_codes.template row<D>(i, lane), c = k_codes.template chunk<D>(i, lane);
-                const int tr = fill_row + r;
-                *reinterpret_cast<uint4*>(to + D * tr + 8 * (c ^ pk_swz<D>(tr))) = k_codes.values(i);
-                uint4 x = v_codes.values(i);
-                if ((uint32_t)r >= left) x = make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4*>(to + D * (64 + tr) + 8 * (c ^ pv_swz<D>(tr))) = x;
+                const int r = fill_row + k_codes.template row<D>(i, lane), c = k_codes.template chunk<D>(i, lane);
+                *reinterpret_cast<uint4*>(to + D * r + 8 * (c ^ pk_swz<D>(r))) = k_codes.values(i);
+                *reinterpret_cast<uint4*>(to + D * (64 + r) + 8 * (c ^ pv_swz<D>(r))) = v_codes.values(i);
             }
         };
         lds_ops_barrier();  // the table's and the tiles' last readers are done
@@ -832,8 +848,9 @@ __device__ __forceinline__ void run_shared(const PagedAttnArgs& a, const ItemVie
                     fill(t + TILES, bases, nxt);
                     bases = bases_of(t + 2 * TILES);
                 }
-            } else if (t + TILES < c1) {
-                // (Loaded a step ago, so that nothing waits for it here.)
+            } else if (RB < 8 || t + TILES < c1) {
+                // (Loaded a step ago, so that nothing waits for it here.  Behind the last
+                // step there are no codes, and nobody reads what is made of them.)
                 expand(t + TILES, nxt);
                 if (t + 2 * TILES < c1) {
                     fill(t + 2 * TILES, bases, nxt);
@@ -1690,7 +1707,7 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
                     }
                 const uint32_t k1 = k0 + 63;
                 const bool hidden = rv.some_hidden(k0, k1);
-                bf16x8_t pf[NARROW ? 2 : 4];
+                bf16x8_t pf[4];
                 if constexpr (NARROW) {
                     if (hidden) hide(st, rv, k0, kg);
                     probabilities<D>(st, s, pf, scale_log2);
@@ -1725,15 +1742,21 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
 #pragma unroll
                 for (int i = 0; i < 4; ++i) value_scale[i] = __uint_as_float(__builtin_amdgcn_readlane(vs, 16 * i));
 #pragma unroll
-                for (int t = 0; t < VT; ++t)
+                for (int t = 0; t < VT; ++t) {
+                    bf16x8_t w[DB];
 #pragma unroll
                     for (int db = 0; db < DB; ++db) {
                         const uint2 x = va[t][db];
                         const float lo = value_scale[NARROW ? 2 * t : t], hi = value_scale[NARROW ? 2 * t + 1 : t];
-                        const uint4 w = make_uint4(fp8x2_to_bf16<false>(x.x, lo), fp8x2_to_bf16<true>(x.x, lo),
-                                                   fp8x2_to_bf16<false>(x.y, hi), fp8x2_to_bf16<true>(x.y, hi));
-                        s.o[db] = products(as_bf16x8(w), pf[t], s.o[db]);
+                        w[db] = as_bf16x8(make_uint4(fp8x2_to_bf16<false>(x.x, lo), fp8x2_to_bf16<true>(x.x, lo),
+                                                     fp8x2_to_bf16<false>(x.y, hi), fp8x2_to_bf16<true>(x.y, hi)));
+                        s.o[db] = products(w[db], pf[t], s.o[db]);
                     }
+                    if constexpr (NARROW) {
+#pragma unroll
+                        for (int db = 0; db < DB; ++db) s.o[db] = products(w[db], pf[2 + t], s.o[db]);
+                    }
+                }
             }
         }
         if (closes) {
