@@ -195,6 +195,20 @@ def test_write_many_tokens(dev):
     w.write((pages[at // 64] * 64 + at % 64).astype(np.uint32))
 
 
+def test_write_rounds_exact_keys(dev):
+    """Keys get the codes that their values in 64 bits round to: the kernel's are
+    within 2^-48 of those, where one in 2^43 lies that close to a border."""
+    w = Writer(dev, 40, 64, 4, 4, 128, seed=11)
+    slots, pos = np.arange(2500) + 16, np.arange(2500) % POSITIONS
+    q, k, v = (w.rows(2500, std) for std in (2.0, 3.0, 1.0))
+    w.launch(q.to(dev), k.to(dev), v.to(dev), ints(pos, dev), ints(slots, dev), q.to(dev))
+    H.sync()
+    x = PO.rms_rope(k.double().numpy(), w.kw.double().numpy(), w.rope.double().numpy()[pos],
+                    float(np.float32(1e-6)))
+    w.k.write(slots, x)
+    assert (w.k_d.cpu().numpy() == w.k.raw).all()
+
+
 def test_write_in_place_and_again(dev):
     """q_out may be q, and a call gives the same bytes every time."""
     w = Writer(dev, 9, 16, 4, 2, 128)
