@@ -42,6 +42,29 @@
 // exponentials, took 577 us with one barrier per tile and 601 with two.
 // Starting an item costs 5 us of a lane (the item, its table and queries, and
 // the first keys, each waiting for the one before), ending it 1.5 to 2.5.
+//
+// 8 bits.  code * 2^e is exact in bf16 (fp8.hpp), so the same products run on codes
+// expanded to bf16 by one instruction a pair, and nothing but the weights is rounded.
+// A block of 16 tokens has one scale, so a lane has one of K, that of its key, and
+// one or two of V.
+//   Up to 32 rows: a stream's step is a tile of 64 keys, whose codes are as many
+//   bytes as 32 keys of bf16, with as many in flight.  Codes reach LDS as they are
+//   and the operands' registers by 16-byte reads (K) and transposing reads of bytes
+//   (V), and are expanded there, once.  A key's operand there may hold dims, and V's
+//   keys, in any order that Q's or the weights' registers share.
+//   More rows: every wave would expand the same tile, so its rows go through the
+//   registers of the wave that loads them and are bf16 in LDS, where the 16-bit
+//   forms go on with them.  A step's codes are loaded two steps ahead and expanded
+//   one ahead, at its start (under the products of K it was 3 to 5 % slower, under
+//   those of V 3 % faster at head_dim 128 and 4 % slower at 64).  Writing them has
+//   two lanes to a bank half the time; loads in halves avoid that and are more, and
+//   were 2 % slower.
+// Measured, at 32 query and 8 KV heads of 128:
+//   streaming, 48 requests of up to 8192 keys (472 MB): 86 us and 5 for the merge;
+//     16 of 32768 118 us, 5.9 TB/s.  Loads alone, without products, waits or scales, are no
+//     faster: 6.5 TB/s in a loop without ends of items;
+//   a prompt of 8192: 525 to 540 us where bf16 takes 517 to 533, 1.02 PFLOP/s; 512
+//     tokens on 7680 keys 82 to 93 (90).
 #pragma once
 
 #include <math.h>
@@ -1270,7 +1293,11 @@ __device__ __forceinline__ f32x16_t products(bf16x8_t a, bf16x8_t b, f32x16_t c)
 __device__ __forceinline__ f32x4_t products(bf16x8_t a, bf16x8_t b, f32x4_t c) { return mfma16x16x32(a, b, c); }
 
 enum : uint32_t { kSegNone = 0, kSegStream = 1, kSegShared = 2, kSegNarrow = 3 };
-// A streamed segment's kind: up to 16 rows in 8 bits have a form of their own.
+// A streamed segment's kind: up to 16 rows in 8 bits have a form of their own, whose
+// smaller products leave registers for the weights in two parts (an element is off
+// by 0.0017 of the outputs' RMS, as a bf16 of the exact value is, in the form for 32
+// rows by 0.0023).  Otherwise the two take the same time: 48 decoded tokens of 32 and
+// 8 heads of 128 91.5 and 91.8 us, 64 of heads of 64 65.0 and 66.2.
 template <int BITS>
 __device__ __forceinline__ uint32_t stream_kind(uint32_t rows) {
     return BITS == 8 && rows <= 16 ? kSegNarrow : kSegStream;
@@ -1362,9 +1389,10 @@ __device__ __forceinline__ void advance(const PagedAttnArgs& a, ItemView& v, con
 }
 
 // Up to 32 rows: wave w < kStreams streams the steps w, w + kStreams, ... of a
-// segment, 32-key halves of its tiles (16 bits) or whole tiles (8 bits), and on into the next segment, which wave kStreams
-// stages meanwhile: a wave's first loads of it go out behind its last ones of
-// this, and are in flight while the streams merge.  (Staged by all waves after
+// segment, 32-key halves of its tiles (16 bits) or whole tiles (8 bits: as many
+// bytes), and on into the next segment, which wave kStreams stages meanwhile: a
+// wave's first loads of it go out behind its last ones of this, and are in flight
+// while the streams merge.  (Staged by all waves after
 // the merge, a new item cost 20 us of its workgroup under load: its ticket, the
 // item, the table and the first keys are fetched one after the other.)
 // Runs segments from `slot` on; returns the slot of one that is not streamed.

@@ -31,7 +31,7 @@ namespace tiattn {
 namespace {
 
 constexpr int kWindow = 16;  // token rows whose runs a workgroup takes
-constexpr uint32_t kWriteWgs = 512;
+constexpr uint32_t kWriteWgs = 512;  // two per compute unit
 
 // The largest of a row's lanes' values, in each of them.
 template <int D>
@@ -93,8 +93,7 @@ __device__ __forceinline__ void norm_rope_f64(uint4 xr, uint4 xi, uint4 wr, uint
 
 // By one workgroup: heads [head0, head1) of K or V in a window's runs, PARTS heads
 // at a time, HALVES waves each, of which one has the first 64 / (D / 16) rows of a
-// group and the other the rest.  (Both in one wave took 157 registers and, at 8192
-// tokens, 4 us longer.)
+// group and the other the rest.  (Both in one wave: 4 us longer at 8192 tokens.)
 template <int D>
 struct WriteShape {
     static constexpr int LPR = D / 16, RPP = 64 / LPR, HALVES = kWindow / RPP, PARTS = 4 / HALVES;
@@ -277,13 +276,21 @@ template <int D>
 hipError_t launch_prologue_t(const PagedPrologueFp8Args& a, hipStream_t st) {
     typedef WriteShape<D> W;
     const uint32_t windows = (a.num_tokens + kWindow - 1) / kWindow;
-    // Heads that a workgroup takes one after the other, the next one's rows on their
-    // way; all at once while that leaves compute units without a workgroup.
+    // Heads of K or V that a workgroup takes one after the other, the next one's rows
+    // on their way, as many as leave kWriteWgs workgroups.  (All heads at once, by
+    // workgroups of their own: 8192 tokens of 32 and 8 heads of 128 45.4 us instead
+    // of 40.5, 8 and 8 heads 32.0 instead of 27.3, 2048 tokens 14.0 instead of 12.6.
+    // Few tokens have to be at once: then there are compute units for all.)
     uint32_t kv_heads = W::PARTS;
     while (kv_heads < a.hkv && (uint64_t)windows * 2 * ((a.hkv + 2 * kv_heads - 1) / (2 * kv_heads)) >= kWriteWgs) kv_heads *= 2;
     const uint32_t kv_parts = (a.hkv + kv_heads - 1) / kv_heads, kv_wgs = windows * 2 * kv_parts;
-    const bool many = (uint64_t)a.num_tokens * a.hq >= 1u << 16;
-    const uint32_t q_heads = (many ? 4 : 1) * 64 / (D / 16), q_parts = (a.hq + q_heads - 1) / q_heads;
+    // A token's heads of Q, 64 / (D / 16) to a wave's load: four loads under way, but
+    // for so few heads that one has them all.  (One load a wave against four: 8192
+    // tokens of 32 heads 44.7 and 40.5 us, of 16 33.9 and 31.2, of 8 26.3 and 27.3;
+    // 1371 tokens of 16 9.4 and 9.6.)
+    constexpr uint32_t per_load = 64 / (D / 16);
+    const bool many = a.hq > per_load;
+    const uint32_t q_heads = (many ? 4 : 1) * per_load, q_parts = (a.hq + q_heads - 1) / q_heads;
     const uint32_t q_wgs = (uint32_t)(((uint64_t)a.num_tokens * q_parts + 3) / 4);
     if (many)
         hipLaunchKernelGGL((paged_prologue_fp8_kernel<D, 4>), dim3(kv_wgs + q_wgs), dim3(256), 0, st, a, kv_wgs, kv_parts,
