@@ -475,7 +475,8 @@ int toyinfer_paged_attention_bf16(const void* q, const void* k_cache, const void
 /* The same cache in 8 bits.  A page is a record of bytes: its codes
  * [Hkv][page_size][D], then its scales, fp32 [Hkv][page_size/16], one for each
  * block of 16 rows and head; page_stride is in bytes, a multiple of 16 and at
- * least toyinfer_paged_fp8_page_bytes (0 for sizes that are not supported).
+ * least toyinfer_paged_fp8_page_bytes (0 for sizes that are not supported); a
+ * multiple of 128 is read faster, by a quarter with pages of 16 rows of 64.
  * page_size is a power of two in 16..65536.  Codes are e4m3 (largest 448, 0x7f
  * and 0xff NaN, no infinities), a scale is a power of two, 2^-100 .. 2^119, and a
  * value code * scale, which bf16 holds exactly.  The caches need no
