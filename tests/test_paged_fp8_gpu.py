@@ -1,10 +1,10 @@
 """The 8-bit paged cache on the GPU.
 
 V's codes and scales have to be the oracle's bit for bit: a value is bf16, its
-code the nearest.  K's scale and codes come from fp32 values that are off by at
-most 2^-16 of the rotation's products (the prologue's norm and rotation): the
-scale is the one of a largest value inside that error, a code off by half a step
-more, 2^-4 of the value or 2^-10 of the scale.  Reading back is exact.
+code the nearest.  K's are those of the normalised and rotated values: most tests
+let these be off by 2^-16 of the rotation's products, so the scale is the one of a
+largest value inside that error, a code off by half a step more, 2^-4 of the value or
+2^-10 of the scale; one asks for the codes bit for bit.  Reading back is exact.
 
 Keys and values enter the attention's products without a rounding of their own,
 so its bounds are those of the bf16 cache over the values that the codes stand
@@ -407,6 +407,16 @@ def test_attention(dev, name, hq, hkv, d):
 def test_attention_page_sizes(dev, ps, d):
     Step8(dev, [(700, 1), (130, 130), (333, 40), (64, 2), (1, 1)], 8, 2, d, ps, seed=ps,
           interleaved=True).run()
+
+
+@pytest.mark.parametrize("ps,apart", [(16, 16), (16, 96), (64, 48), (4096, 0), (16384, 112)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_strides(dev, ps, apart, d):
+    """Pages at any multiple of 16 bytes, and large ones."""
+    class Spread(Step8):
+        pass
+    Spread.apart = apart
+    Spread(dev, [(700, 1), (130, 130), (5000, 40), (64, 2), (1, 1)], 8, 2, d, ps, seed=ps).run()
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (7, 4), (64, 0), (100, 70), (300, 4),
