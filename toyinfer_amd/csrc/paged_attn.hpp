@@ -1758,8 +1758,10 @@ __device__ __forceinline__ uint32_t run_streams(const PagedAttnArgs& a, ItemView
                     __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
                     // (A block past the last key has any scale.)
                     if (k0 + (lane & ~(kFp8Block - 1)) >= v.src.key_end) vs = 0x3f800000u;
+                    // (Blocks that no row sees may hold any bytes: past the writer's largest scale
+                    // a code's bf16 may be infinite.)
                     if (rv.some_hidden(k0, min(k1, v.src.key_end - 1)) &&
-                        (__any((vs & 0x7f800000u) == 0x7f800000u) || any_nan_code<D>(codes)))
+                        (__any((vs & 0x7f800000u) > (uint32_t)(kFp8High + 127) << 23) || any_nan_code<D>(codes)))
                         s_seg[slot].spoilt = 1;
                 }
                 constexpr int VT = NARROW ? 2 : 4, DB = D / ROWS;
