@@ -57,21 +57,24 @@ __device__ __forceinline__ float sticky_f32(double x) {
     return (float)__builtin_bit_cast(double, (uint64_t)hi << 32);
 }
 
-// norm_rope_f32 with 64 bits wherever 32 do not hold a result exactly, as they hold
-// the product of two bf16 values: what it gives rounds to the code that the exact
-// value rounds to, but for values within 2^-48 of a border.  (In 32 bits throughout,
-// one of 2 million values got its neighbour's code.  8192 tokens of 32 and 8 heads
-// of 128 take 40.1 us instead of 39.0, of 8 and 8 heads 27.0 instead of 24.8.)
+// norm_rope_f32 in 64 bits: what it gives rounds to the code that the exact value
+// rounds to, but for values within 2^-48 of a border.  (In 32 bits throughout, one of
+// 2 million values got its neighbour's code.  8192 tokens of 32 and 8 heads of 128
+// took 39.0 us so, and 40.1 with all but the product below in 64 bits, of 8 and 8 heads
+// 24.8 and 27.0.)  The product of a value and its weight too: 32 bits hold it exactly in
+// their range only, which two bf16 leave at both ends where the norm's result does not.
+// (That costs 38.5 -> 39.0 us of those tokens on another card, and 28.2 -> 29.2.)
 template <int D>
 __device__ __forceinline__ void norm_rope_f64(uint4 xr, uint4 xi, uint4 wr, uint4 wi, const float4 (&rope)[4], float eps,
                                               float (&re)[8], float (&im)[8]) {
-    // (Keeps a loop's angles from being held converted.)
+    // (Keeps a loop's angles and weights, and the values over the sum, from being held converted.)
     float4 cs[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         cs[k] = rope[k];
         asm volatile("" : "+v"(cs[k].x), "+v"(cs[k].y), "+v"(cs[k].z), "+v"(cs[k].w));
     }
+    asm volatile("" : "+v"(wr.x), "+v"(wr.y), "+v"(wr.z), "+v"(wr.w), "+v"(wi.x), "+v"(wi.y), "+v"(wi.z), "+v"(wi.w));
     bf16x8_to_f32(xr, re);
     bf16x8_to_f32(xi, im);
     double ss = 0.0;
@@ -82,9 +85,12 @@ __device__ __forceinline__ void norm_rope_f64(uint4 xr, uint4 xi, uint4 wr, uint
     if constexpr (D == 128) ss += dpp_f64<kDppRowHalfMirror>(ss);
     const double inv = rsqrt(ss * (1.0 / D) + (double)eps);
 #pragma unroll
+    for (int k = 0; k < 8; ++k) asm volatile("" : "+v"(re[k]), "+v"(im[k]));
+#pragma unroll
     for (int k = 0; k < 8; ++k) {
         const uint32_t gr = word_of(wr, k / 2), gi = word_of(wi, k / 2);
-        const double r = re[k] * (k % 2 ? bf16_hi(gr) : bf16_lo(gr)), i = im[k] * (k % 2 ? bf16_hi(gi) : bf16_lo(gi));
+        const double r = (double)re[k] * (k % 2 ? bf16_hi(gr) : bf16_lo(gr));
+        const double i = (double)im[k] * (k % 2 ? bf16_hi(gi) : bf16_lo(gi));
         const double c = k % 2 ? cs[k / 2].z : cs[k / 2].x, s = k % 2 ? cs[k / 2].w : cs[k / 2].y;
         re[k] = sticky_f32((c * r - s * i) * inv);
         im[k] = sticky_f32((c * i + s * r) * inv);
