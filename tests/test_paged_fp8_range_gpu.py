@@ -16,19 +16,7 @@ pytestmark = pytest.mark.gpu
 LARGEST = float(torch.finfo(torch.bfloat16).max)
 
 
-@pytest.mark.parametrize("eps", [1e-6, 0.0])
-@pytest.mark.parametrize("size,weight", [
-    (2.0 ** 125, 2.0 ** 10),    # products past the largest fp32
-    (2.0 ** 125, 2.0 ** 115),
-    (2.0 ** 20, 2.0 ** 120),
-    (2.0 ** 125, 2.0 ** -90),
-    (2.0 ** -100, 2.0 ** -30),  # below the normal ones, and below all
-    (2.0 ** -120, 2.0 ** -60),
-    (2.0 ** -130, 1.0),         # subnormal themselves
-    (1.0, 1.0),
-])
-@pytest.mark.parametrize("d", [64, 128])
-def test_keys_get_the_nearest_code(dev, d, size, weight, eps):
+def check_keys(dev, d, size, weight, eps):
     """Bit for bit the codes and scales of the values in 64 bits, as for ordinary keys;
     in every third row one value is bf16's largest."""
     w = Writer(dev, 9, 16, 2, 2, d, seed=d)
@@ -51,3 +39,27 @@ def test_keys_get_the_nearest_code(dev, d, size, weight, eps):
     got = w.k_d.cpu().numpy()
     assert (got == w.k.raw).all(), f"{int((got != w.k.raw).sum())} bytes"
     assert (w.v_d.cpu().numpy() == w.v.raw).all()
+    return y
+
+
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+@pytest.mark.parametrize("size,weight", [
+    (2.0 ** 125, 2.0 ** 10),    # products past the largest fp32
+    (2.0 ** 125, 2.0 ** 115),
+    (2.0 ** 20, 2.0 ** 120),
+    (2.0 ** 125, 2.0 ** -90),
+    (2.0 ** -100, 2.0 ** -30),  # below the normal ones, and below all
+    (2.0 ** -120, 2.0 ** -60),
+    (2.0 ** -130, 1.0),         # subnormal themselves
+    (1.0, 1.0),
+])
+@pytest.mark.parametrize("d", [64, 128])
+def test_keys_get_the_nearest_code(dev, d, size, weight, eps):
+    check_keys(dev, d, size, weight, eps)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_keys_past_the_largest_fp32(dev, d):
+    """Finite keys that fp32 does not hold take the largest code under the largest scale."""
+    y = check_keys(dev, d, 1.0, 2.0 ** 127, 1e-6)
+    assert (np.abs(y) > float(np.finfo(np.float32).max)).sum() > 100

@@ -38,10 +38,10 @@ __device__ __forceinline__ uint32_t fp8x4_of(float a, float b, float c, float d,
 }
 
 __device__ __forceinline__ float fp8_scale(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-// Exponent of the smallest scale with which `most` is at most 448 = 1.75 * 2^8.
-__device__ __forceinline__ int fp8_exponent_for(float most) {
+// Exponent of the smallest scale with which most * 2^down is at most 448 = 1.75 * 2^8.
+__device__ __forceinline__ int fp8_exponent_for(float most, int down) {
     const uint32_t b = __float_as_uint(most);
-    return min(max((int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0), kFp8Low), kFp8High);
+    return min(max((int)(b >> 23) - 127 - 8 + down + ((b & 0x7fffffu) > 0x600000u ? 1 : 0), kFp8Low), kFp8High);
 }
 // Whether a block's scale is one that the writer makes; of memory that it has not
 // written, any.

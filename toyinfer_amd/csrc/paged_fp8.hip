@@ -64,6 +64,12 @@ __device__ __forceinline__ float sticky_f32(double x) {
 // 24.8 and 27.0.)  The product of a value and its weight too: 32 bits hold it exactly in
 // their range only, which two bf16 leave at both ends where the norm's result does not.
 // (That costs 38.5 -> 39.0 us of those tokens on another card, and 28.2 -> 29.2.)
+//
+// The results come times 2^-kKeysDown, in fp32: a finite weight's can pass fp32's range
+// and have to be the largest code then, not NaN (they are below 2^133: a row's largest
+// value is at most sqrt(D) times the mean's root), and what 2^-126 cuts off at the other
+// end has the code 0, whose values end at 2^-110 = 2^kFp8Low * 2^-10.
+constexpr int kKeysDown = 16;
 template <int D>
 __device__ __forceinline__ void norm_rope_f64(uint4 xr, uint4 xi, uint4 wr, uint4 wi, const float4 (&rope)[4], float eps,
                                               float (&re)[8], float (&im)[8]) {
@@ -83,7 +89,7 @@ __device__ __forceinline__ void norm_rope_f64(uint4 xr, uint4 xi, uint4 wr, uint
     ss += dpp_f64<kDppXor1>(ss);
     ss += dpp_f64<kDppXor2>(ss);
     if constexpr (D == 128) ss += dpp_f64<kDppRowHalfMirror>(ss);
-    const double inv = rsqrt(ss * (1.0 / D) + (double)eps);
+    const double inv = rsqrt(ss * (1.0 / D) + (double)eps) * (1.0 / (1 << kKeysDown));
 #pragma unroll
     for (int k = 0; k < 8; ++k) asm volatile("" : "+v"(re[k]), "+v"(im[k]));
 #pragma unroll
@@ -135,6 +141,7 @@ __device__ __forceinline__ void write_blocks(const PagedPrologueFp8Args& a, uint
     asm("" : "+s"(from));  // (or the choice is made through scratch memory)
     if (is_k) from = a.k;
     const uint32_t in_page = (1u << a.page_shift) - 1;
+    const int down = is_k ? kKeysDown : 0;
     uint4 wr = make_uint4(0, 0, 0, 0), wi = wr;
     if (is_k) {
         wr = ldg16(a.k_weight + 8 * c);
@@ -208,9 +215,9 @@ __device__ __forceinline__ void write_blocks(const PagedPrologueFp8Args& a, uint
                 written |= lds.bit[local][j];
             }
             const bool opens = (written & 1) || !fp8_scale_valid(was_scale);
-            const int need = fp8_exponent_for(most), was = (int)(__float_as_uint(was_scale) >> 23) - 127;
+            const int need = fp8_exponent_for(most, down), was = (int)(__float_as_uint(was_scale) >> 23) - 127;
             const int e = opens ? need : max(need, was);
-            const float inv = fp8_scale(-e);
+            const float inv = fp8_scale(down - e);
             uint8_t* const codes = page + (uint64_t)head * rows * D;
             uint8_t* const to = codes + row * D + 8 * c;
             *reinterpret_cast<uint2*>(to) = make_uint2(fp8x4_of(re[0], re[1], re[2], re[3], inv),
@@ -227,7 +234,7 @@ __device__ __forceinline__ void write_blocks(const PagedPrologueFp8Args& a, uint
                 const uint4 w = *at;
                 auto again = [&](uint32_t x) __attribute__((always_inline)) {
                     const uint32_t lo = fp8x2_to_bf16<false>(x, was_scale), hi = fp8x2_to_bf16<true>(x, was_scale);
-                    return fp8x4_of(bf16_lo(lo), bf16_hi(lo), bf16_lo(hi), bf16_hi(hi), inv);
+                    return fp8x4_of(bf16_lo(lo), bf16_hi(lo), bf16_lo(hi), bf16_hi(hi), fp8_scale(-e));
                 };
                 *at = make_uint4(again(w.x), again(w.y), again(w.z), again(w.w));
             }
