@@ -730,7 +730,9 @@ def paged_qkv_prologue_fp8(q, k, v, q_norm_weight, k_norm_weight, rope_cos_sin,
                            page_size: int, page_stride: int, num_q_heads: int, num_kv_heads: int,
                            head_dim: int, stream=None) -> None:
     """paged_qkv_prologue_bf16 into 8-bit caches, with a scale for each block of 16
-    rows and head; page_stride in bytes."""
+    rows and head; page_stride in bytes.  Rows are written in order, and tokens of one
+    block are neighbours in slot_mapping, with none between them that lies elsewhere or
+    has no slot (paged_tables_u32 makes them so)."""
     fn = "paged_qkv_prologue_fp8"
     row = num_tokens * head_dim
     bf16, u32, f32 = _types()

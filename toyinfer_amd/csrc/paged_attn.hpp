@@ -63,8 +63,8 @@
 //   streaming, 48 requests of up to 8192 keys (472 MB): 86 us and 5 for the merge;
 //     16 of 32768 118 us, 5.9 TB/s.  Loads alone, without products, waits or scales, are no
 //     faster: 6.5 TB/s in a loop without ends of items;
-//   a prompt of 8192: 525 to 540 us where bf16 takes 517 to 533, 1.02 PFLOP/s; 512
-//     tokens on 7680 keys 82 to 93 (90).
+//   a prompt of 8192: 525 to 540 us where bf16 takes 515 to 533, 1.02 PFLOP/s; 512
+//     tokens on 7680 keys 82 to 93 (on one card 87 and 84).
 #pragma once
 
 #include <math.h>

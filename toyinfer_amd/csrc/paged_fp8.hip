@@ -14,8 +14,11 @@
 // workgroups share a block: no atomics, and the same bytes every time.  A row is
 // in D / 16 lanes, a run's largest value goes over LDS, and nothing is read twice.
 // The copies in and out bound it: 8192 tokens of 32 and 8 heads of 128 move 189 MB
-// in 40 us, 4.7 TB/s (the bf16 prologue, 201 MB, takes 37).  Few tokens wait for a
-// chain of latencies: slots, rows, LDS, codes; 4 us.
+// in 40 us, 4.7 TB/s (the bf16 prologue, 201 MB, takes 37; Q's part has the registers of
+// K's, four waves a SIMD).  Few tokens wait for a chain of latencies: slots, rows, LDS,
+// codes; 4 us.  Where a block grows its other rows follow, each read, rounded and
+// written before the next: 9 to 13 us for 1 to 256 tokens, and of normal values a step of
+// eight requests with eight heads nearly always has such a block.
 //
 // Read.  code * 2^e is exact in bf16.  A thread has eight values of four heads, so
 // that their loads are under way together.  16 requests of up to 8192 tokens, 8 heads
@@ -300,7 +303,8 @@ hipError_t launch_prologue_t(const PagedPrologueFp8Args& a, hipStream_t st) {
     // A token's heads of Q, 64 / (D / 16) to a wave's load: four loads under way, but
     // for so few heads that one has them all.  (One load a wave against four: 8192
     // tokens of 32 heads 44.7 and 40.5 us, of 16 33.9 and 31.2, of 8 26.3 and 27.3;
-    // 1371 tokens of 16 9.4 and 9.6.)
+    // 1371 tokens of 16 9.4 and 9.6.  Loads past a token's heads repeat the last one's:
+    // two of the four with 16 heads of 128.)
     constexpr uint32_t per_load = 64 / (D / 16);
     const bool many = a.hq > per_load;
     const uint32_t q_heads = (many ? 4 : 1) * per_load, q_parts = (a.hq + q_heads - 1) / q_heads;
